@@ -14,6 +14,7 @@ EXPORTS = ("hkv_version", "hkv_error_string", "hkv_last_cuda_error", "hkv_write"
            "hkv_set_option", "hkv_dequant", "hkv_write_rot",
            "hkv_decode_rot", "hkv_write_k8", "hkv_decode_k8", "hkv_dequant_k8",
            "hkv_prefill", "hkv_prefill_scratch_bytes",
+           "hkv_decode_window", "hkv_prefill_window", "hkv_prefill_window_scratch_bytes", "hkv_accumulate_weights", "hkv_evict",
            "hkv_selftest_wait_timeout", "hkv_selftest_prefill_timeout", "hkv_selftest_codec", "hkv_probe_issue_rates")
 
 _lib = None
@@ -79,6 +80,18 @@ def load():
         L.hkv_prefill.argtypes = [vp, i32, vp, vp, vp, vp, C.POINTER(i64), i32, vp, i32, i32, C.POINTER(i32), i32, i32, i32,
                                   i32, i32, f32, f32, vp, i32, i64, vp, C.c_size_t, vp, i32, vp, vp]
         L.hkv_selftest_prefill_timeout.argtypes = L.hkv_prefill.argtypes
+        L.hkv_decode_window.restype = i32
+        L.hkv_decode_window.argtypes = L.hkv_decode.argtypes[:-2] + [vp, i32, i32, i32, vp, vp, vp]
+        L.hkv_prefill_window_scratch_bytes.restype = C.c_size_t
+        L.hkv_prefill_window_scratch_bytes.argtypes = L.hkv_prefill_scratch_bytes.argtypes + [i32, i32]
+        L.hkv_prefill_window.restype = i32
+        L.hkv_prefill_window.argtypes = L.hkv_prefill.argtypes[:22] + [i32, i32, vp] + L.hkv_prefill.argtypes[22:]
+        L.hkv_accumulate_weights.restype = i32
+        L.hkv_accumulate_weights.argtypes = [vp, vp, vp, C.POINTER(i64), i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32, vp, vp,
+                                             vp, i64, i64, i32, i32, i32, vp, i32, vp, vp]
+        L.hkv_evict.restype = i32
+        L.hkv_evict.argtypes = [vp, vp, vp, vp, C.POINTER(i64), i32, vp, i32, vp, i32, i32, i32, i32, vp, i64, i64, i32, i32, i32,
+                                i32, vp, i32, vp, vp, vp, i64, i64, i32, vp]
         L.hkv_selftest_wait_timeout.restype = i32
         L.hkv_selftest_wait_timeout.argtypes = [vp, i64, vp]
         L.hkv_selftest_codec.restype = i32
@@ -102,6 +115,7 @@ class _NoHost:
         return None
 
     decode = prefill = layer_write = layer_decode = write
+    decode_window = prefill_window = accumulate_weights = evict = write
 
 
 def load_host(path):
@@ -129,7 +143,8 @@ def host():
             h = load_host(HOST_PATH)
             h.bind(*[C.cast(f, C.c_void_p).value for f in (
                 L.hkv_write, L.hkv_write_rot, L.hkv_write_k8, L.hkv_decode, L.hkv_decode_rot, L.hkv_decode_k8,
-                L.hkv_prefill_scratch_bytes, L.hkv_prefill)])
+                L.hkv_prefill_scratch_bytes, L.hkv_prefill, L.hkv_decode_window, L.hkv_prefill_window_scratch_bytes,
+                L.hkv_prefill_window, L.hkv_accumulate_weights, L.hkv_evict)])
         except (ImportError, OSError, AttributeError, TypeError) as e:       # (TypeError: it binds another set of entry points)
             warnings.warn(f"{HOST_PATH} does not load, every call takes the slower Python path: {e} (rebuild it with "
                           "`python -m horizon_kernels_b200.build`)", RuntimeWarning, stacklevel=3)

@@ -6,13 +6,15 @@ CUDA runtime alone (linked statically), not on torch; the host module binds it t
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libhkv.so")
 HOST = os.path.join(OUT_DIR, "hkv_host.so")
-SOURCES = ["hkv_write.cu", "hkv_decode.cu", "hkv_dequant.cu", "hkv_prefill.cu", "hkv_probe.cu"]
+SOURCES = ["hkv_write.cu", "hkv_decode.cu", "hkv_dequant.cu", "hkv_prefill.cu", "hkv_weights.cu", "hkv_evict.cu", "hkv_probe.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "-shared", "-cudart", "static"]
 
@@ -41,8 +43,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= src:
         return LIB
     nvcc = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
-    _run([nvcc, *NVCC_FLAGS, *(["-Xptxas", "-v"] if verbose else []), "-o", LIB,
-          *[os.path.join(CSRC, s) for s in SOURCES]], verbose)
+    # one compiler per source, then the link
+    with tempfile.TemporaryDirectory() as tmp, ThreadPoolExecutor(os.cpu_count()) as pool:
+        objs = [os.path.join(tmp, s + ".o") for s in SOURCES]
+        flags = [f for f in NVCC_FLAGS if f not in ("-shared", "-cudart", "static")] + (["-Xptxas", "-v"] if verbose else [])
+        list(pool.map(lambda so: _run([nvcc, *flags, "-c", "-o", so[1], os.path.join(CSRC, so[0])], verbose), zip(SOURCES, objs)))
+        _run([nvcc, *NVCC_FLAGS, "-o", LIB, *objs])
     return LIB
 
 

@@ -118,8 +118,10 @@ struct Smem {
   static constexpr int TOTAL = RING + BARS + MERGE + COARSE + 64;
 };
 
-template <int D, int LAYOUT, int QT = 1>
-__global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) decode_kernel(const DecodeParams p) {
+// WIN: over a sliding window and the first tokens. The units between them are not part of the stream, those at their edges are
+// masked like the last unit of a sequence; the rows' log-sum-exps are stored too when the caller wants them.
+template <int D, int LAYOUT, int QT, bool WIN>
+__device__ __forceinline__ void decode_body(const DecodeParams& p) {
   using Gm = Geo<D, LAYOUT>;
   using Sm = Smem<D, LAYOUT, QT>;
   constexpr int RP = Sm::RP;
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
   const int ngrp = (B + 31) >> 5;
   for (int grp = w; grp < ngrp; grp += TG) {
     const int b = grp * 32 + lane;
-    int u = b < B ? wt(load_req<LOG_UT>(p, b).U) : 0;
+    int u = b < B ? wt(load_req<LOG_UT, WIN>(p, b).U) : 0;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
     if (lane == 0) coarse[grp + 1] = u;
@@ -212,7 +214,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
       if ((long long)coarse[mid] * KVH <= lo) lo_g = mid; else hi_g = mid;
     }
     const int b = lo_g * 32 + lane;
-    const int u = b < B ? wt(load_req<LOG_UT>(p, b).U) : 0;
+    const int u = b < B ? wt(load_req<LOG_UT, WIN>(p, b).U) : 0;
     int incl = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -230,7 +232,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
   int n_units = 0;
   for (int grp = b0 >> 5; grp < ngrp && (long long)coarse[grp] * KVH < hi; ++grp) {
     const int b = grp * 32 + lane;
-    const int U = b < B ? load_req<LOG_UT>(p, b).U : 0, W = wt(U);
+    const int U = b < B ? load_req<LOG_UT, WIN>(p, b).U : 0, W = wt(U);
     int incl = W;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -262,13 +264,13 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
       wk.seq0 = end_h;
       if (++wk.h == KVH) {
         wk.h = 0;
-        do { wk.r = load_req<LOG_UT>(p, ++wk.b); } while (wk.r.U == 0);
+        do { wk.r = load_req<LOG_UT, WIN>(p, ++wk.b); } while (wk.r.U == 0);
       }
     }
   };
   Walker cw;
   cw.b = b0;
-  cw.r = load_req<LOG_UT>(p, b0);
+  cw.r = load_req<LOG_UT, WIN>(p, b0);
   cw.h = (int)((lo - (long long)base0 * KVH) / wt(cw.r.U));
   cw.seq0 = (long long)base0 * KVH + (long long)cw.h * wt(cw.r.U);
 
@@ -291,6 +293,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
                 VR11 = Gm::tok(9) - Gm::tok(0);                           // t01 - t00, t10 - t00, t11 - t00 (for every c)
 
   int f_b = cw.b, f_h = cw.h, f_U = cw.r.U, f_L = cw.r.L;
+  int f_off = 0;                                    // WIN: how much further the cursor's unit lies in the context
   int f_blk = w + (int)max(0ll, lo - cw.seq0 - PC);  // unit (inside the cursor's sequence) to fetch next; may run past
   int f_fast_end = 0;                               // units below this bound take the fast path
   int f_idx = 0, pg = 0;                            // page ids of the warp's next 32 blocks of the sequence, one per lane
@@ -309,7 +312,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
         if (++f_h == KVH) {
           f_h = 0;
           ReqInfo r;
-          do { r = load_req<LOG_UT>(p, ++f_b); } while (r.U == 0);
+          do { r = load_req<LOG_UT, WIN>(p, ++f_b); } while (r.U == 0);
           f_U = r.U;
           f_L = r.L;
         }
@@ -327,10 +330,19 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
     }
     // refill the page window from the current unit: lane j holds the page of 16-token block j % UB of the warp's
     // (j / UB)-th next unit
-    const int tok_l = (f_blk + (lane / UB) * TG) * UT + (lane % UB) * 16;
-    pg = tok_l < f_L ? __ldg(f_bt + (tok_l >> lps)) : 0;
+    if constexpr (WIN) {                            // (-1: a block that no row sees, whose page may be gone)
+      const ReqInfo r = load_req<LOG_UT, WIN>(p, f_b);
+      const bool sink = f_blk < r.su;
+      f_off = sink ? 0 : r.skip;
+      const int tok_l = (f_blk + f_off + (lane / UB) * TG) * UT + (lane % UB) * 16;
+      pg = tok_l < f_L && (tok_l + 16 > window_from(p, r.L, r.ql) || tok_l < p.sinks) ? __ldg(f_bt + (tok_l >> lps)) : -1;
+      f_fast_end = min(sink ? r.su : f_U, f_blk + (32 / UB) * TG);
+    } else {
+      const int tok_l = (f_blk + (lane / UB) * TG) * UT + (lane % UB) * 16;
+      pg = tok_l < f_L ? __ldg(f_bt + (tok_l >> lps)) : 0;
+      f_fast_end = min(f_U, f_blk + (32 / UB) * TG);
+    }
     f_idx = 0;
-    f_fast_end = min(f_U, f_blk + (32 / UB) * TG);
     return false;
   };
   // fetches this warp's next unit into the stage at shared address st, completion on the barrier at address bar
@@ -342,8 +354,15 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
 #pragma unroll
       for (int bi = 0; bi < UB; ++bi) page[bi] = __shfl_sync(0xffffffffu, pg, f_idx + bi);
       f_idx += UB;
-      const int tok0 = f_blk * UT;
+      const int tok0 = (f_blk + f_off) * UT;
       const int nb = min(UB, (f_L - tok0 + 15) >> 4);          // 16-token blocks of this unit that exist
+      auto there = [&](int bi) { return WIN ? page[bi] >= 0 : bi < nb; };
+      int nv = nb;                                             // .. and that some row sees
+      if constexpr (WIN) {
+        nv = 0;
+#pragma unroll
+        for (int bi = 0; bi < UB; ++bi) nv += page[bi] >= 0;
+      }
       if (Gm::ROWCOPY) {
         // lane -> (side, token row) of every 16-token block: SLOT bytes from its own address, in 8- or 16-byte pieces
         constexpr int CB = D == 128 ? 8 : 16;
@@ -351,7 +370,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
         const uint8_t* base = side ? f_v : f_k;
 #pragma unroll
         for (int bi = 0; bi < UB; ++bi) {
-          if (bi < nb) {
+          if (there(bi)) {
             const unsigned pos0 = (unsigned)(tok0 + 16 * bi) & (unsigned)(p.PS - 1);
             const uint8_t* src = base + (unsigned long long)(unsigned)page[bi] * p.dsp +
                                  (unsigned long long)(pos0 + row) * p.dst;
@@ -362,10 +381,10 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
         }
         cp_async_mbar_arrive_noinc(bar);                        // arrives once this lane's copies have landed
       } else if (elect_one()) {                                 // one lane arms the barrier and issues the copies
-        mbar_expect_tx_u32(bar, nb * (Gm::STAGE / UB));
+        mbar_expect_tx_u32(bar, nv * (Gm::STAGE / UB));
 #pragma unroll
         for (int bi = 0; bi < UB; ++bi) {
-          if (bi < nb) {
+          if (there(bi)) {
             const unsigned pos0 = (unsigned)(tok0 + 16 * bi) & (unsigned)(p.PS - 1);
             const unsigned long long doff = (unsigned long long)(unsigned)page[bi] * p.dsp + pos0 * (unsigned)Gm::SD_ROW;
             if (LAYOUT == 2) {
@@ -560,7 +579,9 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
         lim0[q] = ra < R ? L - ql + (p.row0 + ra) / G + 1 : L;
         lim1[q] = rb < R ? L - ql + (p.row0 + rb) / G + 1 : L;
       }
-      const int blk_mask = (L - ql + p.row0 / G + 1) >> LOG_UT;   // units below this one are visible to every row in full
+      const int blk_mask = ((L - ql + p.row0 / G + 1) >> LOG_UT) - (WIN ? cw.r.skip : 0);   // units below this one are visible to every row in full
+      // (WIN: but for those from the last whole unit of sinks to the first of the last row's window)
+      const int win_end = WIN && p.window > 0 ? ((L - ql + (p.row0 + R - 1) / G + UT - p.window) >> LOG_UT) - cw.r.skip : 0;
       float mneg0[QT], mneg1[QT], thr0[QT], thr1[QT];   // p = 2^(s * sc + mneg)
 #pragma unroll
       for (int q = 0; q < QT; ++q) {
@@ -681,11 +702,12 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
       // every block; x[bi] = {(r0, row 2c), (r0, row 2c+1), (r1, row 2c), (r1, row 2c+1)}. Leaves P^T as the B
       // operand of the second product in pb.
       auto softmax = [&](const uint32_t st, const int blk, const int bb, float (&x)[QT][BB][4], uint32_t (&pb)[QT][BB][2]) {
-        const int tbase = blk * UT;
-        if (blk >= blk_mask) {                        // warp-uniform: only the last unit(s) of a sequence
+        const int tbase = (WIN && blk >= cw.r.su ? blk + cw.r.skip : blk) * UT;
+        const bool masked = WIN ? blk >= blk_mask || (blk < win_end && blk >= p.sinks >> LOG_UT) : blk >= blk_mask;
+        if (masked) {                                 // warp-uniform: only the last unit(s) of a sequence
           // rows past the context hold arbitrary bytes: their scores become -inf below, and their value scales are
           // set to zero here, in shared memory, so that the value product needs no masking code
-          if (bb == 0 && lane < UT && tbase + lane >= L) {
+          if (bb == 0 && lane < UT && (tbase + lane >= L || (WIN && tbase + lane < window_from(p, L, ql) && tbase + lane >= p.sinks))) {
             const uint32_t a = st + Gm::V_BASE + Gm::SF_BASE + lane * Gm::SF_ROW;
 #pragma unroll
             for (int i = 0; i < Gm::SS; i += 8) sts64_zero(a + i);
@@ -698,10 +720,13 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
 #pragma unroll
             for (int bi = 0; bi < BB; ++bi) {
               const int ta = tbase + 16 * (bb + bi) + r0, tb = tbase + 16 * (bb + bi) + r1;
-              x[q][bi][0] = ta < lim0[q] ? x[q][bi][0] : ninf;
-              x[q][bi][1] = ta < lim1[q] ? x[q][bi][1] : ninf;
-              x[q][bi][2] = tb < lim0[q] ? x[q][bi][2] : ninf;
-              x[q][bi][3] = tb < lim1[q] ? x[q][bi][3] : ninf;
+              auto sees = [&](int tok, int lim) {
+                return tok < lim && (!WIN || p.window == 0 || tok >= lim - p.window || tok < p.sinks);
+              };
+              x[q][bi][0] = sees(ta, lim0[q]) ? x[q][bi][0] : ninf;
+              x[q][bi][1] = sees(ta, lim1[q]) ? x[q][bi][1] : ninf;
+              x[q][bi][2] = sees(tb, lim0[q]) ? x[q][bi][2] : ninf;
+              x[q][bi][3] = sees(tb, lim1[q]) ? x[q][bi][3] : ninf;
             }
         }
         // the running max moves only when some score exceeds it by more than TAU (then P stays below 2^TAU, inside
@@ -874,9 +899,10 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
           if (complete) {
             const int t = (p.row0 + row) / G, gq = p.row0 + row - t * G;
             dst_o = p.out + ((long long)(q0 + t) * (KVH * G) + h * G + gq) * D;
+            if (WIN && p.lse && tid == rl * tpr) p.lse[(long long)(q0 + t) * (KVH * G) + h * G + gq] = row_lse(mx, den);
           } else {
             dst_p = opart_ws + ((size_t)slot_id * RP + row) * D;
-            if (tid == rl * tpr) lse_ws[slot_id * RP + row] = den > 0.0f ? log2f(den) + mx : -__int_as_float(0x7f800000);
+            if (tid == rl * tpr) lse_ws[slot_id * RP + row] = (WIN ? den != 0.0f : den > 0.0f) ? log2f(den) + mx : -__int_as_float(0x7f800000);
           }
           for (int ch = (tid - rl * tpr) * 2; ch < D; ch += 2 * tpr) {
             float n0 = 0.0f, n1 = 0.0f;
@@ -924,7 +950,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
       const int first_slot = 2 * first + ((long long)first * per >= sq.seq0 ? 0 : 1);
       const Group gr = group_of(part, first, last);
       MergeOut o{p.out + ((long long)sq.q0 * (KVH * p.G) + sq.h * p.G) * D, (long long)KVH * p.G * D, p.v_scale, p.row0, p.G,
-                 nullptr, nullptr};
+                 nullptr, nullptr, WIN && p.lse ? p.lse + (long long)sq.q0 * (KVH * p.G) + sq.h * p.G : nullptr, KVH * p.G};
       Pieces pc{lse_ws, opart_ws, first_slot, first, 1, last - first + 1};
       if (last - first + 1 > kGroupFrom) {
         // the group's pieces into the partial of its first one; then, if that was the last group, the groups
@@ -933,7 +959,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
         og.row0 = nullptr;
         og.part = opart_ws + (size_t)slot0 * RP * D;
         og.lse = lse_ws + slot0 * RP;
-        merge_pieces<D, RP, NTHREADS>(Pieces{lse_ws, opart_ws, slot0, gr.first, 1, gr.last - gr.first + 1}, sq.R, og, obuf,
+        merge_pieces<D, RP, NTHREADS, WIN>(Pieces{lse_ws, opart_ws, slot0, gr.first, 1, gr.last - gr.first + 1}, sq.R, og, obuf,
                                       Sm::MERGE / 4 - RP);
         __threadfence();
         __syncthreads();
@@ -944,7 +970,7 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
         pc.step = kGroup;
         pc.n = (last - first) / kGroup + 1;
       }
-      merge_pieces<D, RP, NTHREADS>(pc, sq.R, o, obuf, Sm::MERGE / 4 - RP);
+      merge_pieces<D, RP, NTHREADS, WIN>(pc, sq.R, o, obuf, Sm::MERGE / 4 - RP);
     }
   }
 
@@ -958,6 +984,15 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
   }
 }
 
+template <int D, int LAYOUT, int QT = 1>
+__global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) decode_kernel(const DecodeParams p) {
+  decode_body<D, LAYOUT, QT, false>(p);
+}
+template <int D, int LAYOUT, int QT = 1>
+__global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) window_kernel(const DecodeParams p) {
+  decode_body<D, LAYOUT, QT, true>(p);
+}
+
 // ----------------------------------------------------------------------------------------------------- host side
 int record_cuda(cudaError_t e);
 
@@ -965,6 +1000,7 @@ struct DeviceInfo {
   int sms = 0;
   int ctas_per_sm[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};    // [D == 256][LAYOUT]
   int ctas_two_tiles[2] = {0, 0};                    // [D == 256] decode_kernel<D, 0, 2>: sixteen query rows per pass
+  int win_per_sm[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, win_two_tiles[2] = {0, 0};   // the same of window_kernel, at most as many
   std::atomic<bool> ready{false};                    // set (release) after the fields above, under g_setup_mutex
 };
 static DeviceInfo g_dev[64];
@@ -972,11 +1008,17 @@ static std::mutex g_setup_mutex;                     // serialises the once-per-
 static std::atomic<int> g_early_metadata{0};
 
 template <int D, int LAYOUT, int QT = 1>
-static cudaError_t setup_variant(int& ctas) {
-  auto k = decode_kernel<D, LAYOUT, QT>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D, LAYOUT, QT>::TOTAL);
-  if (e != cudaSuccess) return e;
-  return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, k, NTHREADS, Smem<D, LAYOUT, QT>::TOTAL);
+static cudaError_t setup_variant(int& ctas, int& win) {
+  void (*const ks[2])(const DecodeParams) = {decode_kernel<D, LAYOUT, QT>, window_kernel<D, LAYOUT, QT>};
+  int n[2] = {0, 0};
+  for (int i = 0; i < 2; ++i) {
+    cudaError_t e = cudaFuncSetAttribute(ks[i], cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D, LAYOUT, QT>::TOTAL);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n[i], ks[i], NTHREADS, Smem<D, LAYOUT, QT>::TOTAL);
+    if (e != cudaSuccess) return e;
+  }
+  ctas = n[0];
+  win = std::min(n[0], n[1]);                        // (the workspace is sized by the former)
+  return cudaSuccess;
 }
 
 static int device_info(DeviceInfo** out) {
@@ -990,15 +1032,15 @@ static int device_info(DeviceInfo** out) {
     if (!di.ready.load(std::memory_order_relaxed)) {
       e = cudaDeviceGetAttribute(&di.sms, cudaDevAttrMultiProcessorCount, dev);
       if (e != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<128, 0>(di.ctas_per_sm[0][0])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<128, 1>(di.ctas_per_sm[0][1])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<256, 0>(di.ctas_per_sm[1][0])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<256, 1>(di.ctas_per_sm[1][1])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<256, 2>(di.ctas_per_sm[1][2])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<128, 3>(di.ctas_per_sm[0][3])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<256, 3>(di.ctas_per_sm[1][3])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<128, 0, 2>(di.ctas_two_tiles[0])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<256, 0, 2>(di.ctas_two_tiles[1])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<128, 0>(di.ctas_per_sm[0][0], di.win_per_sm[0][0])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<128, 1>(di.ctas_per_sm[0][1], di.win_per_sm[0][1])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<256, 0>(di.ctas_per_sm[1][0], di.win_per_sm[1][0])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<256, 1>(di.ctas_per_sm[1][1], di.win_per_sm[1][1])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<256, 2>(di.ctas_per_sm[1][2], di.win_per_sm[1][2])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<128, 3>(di.ctas_per_sm[0][3], di.win_per_sm[0][3])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<256, 3>(di.ctas_per_sm[1][3], di.win_per_sm[1][3])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<128, 0, 2>(di.ctas_two_tiles[0], di.win_two_tiles[0])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<256, 0, 2>(di.ctas_two_tiles[1], di.win_two_tiles[1])) != cudaSuccess) return record_cuda(e);
       di.ready.store(true, std::memory_order_release);
     }
   }
@@ -1026,11 +1068,15 @@ extern "C" size_t hkv_decode_workspace_bytes(int B, int KVH, int G, int D, int q
   return need;
 }
 
+struct Window {                      // of hkv_decode_window
+  int window, sinks;
+  float* lse;
+};
 static int decode_impl(const void* q, const void* kd, const void* ksf, const void* vd, const void* vsf,
                        const int64_t strides[6], int PS, const int32_t* block_tables, int MP, const int32_t* seq_lens,
                        const int32_t* query_start_loc, int B, int KVH, int G, int D, int qlmax, float sm_scale,
                        float v_scale, const float* gk, const float* gv, void* workspace, size_t workspace_bytes,
-                       int splits, const float* signs, int k8, void* out, void* stream) {
+                       int splits, const float* signs, int k8, void* out, void* stream, const Window* win = nullptr) {
   using namespace hkv;
   if (B < 0 || MP < 0) return HKV_ERR_RANGE;
   if (B == 0) return HKV_OK;
@@ -1082,16 +1128,18 @@ static int decode_impl(const void* q, const void* kd, const void* ksf, const voi
   int rc = device_info(&di);
   if (rc != HKV_OK) return rc;
   // head-major slot pages, more than 8 query rows per kv head: the two-tile kernel serves 16 rows per pass
-  bool two = layout == 0 && G * qlmax > RPAD && di->ctas_two_tiles[D == 256] > 0;
+  const int(&per_sm)[2][4] = win ? di->win_per_sm : di->ctas_per_sm;
+  const int(&two_tiles)[2] = win ? di->win_two_tiles : di->ctas_two_tiles;
+  bool two = layout == 0 && G * qlmax > RPAD && two_tiles[D == 256] > 0;
   auto parts_of = [&](int cps) {
     long long n = std::min<long long>((long long)di->sms * cps, kMaxParts);
     if (splits > 0) n = std::min<long long>(n, (long long)B * KVH * splits);
     return n < 1 ? 1 : n;
   };
   // (at head_dim 256 its partials may not fit a workspace that is enough for eight rows per pass, e.g. the built-in one)
-  if (two && D == 256 && workspace_bytes < WorkspaceLayout((int)parts_of(di->ctas_two_tiles[1]), 2 * RPAD, D).total) two = false;
+  if (two && D == 256 && workspace_bytes < WorkspaceLayout((int)parts_of(two_tiles[1]), 2 * RPAD, D).total) two = false;
   const int rows_per_pass = two ? 2 * RPAD : RPAD;
-  const int cps = two ? di->ctas_two_tiles[D == 256] : di->ctas_per_sm[D == 256][layout];
+  const int cps = two ? two_tiles[D == 256] : per_sm[D == 256][layout];
   if (cps < 1) return HKV_ERR_UNSUPPORTED;
   const long long n_parts = parts_of(cps);
   if (workspace_bytes < WorkspaceLayout((int)n_parts, rows_per_pass, D).total) return HKV_ERR_WORKSPACE;
@@ -1111,9 +1159,16 @@ static int decode_impl(const void* q, const void* kd, const void* ksf, const voi
   p.rot_scale = (float)(1.0 / sqrt((double)D));
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.v_scale = v_scale;
+  p.window = win ? win->window : 0;
+  p.sinks = win ? win->sinks : 0;
+  p.lse = win ? win->lse : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
   const unsigned grid = (unsigned)n_parts;
   void (*k)(const DecodeParams) =
+      win ? (two ? (D == 128 ? window_kernel<128, 0, 2> : window_kernel<256, 0, 2>) :
+             D == 128 ? (layout == 0 ? window_kernel<128, 0> : layout == 1 ? window_kernel<128, 1> : window_kernel<128, 3>)
+                      : (layout == 0 ? window_kernel<256, 0> : layout == 1 ? window_kernel<256, 1>
+                         : layout == 2 ? window_kernel<256, 2> : window_kernel<256, 3>)) :
       two ? (D == 128 ? decode_kernel<128, 0, 2> : decode_kernel<256, 0, 2>) :
       D == 128 ? (layout == 0 ? decode_kernel<128, 0> : layout == 1 ? decode_kernel<128, 1> : decode_kernel<128, 3>)
                : (layout == 0 ? decode_kernel<256, 0> : layout == 1 ? decode_kernel<256, 1>
@@ -1160,6 +1215,21 @@ extern "C" int hkv_decode_k8(const void* q, const void* kd, const void* vd, cons
                              int splits, void* out, void* stream) {
   return decode_impl(q, kd, kd, vd, vsf, strides, PS, block_tables, MP, seq_lens, query_start_loc, B, KVH, G, D, qlmax,
                      sm_scale, v_scale, gk, gv, workspace, workspace_bytes, splits, nullptr, 1, out, stream);
+}
+
+extern "C" int hkv_decode_window(const void* q, const void* kd, const void* ksf, const void* vd, const void* vsf,
+                                 const int64_t strides[6], int PS, const int32_t* block_tables, int MP, const int32_t* seq_lens,
+                                 const int32_t* query_start_loc, int B, int KVH, int G, int D, int qlmax, float sm_scale,
+                                 float v_scale, const float* gk, const float* gv, void* workspace, size_t workspace_bytes,
+                                 int splits, const float* signs, int k8, int window, int sinks, float* lse, void* out,
+                                 void* stream) {
+  if (window < 0 || sinks < 0) return HKV_ERR_RANGE;
+  if ((long long)window >= (long long)MP * PS) window = 0;      // everything is seen
+  if (window > (1 << 30)) return HKV_ERR_RANGE;
+  if ((uintptr_t)lse & 3) return HKV_ERR_ALIGN;
+  const Window w{window, sinks, lse};
+  return decode_impl(q, kd, ksf, vd, vsf, strides, PS, block_tables, MP, seq_lens, query_start_loc, B, KVH, G, D, qlmax,
+                     sm_scale, v_scale, gk, gv, workspace, workspace_bytes, splits, signs, k8, out, stream, &w);
 }
 
 extern "C" int hkv_combine(const void* workspace, size_t workspace_bytes, const int32_t* query_start_loc, int B,

@@ -35,13 +35,21 @@ struct DecodeParams {
   int max_len;                                       // MP * PS, capped at INT_MAX
   int early_meta;                                    // seq_lens / query_start_loc are read before the launch dependency
   float scale_log2, v_scale;
+  int window, sinks;                                 // window_kernel: a row at position x sees the keys j <= x with j > x - window or
+  float* lse;                                        // j < sinks (window 0: all j <= x); the rows' log-sum-exps, or null
 };
 
 // one request as the unit stream sees it; all fields are warp-uniform
 struct ReqInfo {
   int U, L, ql, q0;                                    // units per kv head, context length, query tokens, first query row
+  int su, skip;                                        // WIN: units from su on lie `skip` units further in the context
 };
-template <int LOG_UT>
+// first token of the window of the pass's first row (WIN)
+__device__ __forceinline__ int window_from(const DecodeParams& p, int L, int ql) {
+  return p.window > 0 ? max(0, L - ql + p.row0 / p.G + 1 - p.window) : 0;
+}
+// WIN: the units that hold no visible token, between the sinks and the window, are left out of the stream
+template <int LOG_UT, bool WIN = false>
 __device__ __forceinline__ ReqInfo load_req(const DecodeParams& p, int b) {
   ReqInfo r;
   r.q0 = __ldg(p.qsl + b);
@@ -51,6 +59,13 @@ __device__ __forceinline__ ReqInfo load_req(const DecodeParams& p, int b) {
   // (a length beyond the block table's reach is cut there, so that bad metadata can never read past a table row)
   r.L = ql > 0 ? min(max(__ldg(p.seq_lens + b), 0), p.max_len) : 0;
   r.U = ql > 0 ? max(1, (r.L + (1 << LOG_UT) - 1) >> LOG_UT) : 0;
+  r.su = r.skip = 0;
+  if constexpr (WIN) {
+    const int lo = window_from(p, r.L, ql);
+    r.su = (min(lo, p.sinks) + (1 << LOG_UT) - 1) >> LOG_UT;
+    r.skip = max(0, (lo >> LOG_UT) - r.su);
+    r.U -= r.skip;                                     // (the window holds a token when the context does)
+  }
   return r;
 }
 
@@ -87,7 +102,18 @@ struct MergeOut {
   int first_row, G;                                  // row r of the pass is row first_row + r of the group
   float* part;
   float* lse;
+  float* lse_out;                                    // LSE: the log-sum-exp of output row 0, or null; tokens of a row are lse_stride apart
+  int lse_stride;
 };
+constexpr float kLn2 = 0.6931471805599453f;
+// log2 of a sum of weights relative to 2^m, as a natural log-sum-exp; -inf for a row that sees no key
+__device__ __forceinline__ float row_lse(float m, float total) {
+  return total == 0.0f ? -__int_as_float(0x7f800000) : (m + log2f(total)) * kLn2;
+}
+__device__ __forceinline__ void store_lse(const MergeOut& o, int row, float m, float total) {
+  const int t = (o.first_row + row) / o.G, gq = o.first_row + row - t * o.G;
+  o.lse_out[(long long)t * o.lse_stride + gq] = row_lse(m, total);
+}
 template <int D>
 __device__ __forceinline__ void merge_store(const MergeOut& o, int row, int ch, float4 a, float total) {
   const float inv = total > 0.0f ? (o.row0 ? o.v_scale : 1.0f) / total : 0.0f;
@@ -102,7 +128,7 @@ __device__ __forceinline__ void merge_store(const MergeOut& o, int row, int ch, 
   }
 }
 // sm: RP + cap floats of shared memory
-template <int D, int RP, int NT>
+template <int D, int RP, int NT, bool LSE = false>
 __device__ __forceinline__ void merge_pieces(const Pieces& pc, int R, const MergeOut& o, float* sm, int cap) {
   constexpr int C4 = D / 4;                          // threads of a row, four channels each
   // (six in the sixteen-row kernel at head_dim 256, whose registers are the tightest: with eight it takes 255 and spills. 96
@@ -151,6 +177,7 @@ __device__ __forceinline__ void merge_pieces(const Pieces& pc, int R, const Merg
           fma4(a, v[it][i], w);
         }
         merge_store<D>(o, row, ch, a, tot);
+        if (LSE && o.lse_out && ch == 0) store_lse(o, row, m, tot);
       }
     }
     return;
@@ -181,7 +208,8 @@ __device__ __forceinline__ void merge_pieces(const Pieces& pc, int R, const Merg
       for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
       if (lane == 0) {
         sum[r] = s;
-        if (!o.row0) o.lse[rb + r] = s > 0.0f ? m + log2f(s) : ninf;
+        if (!o.row0) o.lse[rb + r] = (LSE ? s != 0.0f : s > 0.0f) ? m + log2f(s) : ninf;
+        if (LSE && o.row0 && o.lse_out) store_lse(o, rb + r, m, s);
       }
     }
     __syncthreads();

@@ -1,5 +1,5 @@
-// Native side of kernels.write, kernels.decode_ragged and kernels.prefill, and of the backend's cache update and decode: takes
-// the callers' Python arguments as they are, checks them and calls the C ABI (include/hkv.h). What the wrappers do per call in
+// Native side of kernels.write, kernels.decode_ragged, kernels.prefill, their window forms, kernels.accumulate_weights and
+// kernels.evict, and of the backend's cache update and decode: takes the callers' Python arguments as they are, checks them and calls the C ABI (include/hkv.h). What the wrappers do per call in
 // Python (about forty attribute reads and checks, a device context, the conversion of 25 ctypes arguments) costs 20 to 25
 // microseconds, longer than a small decode step runs on the GPU; here it costs two.
 //
@@ -14,6 +14,8 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "../../include/hkv.h"
@@ -29,6 +31,11 @@ struct Abi {                       // entry points of the loaded libhkv.so, hand
   decltype(&hkv_decode_k8) decode_k8 = nullptr;
   decltype(&hkv_prefill_scratch_bytes) prefill_scratch_bytes = nullptr;
   decltype(&hkv_prefill) prefill = nullptr;
+  decltype(&hkv_decode_window) decode_window = nullptr;
+  decltype(&hkv_prefill_window_scratch_bytes) prefill_window_scratch_bytes = nullptr;
+  decltype(&hkv_prefill_window) prefill_window = nullptr;
+  decltype(&hkv_accumulate_weights) accumulate_weights = nullptr;
+  decltype(&hkv_evict) evict = nullptr;
 } abi;
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -88,6 +95,33 @@ bool sign_vector(PyObject* o, int64_t D, int dev, const float** p) {
   return true;
 }
 
+// a sliding window, the tokens that stay visible before it, and where the log-sum-exps go
+struct Window {
+  int window, sinks;
+  float* lse;
+};
+bool lse_rows(const at::Tensor* t, int64_t NT, int64_t HQ, int dev) {
+  return t && on(*t, dev) && t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(0) >= NT && t->size(1) == HQ && t->is_contiguous();
+}
+bool window_of(PyObject* window, PyObject* sinks, PyObject* lse, int64_t NT, int64_t HQ, int dev, Window* w) {
+  long long a, b;
+  if (!integer(window, &a) || !integer(sinks, &b) || a < 0 || b < 0 || a > INT32_MAX || b > INT32_MAX) return false;
+  w->window = (int)a;
+  w->sinks = (int)b;
+  w->lse = nullptr;
+  if (lse == Py_None) return true;
+  const at::Tensor* t = tensor(lse);
+  if (!lse_rows(t, NT, HQ, dev)) return false;
+  w->lse = static_cast<float*>(t->data_ptr());
+  return true;
+}
+// (B, KVH, W) fp32 rows that do not overlap
+bool weight_rows(const at::Tensor* t, int64_t B, int64_t KVH, int dev) {
+  if (!t || !on(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 3 || t->size(0) != B || t->size(1) != KVH || t->size(2) > INT32_MAX)
+    return false;
+  return (t->stride(2) == 1 || t->size(2) <= 1) && (t->stride(1) > 0 || KVH <= 1) && (t->stride(0) > 0 || B <= 1);
+}
+
 // The launches behind the checks. Cache parts and strides as in include/hkv.h.
 struct Rows {                      // new keys and values
   const void *k, *v;
@@ -114,7 +148,7 @@ PyObject* run_write(const Rows& r, const Cache& c, int PS, const at::Tensor& slo
 }
 PyObject* run_decode(const void* q, const Cache& c, int PS, const at::Tensor& bt, const at::Tensor& lens, const at::Tensor& qsl, int64_t HQ,
                      int64_t D, double s1, double s2, const at::Tensor& gk, const at::Tensor& gv, int qlmax, void* out,
-                     const at::Tensor& ws, int splits, const float* signs, bool k8, int dev) {
+                     const at::Tensor& ws, int splits, const float* signs, bool k8, int dev, const Window* win = nullptr) {
   const int32_t *btp = static_cast<const int32_t*>(bt.data_ptr()), *lp = static_cast<const int32_t*>(lens.data_ptr()),
                 *sp = static_cast<const int32_t*>(qsl.data_ptr());
   const float *gkp = static_cast<const float*>(gk.data_ptr()), *gvp = static_cast<const float*>(gv.data_ptr());
@@ -124,7 +158,10 @@ PyObject* run_decode(const void* q, const Cache& c, int PS, const at::Tensor& bt
   void* st = c10::cuda::getCurrentCUDAStream(dev).stream();
   int rc;
   Py_BEGIN_ALLOW_THREADS
-  if (k8)
+  if (win)
+    rc = abi.decode_window(q, c.part[0], c.part[1], c.part[2], c.part[3], c.strides, PS, btp, MP, lp, sp, B, KVH, G, (int)D, qlmax,
+                           (float)s1, (float)s2, gkp, gvp, wp, wsb, splits, signs, k8, win->window, win->sinks, win->lse, out, st);
+  else if (k8)
     rc = abi.decode_k8(q, c.part[0], c.part[2], c.part[3], c.strides, PS, btp, MP, lp, sp, B, KVH, G, (int)D, qlmax, (float)s1,
                        (float)s2, gkp, gvp, wp, wsb, splits, out, st);
   else if (signs)
@@ -190,10 +227,11 @@ PyObject* write(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // decode(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, bmm2_scale, gk, gv, qlmax, out,
-//        workspace, splits, signs, k8)
-PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+//        workspace, splits, signs, k8); decode_window: .., window, sinks, lse
+template <bool WIN>
+PyObject* decode_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
   try {
-    if (n != 17 || !abi.decode) Py_RETURN_NONE;
+    if (n != (WIN ? 20 : 17) || !abi.decode) Py_RETURN_NONE;
     const at::Tensor *q = tensor(a[0]), *bt = tensor(a[4]), *lens = tensor(a[5]), *qsl = tensor(a[6]), *gk = tensor(a[9]),
                      *gv = tensor(a[10]), *out = tensor(a[12]), *ws = tensor(a[13]);
     if (!q || !bt || !lens || !qsl || !gk || !out || !ws || !q->is_cuda() || gk->dim() != 1) Py_RETURN_NONE;
@@ -218,8 +256,111 @@ PyObject* decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (KVH < 1 || HQ % KVH || B > INT32_MAX || MP > INT32_MAX || HQ > INT32_MAX || D > INT32_MAX || !scales(gk, gv, KVH, dev) ||
         !sign_vector(a[15], D, dev, &signs) || (k8 && signs) || !cache_of(a[1], a[2], dev, &c))
       Py_RETURN_NONE;
+    Window w;
+    if (WIN && !window_of(a[17], a[18], a[19], q->size(0), HQ, dev, &w)) Py_RETURN_NONE;
     return run_decode(q->data_ptr(), c, (int)PS, *bt, *lens, *qsl, HQ, D, s1, s2, *gk, *gv, (int)qlmax, out->data_ptr(), *ws, (int)splits, signs,
-                      k8, dev);
+                      k8, dev, WIN ? &w : nullptr);
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// accumulate_weights(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, gk, qlmax, lse, weights, window,
+//                    sinks, signs, k8, workspace)
+PyObject* accumulate_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  try {
+    if (n != 17 || !abi.accumulate_weights) Py_RETURN_NONE;
+    const at::Tensor *q = tensor(a[0]), *bt = tensor(a[4]), *lens = tensor(a[5]), *qsl = tensor(a[6]), *gk = tensor(a[8]),
+                     *wt = tensor(a[11]), *ws = a[16] == Py_None ? nullptr : tensor(a[16]);
+    if (!q || !bt || !lens || !qsl || !gk || !wt || (!ws && a[16] != Py_None) || !q->is_cuda() || gk->dim() != 1) Py_RETURN_NONE;
+    const int dev = q->device().index();
+    long long PS, qlmax;
+    double s1;
+    bool k8;
+    const float* signs;
+    Cache c;
+    Window w;
+    if (dev != c10::cuda::current_device() || !integer(a[3], &PS) || PS != (int)PS || !number(a[7], &s1) || !integer(a[9], &qlmax) ||
+        qlmax != (int)qlmax || !boolean(a[15], &k8) || q->scalar_type() != at::kBFloat16 || q->dim() != 3 || !q->is_contiguous() ||
+        bt->dim() != 2 || lens->dim() != 1 || qsl->dim() != 1 || lens->size(0) != bt->size(0) || qsl->size(0) != bt->size(0) + 1 ||
+        (ws && (!on(*ws, dev) || ws->nbytes() < 64)))
+      Py_RETURN_NONE;
+    for (const at::Tensor* t : {bt, lens, qsl})
+      if (!on(*t, dev) || t->scalar_type() != at::kInt || !t->is_contiguous()) Py_RETURN_NONE;
+    const int64_t B = bt->size(0), MP = bt->size(1), KVH = gk->size(0), HQ = q->size(1), D = q->size(2);
+    if (KVH < 1 || HQ % KVH || B > INT32_MAX || MP > INT32_MAX || HQ > INT32_MAX || D > INT32_MAX || !scales(gk, gk, KVH, dev) ||
+        !sign_vector(a[14], D, dev, &signs) || (k8 && signs) || !cache_of(a[1], a[2], dev, &c) || a[10] == Py_None ||
+        !window_of(a[12], a[13], a[10], q->size(0), HQ, dev, &w) || !weight_rows(wt, B, KVH, dev))
+      Py_RETURN_NONE;
+    const void* qp = q->data_ptr();
+    const int32_t *btp = static_cast<const int32_t*>(bt->data_ptr()), *lp = static_cast<const int32_t*>(lens->data_ptr()),
+                  *sp = static_cast<const int32_t*>(qsl->data_ptr());
+    const float* gkp = static_cast<const float*>(gk->data_ptr());
+    float* wtp = static_cast<float*>(wt->data_ptr());
+    const int64_t wb = wt->stride(0), wh = wt->stride(1);
+    const int W = (int)wt->size(2);
+    void *wp = ws ? ws->data_ptr() : nullptr, *st = c10::cuda::getCurrentCUDAStream(dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = abi.accumulate_weights(qp, c.part[0], c.part[1], c.strides, (int)PS, btp, (int)MP, lp, sp, (int)B, (int)KVH, (int)(HQ / KVH),
+                                (int)D, (int)qlmax, (float)s1, gkp, w.lse, wtp, wb, wh, W, w.window, w.sinks, signs, k8, wp, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// addresses of a tensor's elements: [first, last)
+std::pair<uintptr_t, uintptr_t> extent(const at::Tensor& t) {
+  int64_t n = t.numel() ? 1 : 0;
+  for (int64_t i = 0; n && i < t.dim(); ++i) n += (t.size(i) - 1) * t.stride(i);
+  const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+  return {p, p + n * t.element_size()};
+}
+bool overlap(const at::Tensor& x, const at::Tensor& y) {
+  const auto a = extent(x), b = extent(y);
+  return a.first < b.second && b.first < a.second;
+}
+
+// evict(flat, strides, PS, D, block_tables, seq_lens, weights, keep, sinks, recent, kept, out_lens, out_tables, out_weights, k8)
+PyObject* evict(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  try {
+    if (n != 15 || !abi.evict) Py_RETURN_NONE;
+    const at::Tensor *bt = tensor(a[4]), *lens = tensor(a[5]), *wt = tensor(a[6]), *kept = tensor(a[10]), *ol = tensor(a[11]),
+                     *ot = a[12] == Py_None ? bt : tensor(a[12]), *ow = a[13] == Py_None ? wt : tensor(a[13]);
+    if (!bt || !lens || !wt || !kept || !ol || !ot || !ow || !wt->is_cuda() || bt->dim() != 2 || ot->dim() != 2 || wt->dim() != 3) Py_RETURN_NONE;
+    const int dev = wt->device().index();
+    long long PS, D, keep, sinks, recent;
+    bool k8;
+    Cache c;
+    if (dev != c10::cuda::current_device() || !integer(a[2], &PS) || PS != (int)PS || PS < 1 || !integer(a[3], &D) || D != (int)D ||
+        !integer(a[7], &keep) || keep != (int)keep || !integer(a[8], &sinks) || sinks != (int)sinks || !integer(a[9], &recent) ||
+        recent != (int)recent || !boolean(a[14], &k8) || keep < 1 || sinks < 0 || recent < 0 || sinks + recent > keep ||
+        !cache_of(a[0], a[1], dev, &c))
+      Py_RETURN_NONE;
+    for (const at::Tensor* t : {bt, lens, kept, ol, ot})
+      if (!on(*t, dev) || t->scalar_type() != at::kInt || !t->is_contiguous()) Py_RETURN_NONE;
+    const int64_t B = bt->size(0), MP = bt->size(1), KVH = wt->size(1), OMP = ot->size(1);
+    if (B > INT32_MAX || MP > INT32_MAX || OMP > INT32_MAX || KVH > INT32_MAX || !weight_rows(wt, B, KVH, dev) ||
+        !weight_rows(ow, B, KVH, dev) || ow->size(2) < keep || ot->size(0) != B || lens->dim() != 1 || lens->size(0) != B || ol->dim() != 1 ||
+        ol->size(0) != B || kept->dim() != 3 || kept->size(0) != B || kept->size(1) != KVH || kept->size(2) != keep || keep > OMP * PS ||
+        overlap(*lens, *ol) || ((ow->data_ptr() != wt->data_ptr() || ow->strides() != wt->strides()) && overlap(*wt, *ow)))
+      Py_RETURN_NONE;
+    const int32_t *btp = static_cast<const int32_t*>(bt->data_ptr()), *lp = static_cast<const int32_t*>(lens->data_ptr()),
+                  *otp = static_cast<const int32_t*>(ot->data_ptr());
+    int32_t *kp = static_cast<int32_t*>(kept->data_ptr()), *olp = static_cast<int32_t*>(ol->data_ptr());
+    const float* wtp = static_cast<const float*>(wt->data_ptr());
+    float* owp = static_cast<float*>(ow->data_ptr());
+    const int64_t wb = wt->stride(0), wh = wt->stride(1), ob = ow->stride(0), oh = ow->stride(1);
+    const int W = (int)wt->size(2), OW = (int)ow->size(2);
+    void* st = c10::cuda::getCurrentCUDAStream(dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = abi.evict(c.part[0], c.part[1], c.part[2], c.part[3], c.strides, (int)PS, btp, (int)MP, lp, (int)B, (int)KVH, (int)D, k8, wtp, wb,
+                   wh, W, (int)keep, (int)sinks, (int)recent, otp, (int)OMP, kp, olp, owp, ob, oh, OW, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
   } catch (...) {
     Py_RETURN_NONE;
   }
@@ -286,10 +427,12 @@ PyObject* layer_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
-// prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, chunk, signs, k8, workspace)
-PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, chunk, signs, k8, workspace);
+// prefill_window: .., window, sinks, lse
+template <bool WIN>
+PyObject* prefill_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
   try {
-    if (n != 14 || !abi.prefill) Py_RETURN_NONE;
+    if (n != (WIN ? 17 : 14) || !abi.prefill) Py_RETURN_NONE;
     const at::Tensor *q = tensor(a[0]), *bt = tensor(a[4]), *out = tensor(a[9]), *ws = a[13] == Py_None ? nullptr : tensor(a[13]);
     if (!q || !bt || !out || (!ws && a[13] != Py_None) || !q->is_cuda() || !PyList_CheckExact(a[5])) Py_RETURN_NONE;
     const int dev = q->device().index();
@@ -326,7 +469,11 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
       for (int k = 0; k < 4; ++k) rows[4 * i + k] = (int32_t)v[k];
     }
     const int G = (int)(HQ / KVH);
-    const size_t nb = abi.prefill_scratch_bytes(rows.data(), (int)n_rows, (int)NT, (int)KVH, G, (int)D, chunk, signs != nullptr);
+    Window w;
+    if (WIN && !window_of(a[14], a[15], a[16], NT, HQ, dev, &w)) Py_RETURN_NONE;
+    const size_t nb = WIN ? abi.prefill_window_scratch_bytes(rows.data(), (int)n_rows, (int)NT, (int)KVH, G, (int)D, chunk,
+                                                             signs != nullptr, w.window, w.sinks)
+                          : abi.prefill_scratch_bytes(rows.data(), (int)n_rows, (int)NT, (int)KVH, G, (int)D, chunk, signs != nullptr);
     const void* qp = q->data_ptr();
     const int32_t* btp = static_cast<const int32_t*>(bt->data_ptr());
     void *op = out->data_ptr(), *wp = ws ? ws->data_ptr() : nullptr;
@@ -335,9 +482,14 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
     void* st = c10::cuda::getCurrentCUDAStream(dev).stream();
     int rc;
     Py_BEGIN_ALLOW_THREADS
-    rc = abi.prefill(qp, 0, c.part[0], c.part[1], c.part[2], c.part[3], c.strides, (int)PS, btp, (int)B, (int)MP,
-                     rows.data(), (int)n_rows, (int)NT, (int)KVH, G, (int)D, (float)s1, (float)s2, signs, k8, chunk, sp, nb, op,
-                     out_f32, wp, st);
+    if (WIN)
+      rc = abi.prefill_window(qp, 0, c.part[0], c.part[1], c.part[2], c.part[3], c.strides, (int)PS, btp, (int)B, (int)MP,
+                              rows.data(), (int)n_rows, (int)NT, (int)KVH, G, (int)D, (float)s1, (float)s2, signs, k8, chunk, w.window,
+                              w.sinks, w.lse, sp, nb, op, out_f32, wp, st);
+    else
+      rc = abi.prefill(qp, 0, c.part[0], c.part[1], c.part[2], c.part[3], c.strides, (int)PS, btp, (int)B, (int)MP,
+                       rows.data(), (int)n_rows, (int)NT, (int)KVH, G, (int)D, (float)s1, (float)s2, signs, k8, chunk, sp, nb, op,
+                       out_f32, wp, st);
     Py_END_ALLOW_THREADS
     return PyLong_FromLong(rc);
   } catch (...) {
@@ -347,26 +499,38 @@ PyObject* prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
 
 // bind(addresses of the entry points in the order of Abi)
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long p[8];
-  if (!PyArg_ParseTuple(args, "KKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7])) return nullptr;
-  abi.write = reinterpret_cast<decltype(abi.write)>(p[0]);
-  abi.write_rot = reinterpret_cast<decltype(abi.write_rot)>(p[1]);
-  abi.write_k8 = reinterpret_cast<decltype(abi.write_k8)>(p[2]);
-  abi.decode = reinterpret_cast<decltype(abi.decode)>(p[3]);
-  abi.decode_rot = reinterpret_cast<decltype(abi.decode_rot)>(p[4]);
-  abi.decode_k8 = reinterpret_cast<decltype(abi.decode_k8)>(p[5]);
-  abi.prefill_scratch_bytes = reinterpret_cast<decltype(abi.prefill_scratch_bytes)>(p[6]);
-  abi.prefill = reinterpret_cast<decltype(abi.prefill)>(p[7]);
+  unsigned long long p[13];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8], &p[9], &p[10], &p[11], &p[12]))
+    return nullptr;
+  int i = 0;
+  auto take = [&](auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(p[i++]); };
+  take(abi.write);
+  take(abi.write_rot);
+  take(abi.write_k8);
+  take(abi.decode);
+  take(abi.decode_rot);
+  take(abi.decode_k8);
+  take(abi.prefill_scratch_bytes);
+  take(abi.prefill);
+  take(abi.decode_window);
+  take(abi.prefill_window_scratch_bytes);
+  take(abi.prefill_window);
+  take(abi.accumulate_weights);
+  take(abi.evict);
   Py_RETURN_NONE;
 }
 
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, "hands over the addresses of the C entry points"},
     {"write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(write)), METH_FASTCALL, "status, or None: not the plain form"},
-    {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode_any<false>)), METH_FASTCALL, "status, or None: not the plain form"},
     {"layer_write", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_write)), METH_FASTCALL, "status, or None: not the plain form"},
     {"layer_decode", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_decode)), METH_FASTCALL, "status, or None: not the plain form"},
-    {"prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"prefill", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill_any<false>)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"decode_window", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode_any<true>)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"prefill_window", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill_any<true>)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"accumulate_weights", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(accumulate_weights)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(evict)), METH_FASTCALL, "status, or None: not the plain form"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "hkv_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

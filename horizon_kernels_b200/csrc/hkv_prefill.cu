@@ -71,6 +71,8 @@ struct PrefillParams {
   int n_req;
   int kt_lo, kt_hi;                    // key tiles of this launch's chunk
   int first_chunk;
+  int window, sinks;                   // WIN: a token at position x sees the keys j <= x with j > x - window or j < sinks (window 0: all)
+  float* lse;                          // the rows' log-sum-exps, or null
   PfReq req[kPfReqs];
   PfStart start[kPfCtas + 1];
   PfSplit split[kPfCtas];
@@ -86,11 +88,74 @@ __host__ __device__ inline int pf_hi(const PfReq& r, int rt, int tok, int kt_hi)
 }
 __host__ __device__ inline int pf_row_tiles(const PfReq& r, int tok) { return (r.ql + tok - 1) / tok; }
 
+// WIN: the key tiles of a request without those between the sinks and the window of its first token, which are never made;
+// everywhere below a key tile is one of these. Tile v lies at v, from `su` on at v + skip.
+struct PfKeys {
+  int su, skip;
+};
+__host__ __device__ inline int pf_from(const PfReq& r, int t, int window) {   // first token of the window of query token t
+  return window > 0 ? max(0, r.L - r.ql + t + 1 - window) : 0;
+}
+__host__ __device__ inline PfKeys pf_keys(const PfReq& r, int window, int sinks) {
+  const int lo = pf_from(r, 0, window), su = (min(lo, sinks) + kKeys - 1) / kKeys;
+  return PfKeys{su, max(0, lo / kKeys - su)};
+}
+// the tiles of a chunk [kt_lo, kt_hi) that a row tile sees: [kt_lo, e1), the sinks, and [s2, e2), the window
+struct PfSpan {
+  int e1, s2, e2;
+  __host__ __device__ int count(int kt_lo) const { return e1 - kt_lo + e2 - s2; }
+  __host__ __device__ int begin(int kt_lo) const { return e1 > kt_lo ? kt_lo : s2; }
+};
+// (whole: one past the last tile that it sees at all; first: the first one)
+__host__ __device__ inline PfSpan pf_span(const PfReq& r, int rt, int tok, int kt_lo, int kt_hi, int window, int sinks, int* whole,
+                                          int* first) {
+  const int skip = pf_keys(r, window, sinks).skip, lo = pf_from(r, rt * tok, window), s = (min(lo, sinks) + kKeys - 1) / kKeys;
+  const int t_end = min(r.ql, (rt + 1) * tok), vis = max(1, min(r.L, r.L - r.ql + t_end));
+  const int a = max(s, lo / kKeys - skip), b = (vis + kKeys - 1) / kKeys - skip;
+  *whole = max(s, b);
+  *first = s > 0 ? 0 : a;
+  PfSpan x;
+  x.e1 = max(kt_lo, min(s, kt_hi));
+  x.s2 = max(a, kt_lo);
+  x.e2 = max(x.s2, min(b, kt_hi));
+  return x;
+}
+
+template <bool WIN>
 struct Walk {
   int req, h, rt, kt;
+  int window, sinks;
   __host__ __device__ bool same_tile(const PfStart& e) const { return req == e.req && h == e.h && rt == e.rt; }
   // the next row tile that has keys in this chunk
+  // tiles of the row tile from kt on
+  __host__ __device__ int left(const PfReq* r, int tok, int kt_lo, int kt_hi) const {
+    if (!WIN) return pf_hi(r[req], rt, tok, kt_hi) - kt;
+    int whole, first;
+    const PfSpan x = pf_span(r[req], rt, tok, kt_lo, kt_hi, window, sinks, &whole, &first);
+    return kt < x.e1 ? x.e1 - kt + x.e2 - x.s2 : x.e2 - kt;
+  }
+  __host__ __device__ void step(const PfReq* r, int tok, int kt_lo, int kt_hi, int n) {      // n tiles further in the row tile
+    if (WIN) {
+      int whole, first;
+      const PfSpan x = pf_span(r[req], rt, tok, kt_lo, kt_hi, window, sinks, &whole, &first);
+      if (kt < x.e1 && kt + n >= x.e1) n += x.s2 - x.e1;
+    }
+    kt += n;
+  }
   __host__ __device__ void advance(const PfReq* r, int n_req, int KVH, int tok, int kt_lo, int kt_hi) {
+    if (WIN) {
+      while (true) {
+        if (++rt >= pf_row_tiles(r[req], tok)) {
+          rt = 0;
+          if (++h >= KVH) { h = 0; ++req; }
+        }
+        if (req >= n_req) return;
+        int whole, first;
+        const PfSpan x = pf_span(r[req], rt, tok, kt_lo, kt_hi, window, sinks, &whole, &first);
+        kt = x.begin(kt_lo);
+        if (x.count(kt_lo) > 0) return;
+      }
+    }
     kt = kt_lo;
     do {
       if (++rt >= pf_row_tiles(r[req], tok)) {
@@ -116,6 +181,9 @@ struct TileParams {
   int row[kPfReqs];                    // block-table rows
   int L[kPfReqs];
   int tile0[kPfReqs];
+  int sinks;                           // WIN: tokens from `sinks` to lo - 1 are seen by no row and not read
+  int lo[kPfReqs];
+  int su[kPfReqs], skip[kPfReqs];
 };
 
 template <int BF16>
@@ -130,7 +198,7 @@ __device__ __forceinline__ uint32_t operand_pair(uint32_t h2) {       // f16x2 -
 // of 128 rows (keys) x 128 bytes; values: 2 images of D rows (channels) x 128 bytes (64 keys). Byte b of row r lies at
 // r * 128 + (b ^ ((r & 7) << 4)): the 128-byte swizzle. HBM-bound on its output; every value is converted once per
 // launch, whereas converting inside attend_kernel would repeat it for every row tile (128 times in the chunk above).
-template <int D, int BF16, int K8>
+template <int D, int BF16, int K8, bool WIN>
 __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileParams p) {
   constexpr int NB = D / 16;
   pdl_wait();                                     // the cache may come from the preceding launch
@@ -139,7 +207,8 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
   int r = 0;
   while (r + 1 < p.n_req && p.tile0[r + 1] <= gt) ++r;
   const int n_t = (r + 1 < p.n_req ? p.tile0[r + 1] : p.n_tiles) - p.tile0[r];
-  const int pos0 = (p.kt_lo + gt - p.tile0[r]) * kKeys, L = p.L[r];
+  const int kt = p.kt_lo + gt - p.tile0[r], pos0 = (WIN && kt >= p.su[r] ? kt + p.skip[r] : kt) * kKeys, L = p.L[r];
+  auto there = [&](int pos) { return pos < L && pos / p.PS < p.MP && (!WIN || pos >= p.lo[r] || pos < p.sinks); };
   const int* bt = p.bt + (long long)p.row[r] * p.MP;
   const size_t image = (size_t)kKeys * D * 2;
   // request r's tiles: [head][tile][K, V]
@@ -152,7 +221,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
       uint32_t o[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) o[i] = 0;
-      if (pos < L && pos / p.PS < p.MP) {
+      if (there(pos)) {
         const long long page = __ldg(bt + pos / p.PS), off = pos % p.PS;
         if (K8) {
           const uint4 w8 = *reinterpret_cast<const uint4*>(p.kd + page * p.dsp + off * p.dst + h * p.dsh + blk * 16);
@@ -193,7 +262,7 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
         const int pos = pos0 + kb * 64 + c * 8 + k;
         uint2 w = make_uint2(0, 0);
         uint32_t sb = 0;
-        if (pos < L && pos / p.PS < p.MP) {
+        if (there(pos)) {
           const long long page = __ldg(bt + pos / p.PS), off = pos % p.PS;
           w = *reinterpret_cast<const uint2*>(p.vd + page * p.dsp + off * p.dst + h * p.dsh + blk * 8);
           sb = p.vsf[page * p.ssp + off * p.sst + h * p.ssh + blk];
@@ -341,6 +410,10 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
+// natural log-sum-exp of a row from its maximum (log2 domain) and its sum; -inf for a row that sees no key
+__device__ __forceinline__ float pf_lse(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
 struct PfShared {
   uint64_t full[kStages], empty[kStages];
   uint64_t q_full[2], q_free[2];       // query operands written / read for the last time in a piece
@@ -417,12 +490,14 @@ __device__ __forceinline__ void store_out(const PrefillParams& p, long long elem
 // before the exponentials 1.6 and 1.3 times as long.
 // A walk over the CTA's key tiles, piece by piece. A step to the next row tile of a request costs a few instructions: every
 // role takes it at every piece, two of them in a single thread.
+template <bool WIN>
 struct Tiles {
   const PrefillParams& p;
   PfStart last;
   int req, h, rt, kt, hi;              // hi: end of the current piece
   PfReq r;
   int n_rt;                            // row tiles of the request
+  int e1, s2;                          // WIN: after tile e1 - 1 comes s2 (PfSpan)
   uint32_t piece;
   bool first, end;                     // first tile of its piece; nothing left
   __device__ __forceinline__ explicit Tiles(const PrefillParams& p_) : p(p_), last(p_.start[blockIdx.x + 1]), piece(0) {
@@ -442,11 +517,24 @@ struct Tiles {
   }
   __device__ __forceinline__ bool cut() const { return rt == last.rt && h == last.h && req == last.req; }   // goes on in the next CTA
   __device__ __forceinline__ int tile_hi() const { return pf_hi(r, rt, p.tok, p.kt_hi); }
+  __device__ __forceinline__ PfSpan span(int* whole, int* tile0) const {
+    return pf_span(r, rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, whole, tile0);
+  }
   __device__ __forceinline__ void enter() {
     first = true;
     const bool c = cut();
     end = c && kt >= last.kt;
-    hi = c ? last.kt : tile_hi();
+    if constexpr (WIN) {
+      if (req >= p.n_req) return;
+      int whole, tile0;
+      const PfSpan x = span(&whole, &tile0);
+      e1 = x.e1;
+      s2 = x.s2;
+      hi = c ? last.kt : x.e2 > x.s2 ? x.e2 : x.e1;
+      if (hi == s2 && kt < e1) hi = e1;             // (cut between the sinks and the window)
+    } else {
+      hi = c ? last.kt : tile_hi();
+    }
   }
   __device__ __forceinline__ void next_piece() {
     if (cut()) {
@@ -454,6 +542,7 @@ struct Tiles {
       return;
     }
     kt = p.kt_lo;
+    bool none;
     do {
       if (++rt >= n_rt) {
         rt = 0;
@@ -463,18 +552,34 @@ struct Tiles {
           enter_request();
         }
       }
-    } while (req < p.n_req && tile_hi() <= p.kt_lo);      // (no keys in this chunk)
+      none = false;
+      if constexpr (WIN) {
+        if (req < p.n_req) {
+          int whole, tile0;
+          const PfSpan x = span(&whole, &tile0);
+          none = x.count(p.kt_lo) <= 0;
+          kt = x.begin(p.kt_lo);
+        } else {
+          kt = p.kt_lo;
+        }
+      } else {
+        none = tile_hi() <= p.kt_lo;
+      }
+    } while (req < p.n_req && none);                      // (no keys in this chunk)
     ++piece;
     enter();
   }
   __device__ __forceinline__ void next() {
     first = false;
     if (++kt == hi) next_piece();
+    else if (WIN && kt == e1) kt = s2;
   }
+  // tiles of the piece from kt (its first one) on
+  __device__ __forceinline__ int left() const { return WIN && kt < e1 && hi > e1 ? e1 - kt + hi - s2 : hi - kt; }
 };
 
 // LOSE (the self-test of the give-up path): the copy warp stops after three stages, and waits run out after a millisecond.
-template <int D, bool LOSE>
+template <int D, bool LOSE, bool WIN>
 __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __grid_constant__ PrefillParams p) {
   using S = PfShape<D>;
   constexpr int SETS = S::SETS, SOFT = S::SOFT, NQ = S::NQ;
@@ -522,12 +627,12 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
   if (warp == SOFT + 1) {
     // ------------------------------------------------------------------------------------------------ copy warp
     if (elect_one()) {
-      Tiles k(p), v(p);
+      Tiles<WIN> k(p), v(p);
       uint32_t fill = 0, st = 0, turn = 0;
       bool ok = *abort == 0;
-      auto fetch = [&](Tiles& x, int side) {
+      auto fetch = [&](Tiles<WIN>& x, int side) {
         const PfReq& r = x.r;
-        const int n_t = min(p.kt_hi, (r.L + kKeys - 1) / kKeys) - p.kt_lo;
+        const int n_t = min(p.kt_hi, (r.L + kKeys - 1) / kKeys - (WIN ? pf_keys(r, p.window, p.sinks).skip : 0)) - p.kt_lo;
         const uint8_t* from = p.tiles + ((size_t)r.tile0 * p.KVH + (size_t)x.h * n_t + (x.kt - p.kt_lo)) * 2 * IMAGE + side * IMAGE;
         for (int i = 0; ok && i < PER; ++i) {
           if (LOSE && fill == 3) ok = false;
@@ -556,7 +661,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
       const uint32_t id_qk = base | ((uint32_t)(kKeys / 8) << 17) | (p.k_bf16 ? (1u << 7) | (1u << 10) : 0u);
       const uint32_t id_pv = base | ((uint32_t)(D / 8) << 17);
       const uint32_t q_smem = smem_u32(smem), ring_a = smem_u32(ring);
-      Tiles k(p), v(p);
+      Tiles<WIN> k(p), v(p);
       uint32_t use = 0;                                   // ring stages handed out, in the copy warp's order
       uint32_t sk = 0, sv = 0, tv = 0;                    // score tile (of SETS) of the next score and value product; turn of the latter
       bool ok = *abort == 0;
@@ -625,7 +730,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
     const int row = tid - (SOFT + 4) * 32, quad = warp & 3;              // row of the tile, = tensor-memory lane
     const uint32_t inv_g = 65536u / p.G + 1;              // floor(row / G) = row * inv_g >> 16 for rows below 128
     const int HQ = p.KVH * p.G;
-    Tiles x(p), y(p);                                  // the piece to write out; the piece to fetch queries of
+    Tiles<WIN> x(p), y(p);                                  // the piece to write out; the piece to fetch queries of
     uint32_t g = 0;
     bool ok = *abort == 0;
     // queries of piece y: 16 bytes per lane and copy, whole rows per half warp or warp; rows that do not exist are zero
@@ -659,9 +764,19 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
         y.next_piece();
       }
       const PfReq r = x.r;
-      const int tile_hi = x.tile_hi();
-      g += x.hi - x.kt;
-      const bool divided = x.cut() || x.kt > p.kt_lo;
+      g += x.left();
+      bool divided, last_chunk, state_before;             // parts; no keys in later chunks; some in earlier ones
+      if constexpr (WIN) {
+        int whole, tile0;
+        const PfSpan sp = x.span(&whole, &tile0);
+        divided = x.cut() || x.kt != sp.begin(p.kt_lo);
+        last_chunk = whole <= p.kt_hi;
+        state_before = tile0 < p.kt_lo;
+      } else {
+        divided = x.cut() || x.kt > p.kt_lo;
+        last_chunk = x.tile_hi() == (max(1, min(r.L, r.L - r.ql + min(r.ql, (x.rt + 1) * p.tok))) + kKeys - 1) / kKeys;
+        state_before = !p.first_chunk;
+      }
       const int tk = (int)((uint32_t)row * inv_g >> 16), token = x.rt * p.tok + tk;
       const bool live = tk < p.tok && token < r.ql;
       const int head = x.h * p.G + (row - tk * p.G);
@@ -681,7 +796,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
         p.part_ml[slot * 256 + 128 + row] = l;
       } else if (p.state_o != nullptr && live) {
         float mo = -INFINITY, lo = 0.0f;
-        if (!p.first_chunk) {
+        if (state_before) {
           mo = p.state_ml[2 * st_row];
           lo = p.state_ml[2 * st_row + 1];
         }
@@ -690,7 +805,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
         wn = fast_exp2(m - ms);
         l = l * wn + lo * wo;
         m = mm;
-        finish = tile_hi == (max(1, min(r.L, r.L - r.ql + min(r.ql, (x.rt + 1) * p.tok))) + kKeys - 1) / kKeys;
+        finish = last_chunk;
         if (!finish) {
           p.state_ml[2 * st_row] = m;
           p.state_ml[2 * st_row + 1] = l;
@@ -698,6 +813,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
       }
       float inv = p.vs / fmaxf(l, 1e-30f);
       if (l != l) inv = l;
+      if (WIN && p.lse != nullptr && live && !divided && finish) p.lse[(long long)(r.q0 + token) * HQ + head] = pf_lse(m, l);
       const long long out_row = ((long long)(r.q0 + token) * HQ + head) * D;
       ok = all_wait(o_done0 + 8 * ((g - 1) % SETS), (g - 1) / SETS);
       if (!ok) break;
@@ -755,7 +871,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
 #pragma unroll
             for (int k = 0; k < 32; ++k) {
               f[k] *= wn;
-              if (!p.first_chunk) f[k] += so[k] * wo;
+              if (state_before) f[k] += so[k] * wo;
             }
             if (!finish) {
 #pragma unroll
@@ -780,7 +896,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
     const uint32_t s_bar = s_full0 + 8 * set, my_word = told0 + 8 * (set * 4 + quad);
     const int before = set == 0 ? SETS - 1 : set - 1;     // the set of the tile before
     const uint32_t word_before = told0 + 8 * (before * 4 + quad);
-    Tiles x(p);
+    Tiles<WIN> x(p);
     uint32_t g = set, turn = 0;                           // the set's next tile in the CTA's stream; its tiles done
     uint32_t g0 = 0;                                      // first tile of the piece
     const int tk = row / p.G;
@@ -791,13 +907,17 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
       const int lim = tk < p.tok && token < r.ql ? max(0, min(r.L, r.L - r.ql + token + 1)) : 0;      // keys this row sees
       // keys below this one are seen by every live row of the tile (rows that do not exist may take any value)
       const int whole = max(0, min(r.L, r.L - r.ql + x.rt * p.tok + 1));
-      const uint32_t g_end = g0 + (x.hi - x.kt);
+      const uint32_t g_end = g0 + x.left();
+      // WIN: the piece's tile i lies at x.kt + i, from `jump` on at i + beyond; keys below win_hi are out of the last row's window
+      const int jump = WIN && x.kt < x.e1 ? x.e1 - x.kt : 0;
+      const int beyond = WIN ? (x.kt < x.e1 ? x.s2 - jump : x.kt) + pf_keys(r, p.window, p.sinks).skip : 0;
+      const int win_hi = WIN ? pf_from(r, min(r.ql, (x.rt + 1) * p.tok) - 1, p.window) : 0;
       volatile float* top_now = xm + (x.piece & 1) * 128 + row;
       float m = -INFINITY;                                // the running maximum as this thread knows it
       unsigned long long l2 = 0;                          // two partial sums
       bool any_tile = false;
       for (; g < g_end; g += SETS, ++turn) {
-        const int key = (x.kt + (int)(g - g0)) * kKeys;
+        const int key = (WIN && (int)(g - g0) >= jump ? beyond + (int)(g - g0) : x.kt + (int)(g - g0)) * kKeys;
         const bool head = g == g0;
         ok = all_wait(s_bar, turn);
         if (!ok) break;
@@ -808,7 +928,13 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
           tm_ld32(s0, s_addr + 32 * c);
           tm_wait_ld();
           tm_ready(s0);
-          if (key + 32 * c + 32 > whole) {
+          if (WIN && (key + 32 * c + 32 > whole || (key + 32 * c < win_hi && key + 32 * c + 32 > p.sinks))) {
+            const int rel = lim - key - 32 * c, from = p.window > 0 ? rel - p.window : 0, sinks = p.sinks - key - 32 * c;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (i >= rel || (i < from && i >= sinks)) s0[i] = 0xff800000u;
+          }
+          if (!WIN && key + 32 * c + 32 > whole) {
             const int rel = lim - key - 32 * c;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
@@ -927,7 +1053,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
 
 // ------------------------------------------------------------------------------------------------------ merge_kernel
 // parts of a divided row tile (and the state of earlier chunks) -> output or state; a thread has eight channels of a row
-template <int D>
+template <int D, bool WIN>
 __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ PrefillParams p) {
   constexpr int LPR = D / 8;
   pdl_wait();
@@ -954,12 +1080,14 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Pref
     for (int k = 0; k < 8; ++k) acc[k] = acc[k] * a + v[k] * b;
     m = mm;
   };
-  if (state && !p.first_chunk) add(p.state_ml[2 * st_row], p.state_ml[2 * st_row + 1], p.state_o + st_row * D + ch);
+  int end, tile0 = 0;
+  if constexpr (WIN) pf_span(r, t.rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, &end, &tile0);
+  else end = (max(1, min(r.L, r.L - r.ql + min(r.ql, (t.rt + 1) * p.tok))) + kKeys - 1) / kKeys;
+  if (state && (WIN ? tile0 < p.kt_lo : !p.first_chunk)) add(p.state_ml[2 * st_row], p.state_ml[2 * st_row + 1], p.state_o + st_row * D + ch);
   for (int c = sp.c1; c <= sp.c2; ++c) {
     const long long slot = (long long)c * 2 + (c == sp.c1 ? sp.slot1 : 0);
     add(p.part_ml[slot * 256 + row], p.part_ml[slot * 256 + 128 + row], p.part_o + (slot * 128 + row) * D + ch);
   }
-  const int end = (max(1, min(r.L, r.L - r.ql + min(r.ql, (t.rt + 1) * p.tok))) + kKeys - 1) / kKeys;
   if (state && end > p.kt_hi) {
     float* so = p.state_o + st_row * D + ch;
     // a row's lanes (they agree on the return above) have read its state
@@ -974,6 +1102,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Pref
   }
   float inv = p.vs / fmaxf(l, 1e-30f);
   if (l != l) inv = l;
+  if (WIN && p.lse != nullptr && ch == 0) p.lse[(long long)(r.q0 + token) * HQ + t.h * p.G + (row - tk * p.G)] = pf_lse(m, l);
 #pragma unroll
   for (int k = 0; k < 8; ++k) acc[k] *= inv;
   store_out(p, ((long long)(r.q0 + token) * HQ + t.h * p.G + (row - tk * p.G)) * D + ch, acc);
@@ -982,15 +1111,18 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Pref
 // ---------------------------------------------------------------------------------------------------------- the plan
 // Cuts the key tiles of the launch into at most n_cta shares of equal cost; returns the CTAs used. Greedy: a CTA takes
 // row tiles in order until its share is full, and divides the one that does not fit when both parts are long enough.
+template <bool WIN>
 static int plan(PrefillParams& p, int n_cta, int* n_split) {
   long long total = 0;
-  Walk w0{0, 0, -1, 0};
+  Walk<WIN> w0{0, 0, -1, 0, p.window, p.sinks};
   w0.advance(p.req, p.n_req, p.KVH, p.tok, p.kt_lo, p.kt_hi);      // the first row tile with keys in the chunk
   for (int r = 0; r < p.n_req; ++r) {
     long long head = 0;
     const int n_rt = pf_row_tiles(p.req[r], p.tok);
     for (int rt = 0; rt < n_rt; ++rt) {
-      const int n = pf_hi(p.req[r], rt, p.tok, p.kt_hi) - p.kt_lo;
+      int whole, first;
+      const int n = WIN ? pf_span(p.req[r], rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, &whole, &first).count(p.kt_lo)
+                        : pf_hi(p.req[r], rt, p.tok, p.kt_hi) - p.kt_lo;
       if (n > 0) head += kPieceCost + n;
     }
     total += head * p.KVH;
@@ -998,7 +1130,7 @@ static int plan(PrefillParams& p, int n_cta, int* n_split) {
   long long cap = (total + n_cta - 1) / n_cta;
   if (cap < kPieceCost + 4) cap = kPieceCost + 4;
   for (;; cap += cap / 64 + 1) {
-    Walk w = w0;
+    Walk<WIN> w = w0;
     int c = 0;
     *n_split = 0;
     int part_c1 = -1, part_slot1 = 0, pieces = 0;         // the divided row tile being cut; pieces of the current CTA
@@ -1007,8 +1139,7 @@ static int plan(PrefillParams& p, int n_cta, int* n_split) {
     auto begin = [&]() { p.start[c] = PfStart{w.kt, w.rt, (short)w.h, (short)w.req}; room = cap; pieces = 0; };
     if (w.req < p.n_req) begin();
     while (w.req < p.n_req) {
-      const int hi = pf_hi(p.req[w.req], w.rt, p.tok, p.kt_hi);
-      const int n = hi - w.kt;
+      const int n = w.left(p.req, p.tok, p.kt_lo, p.kt_hi);
       if (kPieceCost + n <= room) {                       // the rest of the row tile
         if (part_c1 >= 0) {
           p.split[(*n_split)++] = PfSplit{(short)part_c1, (short)c, (short)part_slot1, 0};
@@ -1024,7 +1155,7 @@ static int plan(PrefillParams& p, int n_cta, int* n_split) {
       if (n - u < kMinPiece) u = n - kMinPiece;
       if (u >= kMinPiece) {
         if (part_c1 < 0) { part_c1 = c; part_slot1 = pieces == 0 ? 0 : 1; }
-        w.kt += (int)u;
+        w.step(p.req, p.tok, p.kt_lo, p.kt_hi, (int)u);
       } else if (pieces == 0) {                           // (cannot happen: cap holds kPieceCost + 2 * kMinPiece)
         fits = false;
         break;
@@ -1045,10 +1176,19 @@ struct PfGroup {
   int n, tiles;
   bool chunked;
 };
-static PfGroup next_group(const int32_t* rows, int n_rows, int chunk_tiles) {
+// of hkv_prefill_window; without one every key up to the row's own is seen
+struct PfWindow {
+  int window = 0, sinks = 0;
+  float* lse = nullptr;
+};
+static int key_tiles(const int32_t* row, const PfWindow& w) {
+  const PfReq r{row[1], row[2] - row[1], row[3], 0};
+  return (r.L + kKeys - 1) / kKeys - pf_keys(r, w.window, w.sinks).skip;
+}
+static PfGroup next_group(const int32_t* rows, int n_rows, int chunk_tiles, const PfWindow& w) {
   PfGroup g{0, 0, false};
   for (int i = 0; i < n_rows && g.n < kPfReqs; ++i) {
-    const int t = (rows[4 * i + 3] + kKeys - 1) / kKeys;
+    const int t = key_tiles(rows + 4 * i, w);
     if (t > chunk_tiles) {
       if (g.n == 0) g = PfGroup{1, chunk_tiles, true};
       break;
@@ -1070,11 +1210,12 @@ static int prefill_ctas() {
 struct PfScratch {
   size_t tiles, part_o, part_ml, state_o, state_ml, rot, total;
 };
-static PfScratch prefill_scratch(const int32_t* rows, int n_rows, int n_tok, int KVH, int G, int D, int chunk_tiles, int rot) {
+static PfScratch prefill_scratch(const int32_t* rows, int n_rows, int n_tok, int KVH, int G, int D, int chunk_tiles, int rot,
+                                 const PfWindow& w = PfWindow()) {
   int max_tiles = 0;
   size_t state_rows = 0;
   for (int i = 0; i < n_rows;) {
-    const PfGroup g = next_group(rows + 4 * i, n_rows - i, chunk_tiles);
+    const PfGroup g = next_group(rows + 4 * i, n_rows - i, chunk_tiles, w);
     if (g.tiles > max_tiles) max_tiles = g.tiles;
     if (g.chunked) {
       const size_t n = (size_t)(rows[4 * i + 2] - rows[4 * i + 1]) * KVH * G;
@@ -1119,11 +1260,23 @@ extern "C" size_t hkv_prefill_scratch_bytes(const int32_t* rows, int n_rows, int
   return prefill_scratch(rows, n_rows, n_tokens, KVH, G, D, chunk_tiles_of(chunk), rotated).total;
 }
 
+extern "C" size_t hkv_prefill_window_scratch_bytes(const int32_t* rows, int n_rows, int n_tokens, int KVH, int G, int D,
+                                                   int64_t chunk, int rotated, int window, int sinks) {
+  using namespace hkv;
+  if (n_rows < 1 || window < 0 || sinks < 0 || check_rows(rows, n_rows, n_tokens, KVH, G, D) != HKV_OK) return 0;
+  PfWindow w;
+  w.window = window > 0x3fffff00 ? 0 : window;
+  w.sinks = sinks;
+  return prefill_scratch(rows, n_rows, n_tokens, KVH, G, D, chunk_tiles_of(chunk), rotated, w).total;
+}
+
+template <bool WIN>
 static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ksf, const void* vd, const void* vsf,
                            const int64_t strides[6], int PS, const int32_t* block_tables, int n_tables, int MP,
                            const int32_t* rows, int n_rows, int n_tokens, int KVH, int G, int D, float qk_scale, float out_scale,
                            const float* signs, int k8, int64_t chunk, void* scratch, size_t scratch_bytes, void* out,
-                           int out_f32, void* workspace, void* stream, bool lose) {
+                           int out_f32, void* workspace, void* stream, bool lose,
+                           const hkv::PfWindow& win = hkv::PfWindow()) {
   using namespace hkv;
   if (n_rows == 0) return HKV_OK;
   if (n_rows < 0) return HKV_ERR_RANGE;
@@ -1139,7 +1292,7 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
   for (int i = 0; i < n_rows; ++i)
     if (rows[4 * i] >= n_tables || (int64_t)rows[4 * i + 3] > (int64_t)MP * PS) return HKV_ERR_RANGE;
   const int ct = chunk_tiles_of(chunk);
-  const PfScratch sc = prefill_scratch(rows, n_rows, n_tokens, KVH, G, D, ct, signs != nullptr);
+  const PfScratch sc = prefill_scratch(rows, n_rows, n_tokens, KVH, G, D, ct, signs != nullptr, win);
   if (scratch_bytes < sc.total) return HKV_ERR_WORKSPACE;
   cudaStream_t st = (cudaStream_t)stream;
   uint8_t* base = (uint8_t*)scratch;
@@ -1158,6 +1311,9 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
   const float c = qk_scale * 1.4426950408889634f;
   p.c = fmaxf(fabsf(c), 1e-37f);                          // (zero: masked scores would become 0 * -inf)
   p.vs = c != c ? c : out_scale;                          // (fmaxf drops a NaN: the output takes it instead)
+  p.window = win.window;
+  p.sinks = win.sinks;
+  p.lse = win.lse;
   p.out = out;
   p.out_f32 = out_f32;
   p.k_bf16 = !q_f16;                                      // (the cached values are exact in both types)
@@ -1180,25 +1336,32 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
   t.ssp = strides[3]; t.sst = strides[4]; t.ssh = strides[5];
   t.bt = block_tables; t.tiles = base + sc.tiles;
   t.MP = MP; t.PS = PS; t.KVH = KVH;
+  t.sinks = win.sinks;
   t.k_flip = c < 0.0f ? 0x80008000u : 0u;
   void (*tk)(const TileParams);
-  if (k8) tk = q_f16 ? tile_kernel<256, 0, 1> : tile_kernel<256, 1, 1>;
-  else if (D == 128) tk = q_f16 ? tile_kernel<128, 0, 0> : tile_kernel<128, 1, 0>;
-  else tk = q_f16 ? tile_kernel<256, 0, 0> : tile_kernel<256, 1, 0>;
-  void (*ak)(const PrefillParams) = lose ? (D == 128 ? attend_kernel<128, true> : attend_kernel<256, true>)
-                                         : D == 128 ? attend_kernel<128, false> : attend_kernel<256, false>;
-  void (*mk)(const PrefillParams) = D == 128 ? merge_kernel<128> : merge_kernel<256>;
+  if (k8) tk = q_f16 ? tile_kernel<256, 0, 1, WIN> : tile_kernel<256, 1, 1, WIN>;
+  else if (D == 128) tk = q_f16 ? tile_kernel<128, 0, 0, WIN> : tile_kernel<128, 1, 0, WIN>;
+  else tk = q_f16 ? tile_kernel<256, 0, 0, WIN> : tile_kernel<256, 1, 0, WIN>;
+  void (*ak)(const PrefillParams);
+  if constexpr (WIN) ak = D == 128 ? attend_kernel<128, false, true> : attend_kernel<256, false, true>;
+  else ak = lose ? (D == 128 ? attend_kernel<128, true, false> : attend_kernel<256, true, false>)
+                 : D == 128 ? attend_kernel<128, false, false> : attend_kernel<256, false, false>;
+  void (*mk)(const PrefillParams) = D == 128 ? merge_kernel<128, WIN> : merge_kernel<256, WIN>;
   rc = record_cuda(cudaFuncSetAttribute((const void*)ak, cudaFuncAttributeMaxDynamicSharedMemorySize, kPfSmem));
   if (rc != HKV_OK) return rc;
 
   for (int i = 0; i < n_rows;) {
-    const PfGroup g = next_group(rows + 4 * i, n_rows - i, ct);
+    const PfGroup g = next_group(rows + 4 * i, n_rows - i, ct, win);
     int base_tile = 0, all_tiles = 0;
     p.n_req = t.n_req = g.n;
     for (int k = 0; k < g.n; ++k) {
       const int32_t* r = rows + 4 * (i + k);
-      const int n_t = (r[3] + kKeys - 1) / kKeys;
+      const int n_t = key_tiles(r, win);
       p.req[k] = PfReq{r[1], r[2] - r[1], r[3], base_tile};
+      const PfKeys keys = pf_keys(p.req[k], win.window, win.sinks);
+      t.lo[k] = pf_from(p.req[k], 0, win.window);
+      t.su[k] = keys.su;
+      t.skip[k] = keys.skip;
       t.row[k] = r[0];
       t.L[k] = r[3];
       t.tile0[k] = base_tile;
@@ -1213,7 +1376,7 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
       p.kt_hi = g.chunked ? (lo + ct < all_tiles ? lo + ct : all_tiles) : all_tiles;
       t.n_tiles = g.chunked ? p.kt_hi - lo : base_tile;
       int n_split = 0;
-      const int used = plan(p, n_cta, &n_split);
+      const int used = plan<WIN>(p, n_cta, &n_split);
       rc = record_cuda(launch_pdl(tk, dim3((unsigned)t.n_tiles, (unsigned)KVH, 2), dim3(128), 0, st, t));
       if (rc == HKV_OK) rc = record_cuda(launch_pdl(ak, dim3((unsigned)used), dim3(D == 128 ? PfShape<128>::THREADS : PfShape<256>::THREADS), kPfSmem, st, p));
       if (rc == HKV_OK && n_split > 0)
@@ -1231,7 +1394,7 @@ extern "C" int hkv_prefill(const void* q, int q_f16, const void* kd, const void*
                            const int32_t* rows, int n_rows, int n_tokens, int KVH, int G, int D, float qk_scale, float out_scale,
                            const float* signs, int k8, int64_t chunk, void* scratch, size_t scratch_bytes, void* out,
                            int out_f32, void* workspace, void* stream) {
-  return prefill_impl(q, q_f16, kd, ksf, vd, vsf, strides, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D, qk_scale,
+  return prefill_impl<false>(q, q_f16, kd, ksf, vd, vsf, strides, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D, qk_scale,
                       out_scale, signs, k8, chunk, scratch, scratch_bytes, out, out_f32, workspace, stream, false);
 }
 
@@ -1241,6 +1404,21 @@ extern "C" int hkv_selftest_prefill_timeout(const void* q, int q_f16, const void
                                             int D, float qk_scale, float out_scale, const float* signs, int k8, int64_t chunk,
                                             void* scratch, size_t scratch_bytes, void* out, int out_f32, void* workspace,
                                             void* stream) {
-  return prefill_impl(q, q_f16, kd, ksf, vd, vsf, strides, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D, qk_scale,
+  return prefill_impl<false>(q, q_f16, kd, ksf, vd, vsf, strides, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D, qk_scale,
                       out_scale, signs, k8, chunk, scratch, scratch_bytes, out, out_f32, workspace, stream, true);
+}
+
+extern "C" int hkv_prefill_window(const void* q, int q_f16, const void* kd, const void* ksf, const void* vd, const void* vsf,
+                                  const int64_t strides[6], int PS, const int32_t* block_tables, int n_tables, int MP,
+                                  const int32_t* rows, int n_rows, int n_tokens, int KVH, int G, int D, float qk_scale,
+                                  float out_scale, const float* signs, int k8, int64_t chunk, int window, int sinks, float* lse,
+                                  void* scratch, size_t scratch_bytes, void* out, int out_f32, void* workspace, void* stream) {
+  if (window < 0 || sinks < 0) return HKV_ERR_RANGE;
+  if ((uintptr_t)lse & 3) return HKV_ERR_ALIGN;
+  hkv::PfWindow w;
+  w.window = window > 0x3fffff00 ? 0 : window;            // (no context is longer)
+  w.sinks = sinks;
+  w.lse = lse;
+  return prefill_impl<true>(q, q_f16, kd, ksf, vd, vsf, strides, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D,
+                            qk_scale, out_scale, signs, k8, chunk, scratch, scratch_bytes, out, out_f32, workspace, stream, false, w);
 }

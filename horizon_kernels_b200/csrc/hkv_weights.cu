@@ -1,0 +1,524 @@
+// Attention weights that cached tokens gather: weights[b, h, j] += sum over the query rows r of kv head h that see token j of
+// exp(score(r, j) - lse[r]), the rows' log-sum-exps being those of the attention call before. What an eviction goes by.
+//
+// Keys only: per token and kv head 72 bytes (head_dim 128; 144 at 256, 256 as FP8) are read and 4 bytes of weights read and
+// written, against 144 of an attention step. As in the decode kernel the (request, kv head) sequences form one stream of units
+// of 32 tokens that is cut into equal parts, here one per WARP: nothing is merged, every weight belongs to one warp, so there
+// is no order to depend on. A warp fetches its units ahead through a ring of its own and computes S^T = K Q^T per 16 tokens
+// with mma.m16n8k16, the keys dequantised in registers (code * scale is exact in f16). Query rows beyond those of a pass are
+// taken in further passes over the keys.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <cmath>
+
+#include "hkv_common.cuh"
+
+namespace hkv {
+
+int record_cuda(cudaError_t e);
+int noalloc_workspace(void** ws);
+
+constexpr int kWtWarps = 4;
+constexpr int kWtThreads = kWtWarps * 32;
+constexpr int kWtCost = 4;           // what a sequence costs a warp beyond its units (its queries and log-sum-exps), in units
+constexpr int kWtMin = 2;            // least units of a warp
+
+struct WeightsParams {
+  const __nv_bfloat16* q;
+  const uint8_t* kd;
+  const uint8_t* ksf;
+  long long dst, dsh, sst, ssh;
+  unsigned dsp, ssp;
+  const int* bt;
+  const int* seq_lens;
+  const int* qsl;
+  const float* gk;
+  const float* lse;
+  const float* signs;
+  float* w;
+  long long w_b, w_h;
+  int* status;
+  int MP, B, KVH, G, qlmax, lps, row0, max_len, window, sinks;
+  float scale_log2, rot_scale;
+};
+
+// LAYOUT as in the decode kernel: 0 rows of [codes | scales] back to back, 1 codes and scales in regions of their own, 3 rows
+// at any stride, copied one by one; 2 FP8 keys (rows at any stride)
+template <int D, int LAYOUT>
+struct WtGeo {
+  static constexpr bool K8 = LAYOUT == 2;
+  static constexpr bool ROWCOPY = LAYOUT >= 2;
+  static constexpr int SD = K8 ? D : D / 2, SS = K8 ? 0 : D / 16;
+  static constexpr int UT = 32;
+  static constexpr int ROW = LAYOUT == 1 ? SD : SD + SS;             // byte stride between token rows of a stage
+  static constexpr int SF_BASE = LAYOUT == 1 ? UT * SD : SD, SF_ROW = LAYOUT == 1 ? SS : ROW;
+  static constexpr int STAGE = UT * (SD + SS);
+  static constexpr int NS = 4;
+  static constexpr int KS = D / 16, NBL = D / 64, KB = K8 ? 16 : 8;
+  // 72-byte rows: as in the decode kernel, so that the lanes' loads touch every bank once
+  __device__ static constexpr int tok(int i) {
+    return (D == 128 && LAYOUT != 1) ? ((i & 5) | ((i & 2) << 2) | ((i & 8) >> 2)) : i;
+  }
+};
+
+struct WtReq {
+  int U, L, ql, q0;                    // units, context, query tokens, first query row
+  int su, skip;                        // units from su on lie `skip` units further
+};
+__device__ __forceinline__ WtReq wt_req(const WeightsParams& p, int b) {
+  WtReq r;
+  r.q0 = __ldg(p.qsl + b);
+  int ql = __ldg(p.qsl + b + 1) - r.q0;
+  ql = (ql < 0 || ql > p.qlmax || p.G * ql <= p.row0) ? 0 : ql;
+  r.ql = ql;
+  r.L = ql > 0 ? min(max(__ldg(p.seq_lens + b), 0), p.max_len) : 0;
+  const int all = (r.L + 31) >> 5;
+  const int lo = p.window > 0 ? max(0, r.L - ql + p.row0 / p.G - p.window + 1) : 0;      // first token of the first row's window
+  const int su = (min(lo, p.sinks) + 31) >> 5, wu = lo >> 5;
+  r.su = su;
+  r.skip = max(0, wu - su);
+  r.U = all - r.skip;
+  return r;
+}
+
+template <int D, int LAYOUT, int QT>
+__global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams p) {
+  using Gm = WtGeo<D, LAYOUT>;
+  constexpr int NS = Gm::NS, UT = Gm::UT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kWtWarps * NS];
+  int* coarse = reinterpret_cast<int*>(smem + kWtWarps * NS * Gm::STAGE);
+  const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5, g = lane >> 2, c = lane & 3;
+  const int KVH = p.KVH, B = p.B, G = p.G;
+  if (tid < kWtWarps * NS) mbar_init(bars + tid, Gm::ROWCOPY ? 32 : 1);
+  pdl_wait();
+  pdl_launch_dependents();
+
+  // prefix of the requests' weights (units + cost) per kv head, 32 requests at a time
+  auto wt = [](int U) { return U > 0 ? U + kWtCost : 0; };
+  const int ngrp = (B + 31) >> 5;
+  for (int grp = wp; grp < ngrp; grp += kWtWarps) {
+    const int b = grp * 32 + lane;
+    int u = b < B ? wt(wt_req(p, b).U) : 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+    if (lane == 0) coarse[grp + 1] = u;
+  }
+  __syncthreads();
+  if (wp == 0) {
+    const int per_lane = (ngrp + 31) >> 5;
+    int s = 0;
+    for (int i = 0; i < per_lane; ++i) {
+      const int k = lane * per_lane + i;
+      s += k < ngrp ? coarse[k + 1] : 0;
+    }
+    int incl = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    int run = incl - s;
+    for (int i = 0; i < per_lane; ++i) {
+      const int k = lane * per_lane + i;
+      if (k < ngrp) {
+        run += coarse[k + 1];
+        coarse[k + 1] = run;
+      }
+    }
+    if (lane == 0) coarse[0] = 0;
+  }
+  fence_barrier_init();
+  __syncthreads();
+
+  const long long total = (long long)coarse[ngrp] * KVH;
+  const long long parts = (long long)gridDim.x * kWtWarps;
+  const long long per = max((long long)(kWtMin + kWtCost), (total + parts - 1) / parts);
+  const long long lo = ((long long)blockIdx.x + (long long)wp * gridDim.x) * per, hi = min(total, lo + per);
+  if (lo >= hi) return;
+
+  // the sequence that holds stream position lo
+  int b0, base0;
+  {
+    int lo_g = 0, hi_g = ngrp;
+    while (hi_g - lo_g > 1) {
+      const int m = (lo_g + hi_g) >> 1;
+      if ((long long)coarse[m] * KVH <= lo) lo_g = m; else hi_g = m;
+    }
+    const int b = lo_g * 32 + lane;
+    const int u = b < B ? wt(wt_req(p, b).U) : 0;
+    int incl = u;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, (long long)(coarse[lo_g] + incl) * KVH > lo);
+    const int j = __ffs(hit) - 1;
+    b0 = lo_g * 32 + j;
+    base0 = coarse[lo_g] + __shfl_sync(0xffffffffu, incl - u, j);
+  }
+  // A walk over the units of [lo, hi): the fetching side runs NS units ahead of the computing one
+  struct Walk {
+    int b, h, u, end;                  // the next unit of sequence (b, h), one past its last here
+    long long seq0;                    // stream position of the sequence: kWtCost slots, then its units
+    WtReq r;
+  };
+  auto enter = [&](Walk& x, long long pos) {        // from stream position pos on; false: nothing left
+    while (pos < hi) {
+      const long long u0 = x.seq0 + kWtCost, e = u0 + x.r.U;
+      const long long from = max(pos, u0), to = min(hi, e);
+      if (x.r.U > 0 && from < to) {
+        x.u = (int)(from - u0);
+        x.end = (int)(to - u0);
+        return true;
+      }
+      if (hi <= e) return false;
+      x.seq0 = e;
+      pos = max(pos, e);
+      if (++x.h == KVH) {
+        x.h = 0;
+        do {
+          if (++x.b >= B) return false;
+          x.r = wt_req(p, x.b);
+        } while (x.r.U <= 0);
+      }
+    }
+    return false;
+  };
+  Walk cw;
+  cw.b = b0;
+  cw.r = wt_req(p, b0);
+  cw.h = (int)((lo - (long long)base0 * KVH) / wt(cw.r.U));
+  cw.seq0 = (long long)base0 * KVH + (long long)cw.h * wt(cw.r.U);
+  bool more = enter(cw, lo);
+  Walk fw = cw;
+  bool f_more = more;
+
+  const uint32_t ring_a = smem_u32(smem + wp * NS * Gm::STAGE), bars_a = smem_u32(bars + wp * NS);
+  const int PSM = (1 << p.lps) - 1;
+  unsigned f_n = 0, c_n = 0;
+  // fetches the next unit, 16-token blocks that hold a visible token only
+  auto fetch = [&]() {
+    const uint32_t bar = bars_a + 8 * (f_n % NS), st = ring_a + (f_n % NS) * Gm::STAGE;
+    const int tok0 = (fw.u + (fw.u >= fw.r.su ? fw.r.skip : 0)) * UT;
+    const int lo_w = p.window > 0 ? max(0, fw.r.L - fw.r.ql + p.row0 / G - p.window + 1) : 0;
+    bool blk[2];
+    int page[2];
+#pragma unroll
+    for (int bi = 0; bi < 2; ++bi) {
+      const int t = tok0 + 16 * bi;
+      blk[bi] = t < fw.r.L && (t + 16 > lo_w || t < p.sinks);
+      page[bi] = blk[bi] ? __ldg(p.bt + (long long)fw.b * p.MP + (t >> p.lps)) : 0;
+    }
+    const uint8_t* kd = p.kd + (long long)fw.h * p.dsh;
+    const uint8_t* ks = p.ksf + (long long)fw.h * p.ssh;
+    if (Gm::ROWCOPY) {
+      // two lanes per token row (of a 16-token block)
+      constexpr int CB = D == 128 ? 8 : 16, N = (Gm::SD + Gm::SS) / CB;
+      const int row = lane >> 1;
+#pragma unroll
+      for (int bi = 0; bi < 2; ++bi)
+        if (blk[bi]) {
+          const uint8_t* src = kd + (unsigned long long)(unsigned)page[bi] * p.dsp + (((tok0 + 16 * bi) & PSM) + row) * p.dst;
+          const uint32_t d = st + (16 * bi + row) * Gm::ROW;
+          for (int j = lane & 1; j < N; j += 2) cp_async<CB>(d + j * CB, src + j * CB);
+        }
+      cp_async_mbar_arrive_noinc(bar);
+    } else if (elect_one()) {
+      const int nb = (int)blk[0] + (int)blk[1];
+      mbar_expect_tx_u32(bar, nb * 16 * (Gm::SD + Gm::SS));
+#pragma unroll
+      for (int bi = 0; bi < 2; ++bi)
+        if (blk[bi]) {
+          const unsigned pos = (tok0 + 16 * bi) & PSM;
+          const uint8_t* src = kd + (unsigned long long)(unsigned)page[bi] * p.dsp + pos * (unsigned)Gm::ROW;
+          if (LAYOUT == 0) {
+            bulk_g2s_u32(st + bi * 16 * Gm::ROW, src, 16 * Gm::ROW, bar);
+          } else {
+            bulk_g2s_u32(st + bi * 16 * Gm::SD, src, 16 * Gm::SD, bar);
+            bulk_g2s_u32(st + UT * Gm::SD + bi * 16 * Gm::SS, ks + (unsigned long long)(unsigned)page[bi] * p.ssp + pos * (unsigned)Gm::SS,
+                         16 * Gm::SS, bar);
+          }
+        }
+    }
+    ++f_n;
+    if (++fw.u == fw.end) f_more = enter(fw, fw.seq0 + kWtCost + fw.end);
+  };
+  while (f_more && f_n < NS) fetch();
+
+  const int r0 = Gm::tok(g), r1 = Gm::tok(g + 8);
+  const uint32_t koff_d = r0 * Gm::ROW + Gm::KB * Gm::NBL * c, koff_s = Gm::SF_BASE + r0 * Gm::SF_ROW + Gm::NBL * c;
+  constexpr int KR1 = Gm::tok(8) - Gm::tok(0);
+  bool dead = false;
+  while (more && !dead) {
+    // the queries of this sequence: rows 8 q + g, channels of this lane's key blocks, as f16; rows 2 c, 2 c + 1 of the scores
+    const int L = cw.r.L, ql = cw.r.ql, q0 = cw.r.q0, h = cw.h;
+    const int R = min(8 * QT, G * ql - p.row0);
+    const float sc_signed = p.scale_log2 * __ldg(p.gk + h);
+    const bool flip = sc_signed < 0.0f;
+    const float sc = fabsf(sc_signed);
+    uint32_t qa[QT][Gm::KS][2];
+    float le[QT][2];
+    int lim[QT][2], from[QT][2];
+#pragma unroll
+    for (int q = 0; q < QT; ++q) {
+      const bool have = g + 8 * q < R;
+      const int t = have ? (p.row0 + g + 8 * q) / G : 0, gq = have ? p.row0 + g + 8 * q - t * G : 0;
+      const __nv_bfloat16* qrow = p.q + ((long long)(q0 + t) * (KVH * G) + h * G + gq) * D;
+      constexpr int NQ = 16 * Gm::NBL;
+      float qf[NQ];
+#pragma unroll
+      for (int u = 0; u < 2 * Gm::NBL; ++u) {
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (have) x = __ldg(reinterpret_cast<const uint4*>(qrow + NQ * c) + u);
+        const uint32_t ws[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          qf[8 * u + 2 * i] = __uint_as_float(ws[i] << 16);
+          qf[8 * u + 2 * i + 1] = __uint_as_float(ws[i] & 0xffff0000u);
+        }
+      }
+      if (p.signs != nullptr) {
+        // bf16(FWHT(q * signs) * head_dim^-0.5) in the stage order of the decode kernel: the same bits
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) qf[i] = __fmul_rn(qf[i], __ldg(p.signs + NQ * c + i));
+#pragma unroll
+        for (int hh = 1; hh < NQ; hh *= 2)
+#pragma unroll
+          for (int i = 0; i < NQ; ++i)
+            if ((i & hh) == 0) {
+              const float a = qf[i], b = qf[i + hh];
+              qf[i] = __fadd_rn(a, b);
+              qf[i + hh] = __fsub_rn(a, b);
+            }
+#pragma unroll
+        for (int m = 1; m < 4; m *= 2) {
+          const bool upper = (c & m) != 0;
+#pragma unroll
+          for (int i = 0; i < NQ; ++i) {
+            const float o2 = __shfl_xor_sync(0xffffffffu, qf[i], m);
+            qf[i] = upper ? __fsub_rn(o2, qf[i]) : __fadd_rn(qf[i], o2);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) qf[i] = __bfloat162float(__float2bfloat16_rn(__fmul_rn(qf[i], p.rot_scale)));
+      }
+#pragma unroll
+      for (int i = 0; i < NQ / 2; ++i) {
+        const float a = flip ? -qf[2 * i] : qf[2 * i], b = flip ? -qf[2 * i + 1] : qf[2 * i + 1];
+        qa[q][i >> 1][i & 1] = pack_f16x2_sat(a, b);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int r = 8 * q + 2 * c + k, row = p.row0 + r;
+        const bool is = r < R;
+        const int tr = is ? row / G : 0;
+        le[q][k] = is ? __ldg(p.lse + (long long)(q0 + tr) * (KVH * G) + h * G + row - tr * G) * 1.4426950408889634f
+                       : __int_as_float(0x7f800000);              // (a row that does not exist: its scores are 0 - inf)
+        lim[q][k] = is ? L - ql + tr + 1 : 0;       // sees the keys below this one
+        from[q][k] = is && p.window > 0 ? L - ql + tr + 1 - p.window : 0;
+      }
+    }
+    // tokens of [w_hi, t_lo) and whole sinks are seen by every row that exists
+    const int t_lo = L - ql + p.row0 / G + 1;
+    const int w_hi = p.window > 0 ? L - ql + (p.row0 + R - 1) / G + 1 - p.window : 0;
+    float* wrow = p.w + (long long)cw.b * p.w_b + (long long)h * p.w_h;
+    while (true) {
+      const uint32_t bar = bars_a + 8 * (c_n % NS), st = ring_a + (c_n % NS) * Gm::STAGE;
+      const int tok0 = (cw.u + (cw.u >= cw.r.su ? cw.r.skip : 0)) * UT;
+      // this lane's token of the unit, whose weight it adds to: block c / 2, row r0 or r1
+      const int mine = tok0 + 16 * (c >> 1) + (c & 1 ? r1 : r0);
+      const bool masked = tok0 + UT > t_lo || (tok0 < w_hi && tok0 + UT > p.sinks);
+      const int lo_w = p.window > 0 ? L - ql + p.row0 / G + 1 - p.window : 0;
+      const bool add = mine < L && (mine >= lo_w || mine < p.sinks);
+      float old = add ? wrow[mine] : 0.0f;
+      if (!mbar_try_wait_u32(bar, (c_n / NS) & 1) && !mbar_wait_bounded_u32(bar, (c_n / NS) & 1)) {
+        if (lane == 0) atomicExch(p.status, HKV_ERR_DEVICE_WAIT);
+        dead = true;
+        break;
+      }
+      float sum[2][2];                              // [block][row r0 / r1], over this lane's query rows
+#pragma unroll
+      for (int bi = 0; bi < 2; ++bi) {
+        const uint32_t kd_ = st + koff_d + bi * 16 * Gm::ROW, ks_ = st + koff_s + bi * 16 * Gm::SF_ROW;
+        float x[QT][4];
+#pragma unroll
+        for (int q = 0; q < QT; ++q) x[q][0] = x[q][1] = x[q][2] = x[q][3] = 0.0f;
+        if (Gm::K8) {
+#pragma unroll
+          for (int u = 0; u < Gm::NBL; ++u) {
+            const uint4 a = lds128(kd_ + 16 * u), b = lds128(kd_ + KR1 * Gm::ROW + 16 * u);
+            const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              uint32_t A[4];
+              e4m3x4_to_f16x2(wa[v], A[0], A[2]);
+              e4m3x4_to_f16x2(wb[v], A[1], A[3]);
+#pragma unroll
+              for (int q = 0; q < QT; ++q) mma_f16(x[q], A[0], A[1], A[2], A[3], qa[q][4 * u + v][0], qa[q][4 * u + v][1]);
+            }
+          }
+        } else {
+          uint2 w0[Gm::NBL], w1[Gm::NBL];
+          uint32_t h0[(Gm::NBL + 1) / 2], h1[(Gm::NBL + 1) / 2];
+          if (Gm::NBL == 2) {
+            w0[0] = lds64(kd_);
+            w0[1] = lds64(kd_ + 8);
+            w1[0] = lds64(kd_ + KR1 * Gm::ROW);
+            w1[1] = lds64(kd_ + KR1 * Gm::ROW + 8);
+            h0[0] = e4m3x2_to_f16x2(lds16(ks_));
+            h1[0] = e4m3x2_to_f16x2(lds16(ks_ + KR1 * Gm::SF_ROW));
+          } else {
+#pragma unroll
+            for (int j = 0; j < Gm::NBL / 2; ++j) {
+              const uint4 a = lds128(kd_ + 16 * j), b = lds128(kd_ + KR1 * Gm::ROW + 16 * j);
+              w0[2 * j] = make_uint2(a.x, a.y);
+              w0[2 * j + 1] = make_uint2(a.z, a.w);
+              w1[2 * j] = make_uint2(b.x, b.y);
+              w1[2 * j + 1] = make_uint2(b.z, b.w);
+            }
+            e4m3x4_to_f16x2(lds32(ks_), h0[0], h0[(Gm::NBL - 1) / 2]);
+            e4m3x4_to_f16x2(lds32(ks_ + KR1 * Gm::SF_ROW), h1[0], h1[(Gm::NBL - 1) / 2]);
+          }
+#pragma unroll
+          for (int u = 0; u < Gm::NBL; ++u) {
+            const __half2 p0 = u32_as_h2(h0[u >> 1]), p1 = u32_as_h2(h1[u >> 1]);
+            const __half2 sf0 = (u & 1) ? __high2half2(p0) : __low2half2(p0);
+            const __half2 sf1 = (u & 1) ? __high2half2(p1) : __low2half2(p1);
+            uint32_t e0[4], e1[4], e2[4], e3[4];
+            e2m1x8_to_f16x2(w0[u].x, e0);
+            e2m1x8_to_f16x2(w0[u].y, e1);
+            e2m1x8_to_f16x2(w1[u].x, e2);
+            e2m1x8_to_f16x2(w1[u].y, e3);
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {           // k-step v: channels 4 v .. 4 v + 3 of the block
+              const uint32_t a0 = hmul2h(v < 2 ? e0[2 * v & 3] : e1[2 * v & 3], sf0), a1 = hmul2h(v < 2 ? e2[2 * v & 3] : e3[2 * v & 3], sf1);
+              const uint32_t a2 = hmul2h(v < 2 ? e0[(2 * v & 3) + 1] : e1[(2 * v & 3) + 1], sf0),
+                             a3 = hmul2h(v < 2 ? e2[(2 * v & 3) + 1] : e3[(2 * v & 3) + 1], sf1);
+#pragma unroll
+              for (int q = 0; q < QT; ++q) mma_f16(x[q], a0, a1, a2, a3, qa[q][4 * u + v][0], qa[q][4 * u + v][1]);
+            }
+          }
+        }
+        sum[bi][0] = sum[bi][1] = 0.0f;
+        const int ta = tok0 + 16 * bi + r0, tb = tok0 + 16 * bi + r1;
+#pragma unroll
+        for (int q = 0; q < QT; ++q) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float pa = fast_exp2(fmaf(x[q][k], sc, -le[q][k])), pb = fast_exp2(fmaf(x[q][2 + k], sc, -le[q][k]));
+            if (masked) {                           // (warp-uniform)
+              pa = ta < lim[q][k] && (ta >= from[q][k] || ta < p.sinks) ? pa : 0.0f;
+              pb = tb < lim[q][k] && (tb >= from[q][k] || tb < p.sinks) ? pb : 0.0f;
+            }
+            sum[bi][0] += pa;
+            sum[bi][1] += pb;
+          }
+        }
+      }
+      // the four lanes of a token sum up their rows; lane c ends with block c / 2, row r0 (c even) or r1
+      const bool up = c & 2, odd = c & 1;
+      float s0 = up ? sum[1][0] : sum[0][0], s1 = up ? sum[1][1] : sum[0][1];
+      s0 += __shfl_xor_sync(0xffffffffu, up ? sum[0][0] : sum[1][0], 2);
+      s1 += __shfl_xor_sync(0xffffffffu, up ? sum[0][1] : sum[1][1], 2);
+      const float s = (odd ? s1 : s0) + __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, 1);
+      if (add) wrow[mine] = old + s;
+      ++c_n;
+      __syncwarp();
+      if (f_more) fetch();                          // (into the stage just read)
+      if (++cw.u == cw.end) {
+        more = enter(cw, cw.seq0 + kWtCost + cw.end);
+        break;
+      }
+    }
+  }
+  if (dead)                                         // nothing of this warp's may still be on its way when the CTA ends
+    for (; c_n < f_n; ++c_n) (void)mbar_wait_bounded_u32(bars_a + 8 * (c_n % NS), (c_n / NS) & 1);
+}
+
+template <int D, int LAYOUT, int QT>
+static int launch_weights(const WeightsParams& p, cudaStream_t st) {
+  using Gm = WtGeo<D, LAYOUT>;
+  auto k = weights_kernel<D, LAYOUT, QT>;
+  const size_t smem = kWtWarps * Gm::NS * Gm::STAGE + (kMaxBatch / 32 + 2) * 4;
+  int dev = 0, sms = 0, ctas = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, k, kWtThreads, smem);
+  if (e != cudaSuccess) return record_cuda(e);
+  if (ctas < 1) return HKV_ERR_UNSUPPORTED;
+  return record_cuda(launch_pdl(k, dim3((unsigned)(sms * ctas)), dim3(kWtThreads), smem, st, p));
+}
+
+}  // namespace hkv
+
+extern "C" int hkv_accumulate_weights(const void* q, const void* kd, const void* ksf, const int64_t strides[6], int PS,
+                                      const int32_t* block_tables, int MP, const int32_t* seq_lens, const int32_t* query_start_loc,
+                                      int B, int KVH, int G, int D, int qlmax, float sm_scale, const float* gk, const float* lse,
+                                      float* weights, int64_t w_b, int64_t w_h, int W, int window, int sinks, const float* signs,
+                                      int k8, void* workspace, void* stream) {
+  using namespace hkv;
+  if (B < 0 || MP < 0 || W < 0 || window < 0 || sinks < 0) return HKV_ERR_RANGE;
+  if (B == 0) return HKV_OK;
+  if (!q || !kd || !ksf || !strides || !block_tables || !seq_lens || !query_start_loc || !gk || !lse || !weights) return HKV_ERR_NULL;
+  if ((D != 128 && D != 256) || (k8 && (D != 256 || signs))) return HKV_ERR_UNSUPPORTED;
+  if (KVH < 1 || G < 1 || qlmax < 1 || (int64_t)G * qlmax > 64) return HKV_ERR_UNSUPPORTED;
+  if (PS < 16 || (PS & (PS - 1)) != 0) return HKV_ERR_UNSUPPORTED;
+  if (B > kMaxBatch) return HKV_ERR_RANGE;
+  const int SD = D / 2, SS = D / 16;
+  const int64_t dsp = strides[0], dst = strides[1], dsh = strides[2], ssp = strides[3], sst = strides[4], ssh = strides[5];
+  const bool together = !k8 && sst == dst && dsp == ssp && dsh == ssh && (const uint8_t*)ksf == (const uint8_t*)kd + SD;
+  int layout;
+  if (k8) layout = 2;
+  else if (together && dst == SD + SS) layout = 0;
+  else if (dst == SD && sst == SS) layout = 1;
+  else if (together) layout = 3;
+  else return HKV_ERR_UNSUPPORTED;
+  const int a = layout == 3 && D == 128 ? 7 : 15;
+  if (((uintptr_t)kd | (uintptr_t)dsp | (uintptr_t)dsh | (layout >= 2 ? (uintptr_t)dst : 0)) & a) return HKV_ERR_ALIGN;
+  if (layout == 1 && (((uintptr_t)ksf | (uintptr_t)ssp | (uintptr_t)ssh) & 15)) return HKV_ERR_ALIGN;
+  if (((uintptr_t)q & 15) || (signs && ((uintptr_t)signs & 15)) || (((uintptr_t)lse | (uintptr_t)weights) & 3) ||
+      ((uintptr_t)workspace & 255))
+    return HKV_ERR_ALIGN;
+  if (dsp < 0 || ssp < 0 || dst < 0 || dsp >= (1ll << 31) || ssp >= (1ll << 31) || dst >= (1ll << 31)) return HKV_ERR_RANGE;
+  if (!workspace) {
+    const int rc = noalloc_workspace(&workspace);
+    if (rc != HKV_OK) return rc;
+  }
+  WeightsParams p;
+  p.q = (const __nv_bfloat16*)q;
+  p.kd = (const uint8_t*)kd; p.ksf = (const uint8_t*)ksf;
+  p.dsp = (unsigned)dsp; p.ssp = (unsigned)ssp; p.dst = dst; p.dsh = dsh; p.sst = sst; p.ssh = ssh;
+  p.bt = block_tables; p.seq_lens = seq_lens; p.qsl = query_start_loc; p.gk = gk; p.lse = lse; p.signs = signs;
+  p.w = weights; p.w_b = w_b; p.w_h = w_h;
+  p.status = &((Header*)workspace)->status;
+  p.MP = MP; p.B = B; p.KVH = KVH; p.G = G; p.qlmax = qlmax;
+  p.lps = 0;
+  while ((1 << p.lps) < PS) ++p.lps;
+  const long long reach = (long long)MP * PS;
+  p.max_len = (int)(reach < W ? reach : W);               // (a length beyond the table or the weights is cut there)
+  p.window = window >= p.max_len ? 0 : window;            // (everything is seen)
+  p.sinks = sinks;
+  if (p.window > (1 << 30)) return HKV_ERR_RANGE;
+  p.scale_log2 = sm_scale * 1.4426950408889634f;
+  p.rot_scale = (float)(1.0 / sqrt((double)D));
+  cudaStream_t st = (cudaStream_t)stream;
+  const bool two = G * qlmax > 8;
+  for (p.row0 = 0; p.row0 < G * qlmax; p.row0 += two ? 16 : 8) {
+    int rc;
+    if (D == 128)
+      rc = layout == 0 ? (two ? launch_weights<128, 0, 2>(p, st) : launch_weights<128, 0, 1>(p, st))
+           : layout == 1 ? (two ? launch_weights<128, 1, 2>(p, st) : launch_weights<128, 1, 1>(p, st))
+                         : (two ? launch_weights<128, 3, 2>(p, st) : launch_weights<128, 3, 1>(p, st));
+    else
+      rc = layout == 0 ? (two ? launch_weights<256, 0, 2>(p, st) : launch_weights<256, 0, 1>(p, st))
+           : layout == 1 ? (two ? launch_weights<256, 1, 2>(p, st) : launch_weights<256, 1, 1>(p, st))
+           : layout == 2 ? (two ? launch_weights<256, 2, 2>(p, st) : launch_weights<256, 2, 1>(p, st))
+                         : (two ? launch_weights<256, 3, 2>(p, st) : launch_weights<256, 3, 1>(p, st));
+    if (rc != HKV_OK) return rc;
+  }
+  return HKV_OK;
+}

@@ -140,6 +140,30 @@ def write(key, value, flat, strides, PS, slot_mapping, gk, gv, search=True, sign
     _lib.check(rc, "hkv_write")
 
 
+def _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, signs):
+    """the arguments that the decode calls share; returns (kv heads, query heads of one)"""
+    if query.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
+        raise TypeError("query / out must be bf16")
+    if query.dim() != 3 or out.dim() != 3 or out.shape[1:] != query.shape[1:] or out.shape[0] < query.shape[0]:
+        raise ValueError("query (tokens, heads, head_dim); out (>= tokens, heads, head_dim)")
+    if not query.is_contiguous() or not out.is_contiguous():
+        raise ValueError("query / out must be contiguous")
+    for t in (block_tables, seq_lens, query_start_loc):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise TypeError("block_tables / seq_lens / query_start_loc must be contiguous int32")
+    if block_tables.dim() != 2 or seq_lens.shape != (block_tables.shape[0],) or \
+            query_start_loc.shape != (block_tables.shape[0] + 1,):
+        raise ValueError("block_tables (B, MP); seq_lens (B,); query_start_loc (B + 1,)")
+    KVH = gk.shape[0]
+    HQ = query.shape[1]
+    _check_scales(gk, gv, KVH)
+    if HQ % KVH:
+        raise ValueError("query heads must be a multiple of the kv heads")
+    _need_cuda(query, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, *flat)
+    _check_signs(signs, query.shape[2])
+    return KVH, HQ // KVH
+
+
 def decode_ragged(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, bmm2_scale, gk, gv,
                   qlmax, out, workspace, splits=None, nst=None, ncw=None, min_chunk=None, tw=None, signs=None,
                   k8=False):
@@ -159,27 +183,8 @@ def decode_ragged(query, flat, strides, PS, block_tables, seq_lens, query_start_
         return out
     if k8 and signs is not None:
         raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
-    if query.dtype != torch.bfloat16 or out.dtype != torch.bfloat16:
-        raise TypeError("query / out must be bf16")
-    if query.dim() != 3 or out.dim() != 3 or out.shape[1:] != query.shape[1:] or out.shape[0] < query.shape[0]:
-        raise ValueError("query (tokens, heads, head_dim); out (>= tokens, heads, head_dim)")
-    if not query.is_contiguous() or not out.is_contiguous():
-        raise ValueError("query / out must be contiguous")
-    for t in (block_tables, seq_lens, query_start_loc):
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise TypeError("block_tables / seq_lens / query_start_loc must be contiguous int32")
-    if block_tables.dim() != 2 or seq_lens.shape != (block_tables.shape[0],) or \
-            query_start_loc.shape != (block_tables.shape[0] + 1,):
-        raise ValueError("block_tables (B, MP); seq_lens (B,); query_start_loc (B + 1,)")
-    B, MP = block_tables.shape
-    KVH = gk.shape[0]
-    HQ, D = query.shape[1], query.shape[2]
-    _check_scales(gk, gv, KVH)
-    if HQ % KVH:
-        raise ValueError("query heads must be a multiple of the kv heads")
-    G = HQ // KVH
-    _need_cuda(query, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, *flat)
-    _check_signs(signs, query.shape[2])
+    KVH, G = _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, signs)
+    (B, MP), D = block_tables.shape, query.shape[2]
     S = 0 if splits is None else int(splits)
     kd, ksf, vd, vsf = flat
     st = (C.c_int64 * 6)(*strides)
@@ -248,23 +253,8 @@ def dequant_multi(flat, strides, PS, block_tables, rows, cu, n_rows, n_tokens, o
     _dequant(flat, strides, PS, block_tables, block_tables.shape[1], rows, cu, n_rows, 0, n_tokens, out_k, out_v, k8)
 
 
-def prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, chunk=65536, signs=None,
-            k8=False, workspace=None):
-    """rows: [(table row, q0, q1, L)] with q0 < q1 and L >= 1: query tokens q0 .. q1 - 1 against the first L cached
-    tokens of block_tables[row], query token t of ql seeing keys j < L - ql + t + 1. query (NT, HQ, D) bf16 or fp16
-    contiguous; out (>= NT, HQ, D) bf16 or fp32 contiguous, other rows untouched.
-    out = softmax(q k^T * qk_scale) v * out_scale, the cached values taken without their global scales. `chunk` bounds
-    the tokens that are held as 16-bit operands at a time; the scratch comes from torch's allocator. signs as in
-    decode_ragged. A device-side wait that ran out shows in workspace_status(workspace), without one in
-    workspace_status(None). The reference's counterpart is backend.py:438-543."""
-    rc = (_lib._host or _lib.host()).prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out,
-                                             chunk, signs, k8, workspace)
-    if rc is not None:
-        if rc:
-            _lib.check(rc, "hkv_prefill")
-        return out
-    if k8 and signs is not None:
-        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+def _check_prefill(query, flat, PS, block_tables, rows, KVH, out, signs, workspace):
+    """the arguments that the prefill calls share"""
     if query.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError("query must be bf16 or fp16")
     if query.dtype == torch.float16 and signs is not None:
@@ -292,6 +282,27 @@ def prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, K
         _need_cuda(workspace)
         if workspace.device != query.device or workspace.nbytes < WORKSPACE_HEADER_BYTES:
             raise ValueError("workspace must come from alloc_workspace on the query's device")
+
+
+def prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, chunk=65536, signs=None,
+            k8=False, workspace=None):
+    """rows: [(table row, q0, q1, L)] with q0 < q1 and L >= 1: query tokens q0 .. q1 - 1 against the first L cached
+    tokens of block_tables[row], query token t of ql seeing keys j < L - ql + t + 1. query (NT, HQ, D) bf16 or fp16
+    contiguous; out (>= NT, HQ, D) bf16 or fp32 contiguous, other rows untouched.
+    out = softmax(q k^T * qk_scale) v * out_scale, the cached values taken without their global scales. `chunk` bounds
+    the tokens that are held as 16-bit operands at a time; the scratch comes from torch's allocator. signs as in
+    decode_ragged. A device-side wait that ran out shows in workspace_status(workspace), without one in
+    workspace_status(None). The reference's counterpart is backend.py:438-543."""
+    rc = (_lib._host or _lib.host()).prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out,
+                                             chunk, signs, k8, workspace)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_prefill")
+        return out
+    if k8 and signs is not None:
+        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+    _check_prefill(query, flat, PS, block_tables, rows, KVH, out, signs, workspace)
+    (B, MP), (NT, HQ, D) = block_tables.shape, query.shape
     n = len(rows)
     host_rows = (C.c_int32 * (4 * n))(*[int(x) for r in rows for x in r])
     lib = _lib.load()
@@ -306,6 +317,200 @@ def prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, K
                              None if workspace is None else _ptr(workspace), _stream())
     _lib.check(rc, "hkv_prefill")
     return out
+
+
+def _check_window(window, sinks):
+    if not 0 <= window <= 0x7fffffff or not 0 <= sinks <= 0x7fffffff:
+        raise ValueError("window and sinks are numbers of tokens, not negative (window 0: no window)")
+
+
+def _check_lse(lse, n_tokens, HQ):
+    if lse is None:
+        return
+    _need_cuda(lse)
+    if lse.dtype != torch.float32 or lse.dim() != 2 or lse.shape[0] < n_tokens or lse.shape[1] != HQ or not lse.is_contiguous():
+        raise TypeError("lse must be a contiguous fp32 tensor (>= tokens, heads)")
+
+
+def decode_window(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, bmm2_scale, gk, gv, qlmax, out,
+                  workspace, window, sinks=0, splits=None, signs=None, k8=False, lse=None):
+    """decode_ragged over a sliding window and the first tokens: the query token at position p = L - ql + t of its request sees
+    the keys j <= p with j > p - window or j < sinks (window 0: every j <= p). lse, fp32 (>= NT, HQ) contiguous, takes the
+    rows' log-sum-exps (natural logarithm of the scaled scores; -inf for a row that sees no key). A 16-token block that no row
+    of a request sees is not read: its page may be gone, its table entry any int32. The other arguments, the workspace and
+    what stays untouched are as in decode_ragged."""
+    rc = (_lib._host or _lib.host()).decode_window(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale,
+                                                   bmm2_scale, gk, gv, qlmax, out, workspace, splits, signs, k8, window, sinks, lse)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_decode_window")
+        return out
+    if k8 and signs is not None:
+        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+    window, sinks = int(window), int(sinks)
+    _check_window(window, sinks)
+    KVH, G = _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, signs)
+    _check_lse(lse, query.shape[0], query.shape[1])
+    (B, MP), D = block_tables.shape, query.shape[2]
+    kd, ksf, vd, vsf = flat
+    with torch.cuda.device(query.device):
+        rc = _lib.load().hkv_decode_window(
+            _ptr(query), _ptr(kd), _ptr(ksf), _ptr(vd), _ptr(vsf), (C.c_int64 * 6)(*strides), int(PS), _ptr(block_tables), MP,
+            _ptr(seq_lens), _ptr(query_start_loc), B, KVH, G, D, int(qlmax), float(bmm1_scale), float(bmm2_scale), _ptr(gk), _ptr(gv),
+            _ptr(workspace), workspace.numel() * workspace.element_size(), 0 if splits is None else int(splits),
+            None if signs is None else _ptr(signs), int(bool(k8)), window, sinks, None if lse is None else _ptr(lse), _ptr(out),
+            _stream())
+    _lib.check(rc, "hkv_decode_window")
+    return out
+
+
+def prefill_window(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, window, sinks=0, chunk=65536,
+                   signs=None, k8=False, workspace=None, lse=None):
+    """prefill over a sliding window and the first tokens, with the masks and lse of decode_window. Tokens that no row of a
+    request sees are neither read nor counted by `chunk`. The other arguments are as in prefill."""
+    rc = (_lib._host or _lib.host()).prefill_window(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out,
+                                                    chunk, signs, k8, workspace, window, sinks, lse)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_prefill_window")
+        return out
+    if k8 and signs is not None:
+        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+    window, sinks = int(window), int(sinks)
+    _check_window(window, sinks)
+    _check_prefill(query, flat, PS, block_tables, rows, KVH, out, signs, workspace)
+    (B, MP), (NT, HQ, D) = block_tables.shape, query.shape
+    _check_lse(lse, NT, HQ)
+    n = len(rows)
+    host_rows = (C.c_int32 * (4 * n))(*[int(x) for r in rows for x in r])
+    lib = _lib.load()
+    kd, ksf, vd, vsf = flat
+    with torch.cuda.device(query.device):
+        nb = int(lib.hkv_prefill_window_scratch_bytes(host_rows, n, NT, KVH, HQ // KVH, D, int(chunk), int(signs is not None), window,
+                                                      sinks))
+        scratch = torch.empty(max(nb, 1), dtype=torch.uint8, device=query.device)
+        rc = lib.hkv_prefill_window(
+            _ptr(query), int(query.dtype == torch.float16), _ptr(kd), _ptr(ksf), _ptr(vd), _ptr(vsf), (C.c_int64 * 6)(*strides), int(PS),
+            _ptr(block_tables), B, MP, host_rows, n, NT, KVH, HQ // KVH, D, float(qk_scale), float(out_scale),
+            None if signs is None else _ptr(signs), int(bool(k8)), int(chunk), window, sinks, None if lse is None else _ptr(lse),
+            _ptr(scratch), nb, _ptr(out), int(out.dtype == torch.float32), None if workspace is None else _ptr(workspace), _stream())
+    _lib.check(rc, "hkv_prefill_window")
+    return out
+
+
+def _check_weights(weights, B, name="weights"):
+    _need_cuda(weights)
+    if weights.dtype != torch.float32 or weights.dim() != 3 or weights.shape[0] != B:
+        raise TypeError(f"{name} must be an fp32 tensor (requests, kv heads, positions)")
+    if weights.stride(2) != 1 and weights.shape[2] > 1:
+        raise ValueError(f"{name} needs a contiguous last dimension")
+    if any(s <= 0 for s, n in zip(weights.stride(), weights.shape) if n > 1):
+        raise ValueError(f"{name} must not be broadcast")
+
+
+def accumulate_weights(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, gk, qlmax, lse, weights,
+                       window=0, sinks=0, signs=None, k8=False, workspace=None):
+    """weights[b, h, j] += the sum over the query rows of request b and kv head h that see key j (masks as in decode_window) of
+    exp(score - lse): the attention that the cached tokens get from this call's queries, which `evict` goes by. weights
+    (B, KVH, W) fp32 with a contiguous last dimension; a context is taken up to W, entries that no row sees stay. lse
+    (NT, HQ) fp32, as decode_window and prefill_window leave it for the same queries, masks and scales. Requests with no or more
+    than qlmax query tokens are skipped; (HQ / KVH) * qlmax <= 64. The result does not depend on the order in which the GPU
+    works. query .. query_start_loc, gk, signs, k8 as in decode_window; of the cache only the keys are read."""
+    rc = (_lib._host or _lib.host()).accumulate_weights(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale,
+                                                        gk, qlmax, lse, weights, window, sinks, signs, k8, workspace)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_accumulate_weights")
+        return weights
+    if k8 and signs is not None:
+        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+    window, sinks = int(window), int(sinks)
+    _check_window(window, sinks)
+    if lse is None:
+        raise TypeError("lse must be a contiguous fp32 tensor (>= tokens, heads)")
+    KVH, G = _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gk, query, query, signs)
+    _check_lse(lse, query.shape[0], query.shape[1])
+    (B, MP), D = block_tables.shape, query.shape[2]
+    _check_weights(weights, B)
+    if weights.shape[1] != KVH:
+        raise ValueError("weights (requests, kv heads, positions)")
+    if workspace is not None:
+        _need_cuda(workspace)
+        if workspace.device != query.device or workspace.nbytes < WORKSPACE_HEADER_BYTES:
+            raise ValueError("workspace must come from alloc_workspace on the query's device")
+    with torch.cuda.device(query.device):
+        rc = _lib.load().hkv_accumulate_weights(
+            _ptr(query), _ptr(flat[0]), _ptr(flat[1]), (C.c_int64 * 6)(*strides), int(PS), _ptr(block_tables), MP, _ptr(seq_lens),
+            _ptr(query_start_loc), B, KVH, G, D, int(qlmax), float(bmm1_scale), _ptr(gk), _ptr(lse), _ptr(weights), weights.stride(0),
+            weights.stride(1), weights.shape[2], window, sinks, None if signs is None else _ptr(signs), int(bool(k8)),
+            None if workspace is None else _ptr(workspace), _stream())
+    _lib.check(rc, "hkv_accumulate_weights")
+    return weights
+
+
+def _extent(t):
+    """[first, last) byte address of a tensor's elements"""
+    n = 1 + sum((s - 1) * abs(st) for s, st in zip(t.shape, t.stride())) if t.numel() else 0
+    return t.data_ptr(), t.data_ptr() + n * t.element_size()
+
+
+def evict(flat, strides, PS, D, block_tables, seq_lens, weights, keep, sinks, recent, kept, out_lens, out_tables=None,
+          out_weights=None, k8=False):
+    """Cuts every request to n = min(L, keep) tokens. Per kv head the first `sinks` tokens stay, the last `recent`, and of those
+    between the (keep - sinks - recent) with the largest weights (B, KVH, W) (the lowest position first among equals, a NaN
+    above every number), in their order. Their slots are copied, byte for byte, to the positions 0 .. n - 1 of out_tables
+    (B, OMP) int32: None or a row equal to the request's own moves them in place (no other row of the call may name those pages
+    then); otherwise the pages of a row must be read by nobody in the call, which is what pages shared between requests need.
+    kept (B, KVH, keep) int32 takes the old positions of what stays, -1 from n on; out_lens (B,) int32, another tensor than
+    seq_lens, the new lengths; out_weights (None: the weights themselves) the weights of what stays, and 0 from n to
+    min(L, its width) - 1. Slots from n on keep their bytes. A context is taken up to W."""
+    rc = (_lib._host or _lib.host()).evict(flat, strides, PS, D, block_tables, seq_lens, weights, keep, sinks, recent, kept, out_lens,
+                                           out_tables, out_weights, k8)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_evict")
+        return kept
+    keep, sinks, recent = int(keep), int(sinks), int(recent)
+    if keep < 1 or sinks < 0 or recent < 0 or sinks + recent > keep:
+        raise ValueError("keep >= 1 tokens, of which `sinks` and `recent` (not negative) are part")
+    out_tables = block_tables if out_tables is None else out_tables
+    out_weights = weights if out_weights is None else out_weights
+    for t in (block_tables, out_tables, seq_lens, out_lens, kept):
+        if t.dtype != torch.int32 or not t.is_contiguous():
+            raise TypeError("tables, lengths and kept must be contiguous int32")
+    if block_tables.dim() != 2 or out_tables.dim() != 2:
+        raise ValueError("block_tables (B, MP), out_tables (B, OMP)")
+    B, MP = block_tables.shape
+    if weights.dim() != 3:
+        raise TypeError("weights must be an fp32 tensor (requests, kv heads, positions)")
+    KVH = weights.shape[1]
+    if out_tables.shape[0] != B or seq_lens.shape != (B,) or out_lens.shape != (B,) or kept.shape != (B, KVH, keep):
+        raise ValueError("seq_lens, out_lens (B,); kept (B, KVH, keep); out_tables (B, OMP)")
+    _need_cuda(block_tables, out_tables, seq_lens, out_lens, kept, *flat)
+    _check_weights(weights, B)
+    _check_weights(out_weights, B, "out_weights")
+    if out_weights.shape[1] != KVH or out_weights.shape[2] < keep:
+        raise ValueError("out_weights (requests, kv heads, >= keep positions)")
+    if keep > out_tables.shape[1] * PS:
+        raise ValueError("keep is more than the new pages hold")
+    if any(t.device != weights.device for t in (block_tables, out_tables, seq_lens, out_lens, kept, out_weights, *flat)):
+        raise ValueError("tensors on more than one device")
+    same = out_weights.data_ptr() == weights.data_ptr() and out_weights.stride() == weights.stride()
+    (a0, a1), (b0, b1) = _extent(weights), _extent(out_weights)
+    if not same and a0 < b1 and b0 < a1:
+        raise ValueError("out_weights overlap the weights")
+    (a0, a1), (b0, b1) = _extent(seq_lens), _extent(out_lens)
+    if a0 < b1 and b0 < a1:
+        raise ValueError("out_lens must be another tensor than seq_lens")
+    kd, ksf, vd, vsf = flat
+    with torch.cuda.device(weights.device):
+        rc = _lib.load().hkv_evict(
+            _ptr(kd), _ptr(ksf), _ptr(vd), _ptr(vsf), (C.c_int64 * 6)(*strides), int(PS), _ptr(block_tables), MP, _ptr(seq_lens), B, KVH,
+            int(D), int(bool(k8)), _ptr(weights), weights.stride(0), weights.stride(1), weights.shape[2], keep, sinks, recent,
+            _ptr(out_tables), out_tables.shape[1], _ptr(kept), _ptr(out_lens), _ptr(out_weights), out_weights.stride(0),
+            out_weights.stride(1), out_weights.shape[2], _stream())
+    _lib.check(rc, "hkv_evict")
+    return kept
 
 
 OPT_EARLY_METADATA = 1

@@ -262,6 +262,69 @@ int hkv_selftest_prefill_timeout(const void* q, int q_f16, const void* kd, const
                                  size_t scratch_bytes, void* out, int out_f32, void* workspace, void* stream);
 
 /*
+ * Attention over a sliding window and the first tokens ("sinks") that stay visible: hkv_decode (signs, k8: as hkv_decode_rot,
+ * hkv_decode_k8; signs may be NULL; with k8 ksf is unused but not NULL) and hkv_prefill where the query token at position
+ * p = L - ql + t sees the keys j <= p with j > p - window or j < sinks. window 0: all j <= p. No counterpart in the reference,
+ * which refuses sliding windows.
+ *   lse     fp32 (>= n_tokens, KVH * G) contiguous or NULL: the rows' log-sum-exps (natural logarithm) of the scaled scores;
+ *           -inf for a row that sees no key
+ * A 16-token block (prefill: a token) that no row of a request sees is not read, and its page may be gone: the table entry may
+ * be any number within int32's range, the page's contents anything.
+ * The workspace is hkv_decode's; the scratch of the prefill has hkv_prefill_window_scratch_bytes(..) bytes (0: refused arguments),
+ * and `chunk` counts the tokens that some row sees.
+ */
+int hkv_decode_window(const void* q, const void* kd, const void* ksf, const void* vd, const void* vsf,
+                      const int64_t strides[6], int PS, const int32_t* block_tables, int MP, const int32_t* seq_lens,
+                      const int32_t* query_start_loc, int B, int KVH, int G, int D, int qlmax, float sm_scale, float v_scale,
+                      const float* gk, const float* gv, void* workspace, size_t workspace_bytes, int splits, const float* signs,
+                      int k8, int window, int sinks, float* lse, void* out, void* stream);
+size_t hkv_prefill_window_scratch_bytes(const int32_t* rows, int n_rows, int n_tokens, int KVH, int G, int D, int64_t chunk,
+                                        int rotated, int window, int sinks);
+int hkv_prefill_window(const void* q, int q_f16, const void* kd, const void* ksf, const void* vd, const void* vsf,
+                       const int64_t strides[6], int PS, const int32_t* block_tables, int n_tables, int MP, const int32_t* rows,
+                       int n_rows, int n_tokens, int KVH, int G, int D, float qk_scale, float out_scale, const float* signs,
+                       int k8, int64_t chunk, int window, int sinks, float* lse, void* scratch, size_t scratch_bytes, void* out,
+                       int out_f32, void* workspace, void* stream);
+
+/*
+ * Attention weights that cached tokens gather, what hkv_evict goes by:
+ *   weights[b, h, j] += sum over the query tokens t and group members g that see token j of
+ *                       exp(q . k_j * sm_scale * gk[h] - lse[qsl[b] + t, h * G + g])
+ * with hkv_decode_window's masks (window 0: all keys up to the query token's own). Other entries are not touched. Every entry
+ * is written by one thread in a fixed order: repeated calls give the same bits.
+ *   q .. seq_lens, query_start_loc, signs, k8   as hkv_decode_window; requests with 0 or more than qlmax query tokens are skipped
+ *   lse       fp32 (n_tokens, KVH * G) contiguous, natural logarithm, as hkv_decode_window and hkv_prefill_window leave it
+ *   weights   fp32, entry (b, h, j) at b * w_b + h * w_h + j, W of them per (b, h): a context is taken up to min(MP * PS, W)
+ *   workspace a decode workspace whose status word a wait that ran out would set, or NULL: the built-in one's
+ * G * qlmax <= 64; a pass over the keys serves 8 query rows per kv head, or 16 when there are more than 8.
+ */
+int hkv_accumulate_weights(const void* q, const void* kd, const void* ksf, const int64_t strides[6], int PS,
+                           const int32_t* block_tables, int MP, const int32_t* seq_lens, const int32_t* query_start_loc, int B,
+                           int KVH, int G, int D, int qlmax, float sm_scale, const float* gk, const float* lse, float* weights,
+                           int64_t w_b, int64_t w_h, int W, int window, int sinks, const float* signs, int k8, void* workspace,
+                           void* stream);
+
+/*
+ * Eviction by gathered weight. Of every request and kv head n = min(L, keep) tokens stay: the first `sinks`, the last `recent`
+ * and, of those between, the (keep - sinks - recent) heaviest (the lowest position first among equals; a NaN counts as more
+ * than any number; the two zeros are equal), in their order. A request of at most `keep` tokens keeps all of them.
+ *   kept        int32 (B, KVH, keep): the old positions of the tokens that stay, ascending; -1 from n on
+ *   out_lens    int32 (B): n; not the array seq_lens
+ *   out_tables  int32 (B, OMP): the slots of token kept[b, h, r] (codes and scales of keys and values, byte for byte) are copied
+ *               to position r of this row. A row holds either the request's own first pages (in place; no other row of the call
+ *               may name them), or pages that the call reads from nowhere. May be block_tables itself.
+ *   out_weights fp32, like weights, OW >= keep entries per (b, h): entry r = weights[kept[r]], entries n .. min(L, OW) - 1 = 0.
+ *               Either the weights themselves (the same address and strides) or memory that does not overlap them
+ *   cache       any layout hkv_write accepts whose pointers and strides are multiples of 8 (head_dim 128) or 16 bytes; k8: the
+ *               K8V4 slot, ksf unused but not NULL
+ * A context is taken up to min(MP * PS, W). Slots from n on keep their bytes. keep <= OMP * PS, sinks + recent <= keep.
+ */
+int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t strides[6], int PS, const int32_t* block_tables, int MP,
+              const int32_t* seq_lens, int B, int KVH, int D, int k8, const float* weights, int64_t w_b, int64_t w_h, int W,
+              int keep, int sinks, int recent, const int32_t* out_tables, int OMP, int32_t* kept, int32_t* out_lens,
+              float* out_weights, int64_t ow_b, int64_t ow_h, int OW, void* stream);
+
+/*
  * Self-test of the narrow-float conversions the kernels stand on, no counterpart in the reference (whose CPU tests
  * pin the equivalent bit formulas exhaustively: scripts/kernels/kvfp4/test_kvfp4_cpu.py:54-99, :390-434,
  * test_kvfp4_serving_cpu.py:47-110). Writes to `out` (device memory, 8-byte aligned, HKV_SELFTEST_CODEC_BYTES):
