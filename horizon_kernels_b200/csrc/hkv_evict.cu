@@ -1,18 +1,20 @@
 // Eviction from the paged cache by gathered attention weight: per (request, kv head) the first `sinks` tokens, the last
 // `recent` and, of those between, the heaviest stay, in their order; their slots move to the front of the sequence.
 //
-// One cluster of 1 to 8 CTAs per (request, kv head) does all of it in one launch:
-//   select   the weight that the last token to stay has, by a radix selection over the fp32 values as ordered integers
-//            (11 + 11 + 10 bits). Every CTA counts its share of the tokens into a shared-memory histogram; the CTAs read one
-//            another's through distributed shared memory and all come to the same digit.
-//   list     which tokens stay, ascending: ranks from ballots and the counts of the warps and CTAs before, written to `kept`
-//   move     the kept tokens' slots and weights to their new places, byte for byte
+// Two launches:
+//   select_kernel  which tokens stay. A cluster of 1 to 8 CTAs per (request, kv head) finds the weight of the last one by a radix
+//                  selection over the fp32 values as ordered integers (11 + 11 + 10 bits): every CTA counts its share of the
+//                  tokens into a shared-memory histogram, the CTAs read one another's through distributed shared memory and all
+//                  come to the same digit. Two passes do unless weights agree in 22 bits. Ranks come from ballots and the counts
+//                  of the warps and CTAs before; `kept` takes the positions in ascending order.
+//   move_kernel    the kept tokens' slots and weights to their new places, byte for byte
 // No sums are formed and nothing depends on an order of atomics: the histogram counts are whole numbers.
 //
-// In place (a request's new pages are its own first ones) a slot may be read by one CTA and written by another. A token's rank
-// never exceeds its position, so the moves are cut into rounds of ascending rank, a round's slots are all read before the first
-// of them is written (cluster barrier between), and what a round writes lies at or below every position that later rounds read
-// only where it has been read already: position j of rank r' >= r(round end) > any rank written so far.
+// In place (a request's new pages are its own first ones) one CTA may write a slot that another one reads. A token's rank never
+// exceeds its position, so the moves are cut into rounds of ascending rank by ONE cluster per (request, kv head): a round's slots
+// are all read before the first of them is written (cluster barrier between), and later rounds read positions that are at least
+// as high as their ranks, above every rank written so far. Moves to other pages need no order: all warps work on their own.
+#include <algorithm>
 #include <type_traits>
 
 #include "hkv_common.cuh"
@@ -21,10 +23,12 @@ namespace hkv {
 
 int record_cuda(cudaError_t e);
 
-constexpr int kEvThreads = 512, kEvWarps = kEvThreads / 32;
+constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
 constexpr int kEvBins = 2048;
 constexpr int kEvCluster = 8;
-constexpr int kEvKeys = 20480;                      // weights that a CTA keeps in shared memory (80 KB; the rest is read again)
+constexpr int kSelRegs = 32;                        // weights of a thread that stay in registers
+constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
+constexpr int kMoveCtas = 592;
 
 struct EvictParams {
   uint8_t* kd;
@@ -40,7 +44,8 @@ struct EvictParams {
   float* ow;
   long long w_b, w_h, ow_b, ow_h;                   // element strides of the weights
   int* kept;
-  int MP, OMP, lps, KVH, keep, sinks, recent, max_len, OW, cap;
+  int MP, OMP, lps, KVH, keep, sinks, recent, max_len, OW;
+  int bulk, split;                                  // a tile's new rows lie back to back and 16-byte aligned; codes apart from scales
 };
 
 __device__ __forceinline__ uint32_t cluster_size() {
@@ -64,6 +69,23 @@ __device__ __forceinline__ int peer_load(const int* p, uint32_t rank) {   // *p 
   return v;
 }
 
+__device__ __forceinline__ int4 peer_load4(const int* p, uint32_t rank) {
+  uint32_t a;
+  int4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+// sum of v over the lanes up to this one
+__device__ __forceinline__ int scan_warp(int v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int t = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += t;
+  }
+  return v;
+}
+
 // fp32 -> unsigned integers of the same order; both zeros are one, every NaN lies above infinity
 __device__ __forceinline__ uint32_t weight_key(float w) {
   const uint32_t u = __float_as_uint(w);
@@ -72,207 +94,302 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// PB: bytes of a piece of a slot (8 at head_dim 128, whose rows are 8-byte aligned; 16 at 256). A slot's side is NP pieces of
-// codes (FP8 keys: 16) and one of scales; NP + 1 lanes copy a side.
-template <int D, bool K8>
-struct EvGeo {
-  static constexpr int PB = D == 128 ? 8 : 16;
-  static constexpr int NP = 8;                      // pieces of D / 2 code bytes
-  static constexpr int LANES = K8 ? 16 + NP + 1 : 3 * (NP + 1);      // a token; or three sides of tokens
-  static constexpr int SIDES = K8 ? 1 : 3;          // sides (K8: tokens) a warp copies at a time
-  static constexpr int U = 8;                       // of those in flight
-  static constexpr int TOK = K8 ? U : U * 3 / 2;    // tokens of a warp and round
-};
-
-template <int D, bool K8>
-__global__ void __launch_bounds__(kEvThreads, 2) evict_kernel(const EvictParams p) {
-  using Gm = EvGeo<D, K8>;
-  using Piece = typename std::conditional<Gm::PB == 8, uint2, uint4>::type;
-  extern __shared__ uint32_t keys[];
-  __shared__ int hist[kEvBins];
-  __shared__ int wsum[kEvWarps], counts[2 * kEvWarps], totals[2], found[3];
+// A warp has a run of the CTA's tokens, 32 at a time, a lane one of them: the order of (warp, turn, lane) is that of the tokens.
+// The first kSelRegs turns stay in registers from pass to pass, further ones (contexts beyond 8 x 16384 tokens) are read again.
+__global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParams p) {
+  __shared__ __align__(16) int hist[kEvBins];
+  __shared__ int wsum[kSelWarps], counts[2 * kSelWarps], totals[2], found[3];
   const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5;
   const int nc = (int)cluster_size(), cr = (int)cluster_rank(), h = blockIdx.y, b = blockIdx.z;
   pdl_wait();
   pdl_launch_dependents();
   const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_len), n = min(L, p.keep);
   const float* w = p.w + b * p.w_b + h * p.w_h;
-  float* ow = p.ow + b * p.ow_b + h * p.ow_h;
   int* kept = p.kept + ((long long)b * p.KVH + h) * p.keep;
-  const int* bt = p.bt + (long long)b * p.MP;
-  const int* obt = p.out_bt + (long long)b * p.OMP;
+  const int t0 = cr * kSelThreads + tid, step = nc * kSelThreads;
   if (cr == 0 && h == 0 && tid == 0) p.out_lens[b] = n;
-
-  if (L <= p.keep) {
-    for (int r = cr * kEvThreads + tid; r < p.keep; r += nc * kEvThreads) kept[r] = r < n ? r : -1;
-  } else {
-    const int mid = L - p.sinks - p.recent, need = p.keep - p.sinks - p.recent;      // candidates, of which so many stay
-    const int share = (mid + nc - 1) / nc, m0 = min(mid, cr * share), m1 = min(mid, m0 + share), first = p.sinks + m0, cnt = m1 - m0;
-    for (int i = tid; i < cnt; i += kEvThreads)
-      if (i < p.cap) keys[i] = weight_key(w[first + i]);
-    auto key = [&](int i) { return i < p.cap ? keys[i] : weight_key(w[first + i]); };
-    uint32_t prefix = 0;                            // the leading bits of the threshold
-    int left = need, shift = 32;                    // tokens to take among those that share them
-    const int widths[3] = {11, 11, 10};
+  if (L <= p.keep) {                                // (the whole cluster leaves)
+    for (int r = t0; r < p.keep; r += step) kept[r] = r < n ? r : -1;
+    return;
+  }
+  for (int i = t0; i < p.sinks; i += step) kept[i] = i;
+  for (int i = t0; i < p.recent; i += step) kept[p.keep - p.recent + i] = L - p.recent + i;
+  const int mid = L - p.sinks - p.recent, need = p.keep - p.sinks - p.recent;        // candidates, of which so many stay
+  if (need == 0) return;
+  const int share = (mid + nc - 1) / nc, m0 = min(mid, cr * share), cnt = min(mid, m0 + share) - m0;
+  const int turns = ((cnt + kSelWarps - 1) / kSelWarps + 31) >> 5;                   // of a warp
+  const int i0 = wp * turns * 32 + lane, first = p.sinks + m0 + i0;                  // this lane's first token, of the CTA's and of all
+  const float* wl = w + first;
+  // (0: no token; no weight has this key)
+  auto fetch = [&](int u) { return i0 + 32 * u < cnt ? weight_key(wl[32 * u]) : 0u; };
+  uint32_t key[kSelRegs];
+#pragma unroll
+  for (int u = 0; u < kSelRegs; ++u) key[u] = u < turns ? fetch(u) : 0u;
+  auto each = [&](auto f) {                         // f(turn, key) over this lane's tokens
+#pragma unroll
+    for (int g = 0; g < kSelRegs; g += 4)
+      if (g < turns) {
+#pragma unroll
+        for (int u = g; u < g + 4; ++u) f(u, key[u]);
+      }
 #pragma unroll 1
-    for (int pass = 0; pass < 3 && need > 0; ++pass) {
-      const int from = shift;
-      shift -= widths[pass];
-      for (int i = tid; i < kEvBins; i += kEvThreads) hist[i] = 0;
-      __syncthreads();
-      for (int i = tid; i < cnt; i += kEvThreads) {
-        const uint32_t k = key(i);
-        if (from == 32 || k >> from == prefix) atomicAdd(&hist[(k >> shift) & ((1 << widths[pass]) - 1)], 1);
-      }
-      cluster_sync();
-      // the bins of all CTAs; thread t has the bins 4 t .. 4 t + 3 counted from the top
-      int c[4], s = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int bin = kEvBins - 1 - (4 * tid + u);
-        c[u] = 0;
-        for (int r = 0; r < nc; ++r) c[u] += peer_load(&hist[bin], (cr + r) % nc);
-        s += c[u];
-      }
-      int incl = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
-      }
-      if (lane == 31) wsum[wp] = incl;
-      __syncthreads();
-      int above = incl - s;
-      for (int i = 0; i < wp; ++i) above += wsum[i];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if (above < left && left <= above + c[u]) {
-          found[0] = kEvBins - 1 - (4 * tid + u);
-          found[1] = left - above;
-          found[2] = c[u];
-        }
-        above += c[u];
-      }
-      cluster_sync();                               // (the histograms have been read)
-      prefix = (prefix << widths[pass]) | (uint32_t)found[0];
-      left = found[1];
-      if (found[2] == left) break;                  // the whole bin stays
-    }
-    // who stays: key >> shift above the prefix, and the first `left` of those equal to it
-    auto rel = [&](int i) {                         // 2: above, 1: equal, 0: below
-      if (need == 0) return 0;
-      const uint32_t k = key(i) >> shift;
-      return k > prefix ? 2 : k == prefix ? 1 : 0;
-    };
-    const int part = (cnt + kEvWarps - 1) / kEvWarps, i0 = min(cnt, wp * part), i1 = min(cnt, i0 + part);
-    int gt = 0, eq = 0;
-    for (int i = i0; i < i1; i += 32) {
-      const int v = i + lane < i1 ? rel(i + lane) : 0;
-      gt += __popc(__ballot_sync(0xffffffffu, v == 2));
-      eq += __popc(__ballot_sync(0xffffffffu, v == 1));
-    }
-    if (lane == 0) {
-      counts[2 * wp] = gt;
-      counts[2 * wp + 1] = eq;
-    }
+    for (int u = kSelRegs; u < turns; ++u) f(u, fetch(u));
+  };
+  uint32_t prefix = 0;                              // the leading bits of the threshold
+  int left = need, shift = 32;                      // tokens to take among those that share them
+  bool ties = true;
+#pragma unroll 1
+  for (int pass = 0; pass < 3 && ties; ++pass) {
+    const int from = shift, width = pass < 2 ? 11 : 10;
+    shift -= width;
+    reinterpret_cast<int4*>(hist)[tid] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    if (tid < 2) {
-      int t = 0;
-      for (int i = 0; i < kEvWarps; ++i) t += counts[2 * i + tid];
-      totals[tid] = t;
+    if (pass == 0) {
+      each([&](int, uint32_t k) {
+        if (k) atomicAdd(&hist[k >> 21], 1);
+      });
+    } else {
+      const uint32_t mask = (1u << width) - 1;
+      each([&](int, uint32_t k) {
+        if (k >> from == prefix) atomicAdd(&hist[(k >> shift) & mask], 1);
+      });
+    }
+    // the bins of all CTAs; thread t has the bins 4 t .. 4 t + 3 counted from the top
+    int c[4] = {0, 0, 0, 0};
+    const int top = kEvBins - 4 - 4 * tid;
+    auto add = [&](const int4& v) { c[0] += v.w; c[1] += v.z; c[2] += v.y; c[3] += v.x; };
+    if (nc == 1) {
+      __syncthreads();
+      add(*reinterpret_cast<const int4*>(hist + top));
+    } else {
+      cluster_sync();
+      int4 v[kEvCluster];                           // (a CTA begins with its own: they do not all ask the same one)
+#pragma unroll
+      for (int r = 0; r < kEvCluster; ++r) v[r] = r < nc ? peer_load4(hist + top, (cr + r) & (nc - 1)) : make_int4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < kEvCluster; ++r) add(v[r]);
+    }
+    const int s = c[0] + c[1] + c[2] + c[3], incl = scan_warp(s, lane);
+    if (lane == 31) wsum[wp] = incl;
+    __syncthreads();
+    int above = incl - s + __reduce_add_sync(0xffffffffu, lane < wp ? wsum[lane] : 0);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (above < left && left <= above + c[u]) {
+        found[0] = top + 3 - u;
+        found[1] = left - above;
+        found[2] = c[u];
+      }
+      above += c[u];
+    }
+    if (nc == 1) __syncthreads(); else cluster_sync();   // (the histograms have been read)
+    prefix = (prefix << width) | (uint32_t)found[0];
+    left = found[1];
+    ties = found[2] != left;                        // (else the whole bin stays)
+  }
+  // who stays: keys above `low`, and with ties (all 32 bits are known then) the first `left` of those equal to it
+  const uint32_t low = ties ? prefix : (prefix << shift) - 1;
+  int gt = 0, eq = 0;
+  each([&](int, uint32_t k) {
+    gt += k > low;
+    eq += k == low;
+  });
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (lane == 0) {
+    counts[2 * wp] = gt;
+    counts[2 * wp + 1] = eq;
+  }
+  __syncthreads();
+  // of the tokens before this warp's
+  const int gw = lane < kSelWarps ? counts[2 * lane] : 0, ew = lane < kSelWarps ? counts[2 * lane + 1] : 0;
+  int gb = __reduce_add_sync(0xffffffffu, lane < wp ? gw : 0), eb = __reduce_add_sync(0xffffffffu, lane < wp ? ew : 0);
+  if (nc > 1) {
+    if (wp == 0) {
+      const int gt_all = __reduce_add_sync(0xffffffffu, gw), eq_all = __reduce_add_sync(0xffffffffu, ew);
+      if (lane == 0) {
+        totals[0] = gt_all;
+        totals[1] = eq_all;
+      }
     }
     cluster_sync();
-    int gb = 0, eb = 0;
-    for (int r = 0; r < cr; ++r) {
-      gb += peer_load(&totals[0], r);
-      eb += peer_load(&totals[1], r);
-    }
-    for (int i = 0; i < wp; ++i) {
-      gb += counts[2 * i];
-      eb += counts[2 * i + 1];
-    }
-    const unsigned below = (1u << lane) - 1;
-    for (int i = i0; i < i1; i += 32) {
-      const int v = i + lane < i1 ? rel(i + lane) : 0;
-      const unsigned bg = __ballot_sync(0xffffffffu, v == 2), be = __ballot_sync(0xffffffffu, v == 1);
-      const int g = gb + __popc(bg & below), e = eb + __popc(be & below);
-      if (v == 2 || (v == 1 && e < left)) kept[p.sinks + g + min(e, left)] = first + i + lane;
+    gb += __reduce_add_sync(0xffffffffu, lane < cr ? peer_load(&totals[0], lane) : 0);
+    eb += __reduce_add_sync(0xffffffffu, lane < cr ? peer_load(&totals[1], lane) : 0);
+  }
+  const unsigned below = (1u << lane) - 1;
+  if (!ties) {
+    int r = p.sinks + gb;
+    each([&](int u, uint32_t k) {
+      const unsigned bg = __ballot_sync(0xffffffffu, k > low);
+      if (k > low) kept[r + __popc(bg & below)] = first + 32 * u;
+      r += __popc(bg);
+    });
+  } else {
+    each([&](int u, uint32_t k) {
+      const unsigned bg = __ballot_sync(0xffffffffu, k > low), be = __ballot_sync(0xffffffffu, k == low);
+      const int er = eb + __popc(be & below);
+      if (k > low || (k == low && er < left)) kept[p.sinks + gb + __popc(bg & below) + min(er, left)] = first + 32 * u;
       gb += __popc(bg);
       eb += __popc(be);
-    }
-    for (int i = cr * kEvThreads + tid; i < p.sinks; i += nc * kEvThreads) kept[i] = i;
-    for (int i = cr * kEvThreads + tid; i < p.recent; i += nc * kEvThreads) kept[p.keep - p.recent + i] = L - p.recent + i;
+    });
   }
-  cluster_sync();                                   // the list is complete, also where another CTA wrote it
-
-  if (n > 0) {
-    // a request's own first pages, or weights that move within their row: read before written
-    const bool in_place = ow == w || __ldg(bt) == __ldg(obt);
-    const int PSM = (1 << p.lps) - 1;
-    const long long dh = h * p.dsh, sh = h * p.ssh;
-    // what this lane copies of a (token, side): pieces 0 .. 7 codes, 8 scales; K8: 0 .. 15 keys, then the same of the values
-    const int sub = K8 ? 0 : lane / (Gm::NP + 1), pc = K8 ? lane : lane - sub * (Gm::NP + 1);
-    const bool on = lane < Gm::LANES;
-    constexpr int ROUND = kEvWarps * Gm::TOK;
-    for (int r0 = cr * ROUND; r0 - cr * ROUND < n; r0 += nc * ROUND) {
-      Piece v[Gm::U];
-      uint8_t* to[Gm::U];
-      const int rw = r0 + wp * Gm::TOK;
-#pragma unroll
-      for (int u = 0; u < Gm::U; ++u) {
-        const int item = u * Gm::SIDES + sub, r = rw + (K8 ? item : item >> 1), side = K8 ? 0 : item & 1;
-        to[u] = nullptr;
-        if (on && r < n) {
-          const int j = __ldcg(kept + r);
-          const long long pg = __ldg(bt + (j >> p.lps)), og = __ldg(obt + (r >> p.lps));
-          const int so = j & PSM, oo = r & PSM;
-          const bool scales = K8 ? pc == 24 : pc == 8;
-          uint8_t* base;
-          if (K8) base = pc < 16 ? p.kd + pc * 16 : scales ? p.vsf : p.vd + (pc - 16) * 16;
-          else base = scales ? (side ? p.vsf : p.ksf) : (side ? p.vd : p.kd) + pc * Gm::PB;
-          const uint8_t* from;
-          if (scales) {
-            from = base + pg * p.ssp + so * p.sst + sh;
-            to[u] = base + og * p.ssp + oo * p.sst + sh;
-          } else {
-            from = base + pg * p.dsp + so * p.dst + dh;
-            to[u] = base + og * p.dsp + oo * p.dst + dh;
-          }
-          if (from == to[u]) to[u] = nullptr;       // it stays where it is
-          else v[u] = *reinterpret_cast<const Piece*>(from);
-        }
-      }
-      float wv = 0.0f;
-      const int rt = rw + lane;
-      const bool mine = lane < Gm::TOK && rt < n;
-      if (mine) wv = w[__ldcg(kept + rt)];
-      if (in_place) cluster_sync();
-#pragma unroll
-      for (int u = 0; u < Gm::U; ++u)
-        if (to[u]) *reinterpret_cast<Piece*>(to[u]) = v[u];
-      if (mine) ow[rt] = wv;
-    }
-    // (CTAs beyond the last round's ranks have nothing to read but meet the others at every barrier: the loop's bound is the
-    // cluster's first rank of the round)
-  }
-  for (int r = n + cr * kEvThreads + tid; r < min(L, p.OW); r += nc * kEvThreads) ow[r] = 0.0f;
+  if (nc > 1) cluster_sync();                       // (the totals have been read)
 }
 
+// A tile of moves: 16 tokens whose new places are one 16-token block of a page. A warp gathers their rows into shared memory,
+// piece by piece (PB bytes: 8 at head_dim 128, whose rows are 8-byte aligned, 16 at 256; a row is 8 pieces of codes, FP8 keys
+// 16 before them, and one of scales), and writes the tile out: with one bulk copy a side where rows lie back to back in the
+// cache, else piece by piece. The rows hold no registers on their way, so that a warp has the next tile in flight while it
+// writes this one. 64 requests of 1.5k to 16k tokens to 2048, 8 kv heads x 128: 75 us with the rows in registers and 8-byte
+// stores (bound by the L1's work on them and the address arithmetic), MEASURE now.
 template <int D, bool K8>
-static int launch_evict(const EvictParams& p, int B, int nc, size_t smem, cudaStream_t st) {
-  auto k = evict_kernel<D, K8>;
-  int rc = record_cuda(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvKeys * 4));
-  if (rc != HKV_OK) return rc;
+struct EvGeo {
+  static constexpr int PB = D == 128 ? 8 : 16;
+  static constexpr int NP = K8 ? 25 : 9;            // pieces of a row
+  static constexpr int ROWS = K8 ? 16 : 32;         // rows of a tile: keys, then values (K8: both in one)
+  static constexpr int PIECES = ROWS * NP, TURNS = (PIECES + 31) / 32;
+  static constexpr int TILE = PIECES * PB;
+  static constexpr int WARP = 2 * (TILE + 256);     // shared memory of a warp: two tiles, the rows' old places (codes, scales)
+  static constexpr int SMEM = kMoveWarps * WARP;
+};
+
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+// CLUSTER: calls in place; else a row in place, which the caller may mix in, is one CTA's work
+template <int D, bool K8, bool CLUSTER>
+__global__ void __launch_bounds__(kMoveThreads, D == 128 ? 4 : 2) move_kernel(const EvictParams p) {
+  using Gm = EvGeo<D, K8>;
+  constexpr int PB = Gm::PB, NP = Gm::NP;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5, h = blockIdx.y, b = blockIdx.z;
+  const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_len), n = min(L, p.keep);      // (older than the preceding launch)
+  const int* bt = p.bt + (long long)b * p.MP;
+  const int* obt = p.out_bt + (long long)b * p.OMP;
+  pdl_wait();
+  pdl_launch_dependents();
+  if (n == 0) return;
+  const float* w = p.w + b * p.w_b + h * p.w_h;
+  float* ow = p.ow + b * p.ow_b + h * p.ow_h;
+  const int* kept = p.kept + ((long long)b * p.KVH + h) * p.keep;
+  const bool own_pages = __ldg(bt) == __ldg(obt), own_weights = ow == w, in_place = own_pages || own_weights;
+  if (own_pages && own_weights && L <= p.keep) return;             // everything stays where it is
+  const int cl = CLUSTER ? (int)cluster_size() : 1;
+  if (in_place && (int)blockIdx.x >= cl) return;    // one cluster's work
+  const int ctas = in_place ? cl : (int)gridDim.x, PSM = (1 << p.lps) - 1;
+  const long long dh = h * p.dsh, sh = h * p.ssh;
+  uint8_t* const mine = smem + wp * Gm::WARP;
+  const uint32_t tiles_a = smem_u32(mine);
+  long long* const places = reinterpret_cast<long long*>(mine + 2 * Gm::TILE);           // [tile][codes, scales][16]
+  // piece x of a tile: its row, its place in the row, and where that lies in shared memory
+  auto row_of = [](int x) { return x / NP; };
+  auto base_of = [&](int row, int pc) -> uint8_t* {
+    if (K8) return pc < 16 ? p.kd + pc * 16 : pc == 24 ? p.vsf : p.vd + (pc - 16) * 16;
+    return pc == 8 ? (row < 16 ? p.ksf : p.vsf) : (row < 16 ? p.kd : p.vd) + pc * PB;
+  };
+  auto at = [&](int x, int row, int pc) {           // (split: codes and scales have regions of their own)
+    return K8 || !p.split ? x * PB : pc < 8 ? row * 8 * PB + pc * PB : (32 * 8 + row) * PB;
+  };
+  // The old place of a token hangs on two loads one after the other (position, page), its rows on those: the positions are
+  // fetched two tiles ahead, the rows one. (Every CTA of a cluster takes every round, so that all of them meet at its barrier.)
+  const int stride = ctas * kMoveWarps * 16;
+  int rt = (blockIdx.x * kMoveWarps + wp) * 16;
+  auto position = [&](int r) { return lane < 16 && r + lane < n ? __ldg(kept + r + lane) : -1; };
+  int j = position(rt);
+  float wv = 0.0f, wn = 0.0f;
+  bool still = false, still_n = false;              // (the tile stays where it is)
+  auto gather = [&](int buf, int r, float& weight, bool& same) {      // the rows of tokens r .. r + 15, at positions j
+    const int left = n - r;
+    // (positions ascend: the tile's last one tells whether all of them are their ranks)
+    same = own_pages && left >= 16 && __shfl_sync(0xffffffffu, j, 15) == r + 15;
+    if (left > 0 && !same) {
+      if (j >= 0) {
+        const long long pg = __ldg(bt + (j >> p.lps));
+        const int so = j & PSM;
+        places[buf * 32 + lane] = pg * p.dsp + so * p.dst + dh;
+        places[buf * 32 + 16 + lane] = pg * p.ssp + so * p.sst + sh;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int u = 0; u < Gm::TURNS; ++u) {
+        const int x = u * 32 + lane, row = row_of(x), pc = x - row * NP, i = row & 15;
+        const bool scales = pc == NP - 1;
+        if ((Gm::PIECES % 32 == 0 || x < Gm::PIECES) && i < left)
+          cp_async<PB>(tiles_a + buf * Gm::TILE + at(x, row, pc), base_of(row, pc) + places[buf * 32 + (scales ? 16 : 0) + i]);
+      }
+    }
+    if (j >= 0) weight = w[j];
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    j = position(r + stride);
+  };
+  gather(0, rt, wv, still);
+  int buf = 0;
+  for (int base = 0; base < n; base += stride, rt += stride, buf ^= 1) {
+    // (the copy out of the other buffer, a turn ago, must have read it)
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+    gather(buf ^ 1, rt + stride, wn, still_n);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    if (in_place) {
+      if (CLUSTER) cluster_sync();
+      else __syncthreads();
+    }
+    const int left = n - rt;
+    if (left > 0 && !still) {
+      const long long og = __ldg(obt + (rt >> p.lps));
+      const int oo = rt & PSM;
+      const long long to = og * p.dsp + oo * p.dst + dh, to_s = og * p.ssp + oo * p.sst + sh;
+      const uint32_t tile = tiles_a + buf * Gm::TILE;
+      if (p.bulk && left >= 16) {
+        fence_proxy_async();
+        __syncwarp();
+        if (K8) {
+          if (lane == 0) bulk_s2g(p.kd + to, tile, Gm::TILE);
+        } else if (!p.split) {
+          if (lane < 2) bulk_s2g((lane ? p.vd : p.kd) + to, tile + lane * 16 * NP * PB, 16 * NP * PB);
+        } else if (lane < 2) {
+          bulk_s2g((lane ? p.vd : p.kd) + to, tile + lane * 16 * 8 * PB, 16 * 8 * PB);
+          bulk_s2g((lane ? p.vsf : p.ksf) + to_s, tile + (32 * 8 + lane * 16) * PB, 16 * PB);
+        }
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      } else {
+        __syncwarp();
+#pragma unroll 3
+        for (int u = 0; u < Gm::TURNS; ++u) {
+          const int x = u * 32 + lane, row = row_of(x), pc = x - row * NP, i = row & 15;
+          if ((Gm::PIECES % 32 == 0 || x < Gm::PIECES) && i < left) {
+            uint8_t* d = base_of(row, pc) + (pc == NP - 1 ? to_s + i * p.sst : to + i * p.dst);
+            const uint32_t s = tile + at(x, row, pc);
+            if (PB == 8) *reinterpret_cast<uint2*>(d) = lds64(s);
+            else *reinterpret_cast<uint4*>(d) = lds128(s);
+          }
+        }
+      }
+    }
+    if (lane < 16 && rt + lane < n) ow[rt + lane] = wv;
+    wv = wn;
+    still = still_n;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  // (in place: the last barrier lies behind every read)
+  for (int r = n + blockIdx.x * kMoveThreads + tid; r < min(L, p.OW); r += ctas * kMoveThreads) ow[r] = 0.0f;
+}
+
+template <typename K>
+static int launch_clusters(K k, const EvictParams& p, unsigned x, unsigned y, unsigned z, unsigned cluster, int threads, size_t smem,
+                           cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)nc, (unsigned)p.KVH, (unsigned)B);
-  cfg.blockDim = dim3(kEvThreads);
+  cfg.gridDim = dim3(x, y, z);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = (unsigned)nc;
+  attr[1].val.clusterDim.x = cluster;
   attr[1].val.clusterDim.y = 1;
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
@@ -311,17 +428,37 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   p.w = weights; p.ow = out_weights; p.w_b = w_b; p.w_h = w_h; p.ow_b = ow_b; p.ow_h = ow_h;
   p.kept = kept;
   p.MP = MP; p.OMP = OMP; p.KVH = KVH; p.keep = keep; p.sinks = sinks; p.recent = recent; p.OW = OW;
+  // rows back to back, and bulk copies' 16-byte alignment (a tile begins at a multiple of 16 tokens)
+  const int64_t SD = k8 ? D + D / 2 : D / 2, SS = D / 16, row = SD + SS;
+  const bool al16 = (((uintptr_t)kd | (uintptr_t)vd | (uintptr_t)strides[0] | (uintptr_t)strides[2]) & 15) == 0;
+  const bool together = strides[1] == row && strides[4] == row && strides[0] == strides[3] && strides[2] == strides[5];
+  const bool slots = k8 ? together && (uint8_t*)vd == (uint8_t*)kd + D && (uint8_t*)vsf == (uint8_t*)vd + D / 2
+                        : together && (uint8_t*)ksf == (uint8_t*)kd + SD && (uint8_t*)vsf == (uint8_t*)vd + SD;
+  p.split = !k8 && !slots && strides[1] == SD && strides[4] == SS &&
+            (((uintptr_t)ksf | (uintptr_t)vsf | (uintptr_t)strides[3] | (uintptr_t)strides[5]) & 15) == 0;
+  p.bulk = al16 && (slots || p.split);
+  p.split = p.split && p.bulk;
   p.lps = 0;
   while ((1 << p.lps) < PS) ++p.lps;
   const long long reach = (long long)MP * PS;
   p.max_len = (int)(reach < W ? reach : W);               // (a length beyond the table or the weights is cut there)
   const long long pairs = (long long)B * KVH;
   int nc = kEvCluster;
-  while (nc > 1 && (pairs * nc > 600 || p.max_len < nc * 1024)) nc /= 2;
-  const int share = (p.max_len + nc - 1) / nc;
-  p.cap = share < kEvKeys ? share : kEvKeys;
-  const size_t smem = (size_t)(p.cap > 0 ? p.cap : 1) * 4;
+  while (nc > 1 && (pairs * nc > 600 || p.max_len < nc * 2048)) nc /= 2;
   cudaStream_t st = (cudaStream_t)stream;
-  return k8 ? launch_evict<256, true>(p, B, nc, smem, st)
-            : D == 128 ? launch_evict<128, false>(p, B, nc, smem, st) : launch_evict<256, false>(p, B, nc, smem, st);
+  int rc = launch_clusters(select_kernel, p, nc, KVH, B, nc, kSelThreads, 0, st);
+  if (rc != HKV_OK) return rc;
+  const bool cluster = out_tables == block_tables || out_weights == weights;
+  void (*mk)(const EvictParams) = nullptr;
+  if (k8) mk = cluster ? move_kernel<256, true, true> : move_kernel<256, true, false>;
+  else if (D == 128) mk = cluster ? move_kernel<128, false, true> : move_kernel<128, false, false>;
+  else mk = cluster ? move_kernel<256, false, true> : move_kernel<256, false, false>;
+  const int smem = k8 ? EvGeo<256, true>::SMEM : D == 128 ? EvGeo<128, false>::SMEM : EvGeo<256, false>::SMEM;
+  rc = record_cuda(cudaFuncSetAttribute((const void*)mk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (rc != HKV_OK) return rc;
+  if (cluster) return launch_clusters(mk, p, kEvCluster, KVH, B, kEvCluster, kMoveThreads, smem, st);
+  // as many CTAs per (request, kv head) as find work at once
+  const long long most = keep < p.max_len ? keep : p.max_len, round = kMoveWarps * 16;
+  const long long x = std::max(1ll, std::min((most + round - 1) / round, (kMoveCtas + pairs - 1) / pairs));
+  return record_cuda(launch_pdl(mk, dim3((unsigned)x, (unsigned)KVH, (unsigned)B), dim3(kMoveThreads), smem, st, p));
 }
