@@ -69,12 +69,10 @@ __device__ __forceinline__ int peer_load(const int* p, uint32_t rank) {   // *p 
   return v;
 }
 
-__device__ __forceinline__ int4 peer_load4(const int* p, uint32_t rank) {
+__device__ __forceinline__ void peer_store(int* p, uint32_t rank, int v) {
   uint32_t a;
-  int4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
 // sum of v over the lanes up to this one
 __device__ __forceinline__ int scan_warp(int v, int lane) {
@@ -98,7 +96,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // The first kSelRegs turns stay in registers from pass to pass, further ones (contexts beyond 8 x 16384 tokens) are read again.
 __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParams p) {
   __shared__ __align__(16) int hist[kEvBins];
-  __shared__ int wsum[kSelWarps], counts[2 * kSelWarps], totals[2], found[3];
+  __shared__ int wsum[kSelWarps], counts[2 * kSelWarps], totals[2], found[3], slice;
   const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5;
   const int nc = (int)cluster_size(), cr = (int)cluster_rank(), h = blockIdx.y, b = blockIdx.z;
   pdl_wait();
@@ -124,7 +122,15 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
   auto fetch = [&](int u) { return i0 + 32 * u < cnt ? weight_key(wl[32 * u]) : 0u; };
   uint32_t key[kSelRegs];
 #pragma unroll
-  for (int u = 0; u < kSelRegs; ++u) key[u] = u < turns ? fetch(u) : 0u;
+  for (int g = 0; g < kSelRegs; g += 8) {           // (eight loads at a time, none of them behind a branch)
+    float x[8];
+    if (g < turns) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = w[p.sinks + m0 + min(i0 + 32 * (g + u), cnt - 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) key[g + u] = g + u < turns && i0 + 32 * (g + u) < cnt ? weight_key(x[u]) : 0u;
+  }
   auto each = [&](auto f) {                         // f(turn, key) over this lane's tokens
 #pragma unroll
     for (int g = 0; g < kSelRegs; g += 4)
@@ -154,35 +160,40 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
         if (k >> from == prefix) atomicAdd(&hist[(k >> shift) & mask], 1);
       });
     }
-    // the bins of all CTAs; thread t has the bins 4 t .. 4 t + 3 counted from the top
-    int c[4] = {0, 0, 0, 0};
-    const int top = kEvBins - 4 - 4 * tid;
-    auto add = [&](const int4& v) { c[0] += v.w; c[1] += v.z; c[2] += v.y; c[3] += v.x; };
-    if (nc == 1) {
-      __syncthreads();
-      add(*reinterpret_cast<const int4*>(hist + top));
-    } else {
-      cluster_sync();
-      int4 v[kEvCluster];                           // (a CTA begins with its own: they do not all ask the same one)
+    // The bin that holds the left-th key from the top, and how many of it are wanted. A CTA of a cluster sums up its share of the
+    // bins over all CTAs and scans it; the one whose share holds the key tells the others.
+    const int share_b = kEvBins / nc, nb = max(1, share_b / kSelThreads);              // bins of a CTA, of a thread (1, 2 or 4)
+    if (nc == 1) __syncthreads(); else cluster_sync();
+    int c[4] = {0, 0, 0, 0}, s = 0;
+    const int top = kEvBins - 1 - cr * share_b - tid * nb;                             // this thread's bins, downwards
 #pragma unroll
-      for (int r = 0; r < kEvCluster; ++r) v[r] = r < nc ? peer_load4(hist + top, (cr + r) & (nc - 1)) : make_int4(0, 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < kEvCluster; ++r) add(v[r]);
-    }
-    const int s = c[0] + c[1] + c[2] + c[3], incl = scan_warp(s, lane);
+    for (int u = 0; u < 4; ++u)
+      if (u < nb && tid < share_b) {
+        if (nc == 1) c[u] = hist[top - u];
+        else
+          for (int r = 0; r < nc; ++r) c[u] += peer_load(hist + top - u, (cr + r) & (nc - 1));
+        s += c[u];
+      }
+    const int incl = scan_warp(s, lane);
     if (lane == 31) wsum[wp] = incl;
     __syncthreads();
     int above = incl - s + __reduce_add_sync(0xffffffffu, lane < wp ? wsum[lane] : 0);
+    if (nc > 1) {
+      if (tid == kSelThreads - 1) slice = above + s;
+      cluster_sync();
+      above += __reduce_add_sync(0xffffffffu, lane < cr ? peer_load(&slice, lane) : 0);
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (above < left && left <= above + c[u]) {
-        found[0] = top + 3 - u;
-        found[1] = left - above;
-        found[2] = c[u];
-      }
+      if (u < nb && above < left && left <= above + c[u])
+        for (int r = 0; r < nc; ++r) {
+          peer_store(&found[0], r, top - u);
+          peer_store(&found[1], r, left - above);
+          peer_store(&found[2], r, c[u]);
+        }
       above += c[u];
     }
-    if (nc == 1) __syncthreads(); else cluster_sync();   // (the histograms have been read)
+    if (nc == 1) __syncthreads(); else cluster_sync();
     prefix = (prefix << width) | (uint32_t)found[0];
     left = found[1];
     ties = found[2] != left;                        // (else the whole bin stays)
@@ -236,7 +247,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
   if (nc > 1) cluster_sync();                       // (the totals have been read)
 }
 
-// A tile of moves: 16 tokens whose new places are one 16-token block of a page. A warp gathers their rows into shared memory,
+// A tile of moves: 16 tokens (8 at head_dim 256) whose new places lie in one 16-token block of a page. A warp gathers their rows into shared memory,
 // piece by piece (PB bytes: 8 at head_dim 128, whose rows are 8-byte aligned, 16 at 256; a row is 8 pieces of codes, FP8 keys
 // 16 before them, and one of scales), and writes the tile out: with one bulk copy a side where rows lie back to back in the
 // cache, else piece by piece. The rows hold no registers on their way, so that a warp has the next tile in flight while it
@@ -246,10 +257,11 @@ template <int D, bool K8>
 struct EvGeo {
   static constexpr int PB = D == 128 ? 8 : 16;
   static constexpr int NP = K8 ? 25 : 9;            // pieces of a row
-  static constexpr int ROWS = K8 ? 16 : 32;         // rows of a tile: keys, then values (K8: both in one)
+  static constexpr int TOK = D == 128 ? 16 : 8;     // tokens of a tile
+  static constexpr int ROWS = K8 ? TOK : 2 * TOK;   // rows of a tile: keys, then values (K8: both in one)
   static constexpr int PIECES = ROWS * NP, TURNS = (PIECES + 31) / 32;
   static constexpr int TILE = PIECES * PB;
-  static constexpr int WARP = 2 * (TILE + 256);     // shared memory of a warp: two tiles, the rows' old places (codes, scales)
+  static constexpr int WARP = 2 * (TILE + 16 * TOK);               // shared memory of a warp: two tiles, the rows' old places (codes, scales)
   static constexpr int SMEM = kMoveWarps * WARP;
 };
 
@@ -259,9 +271,9 @@ __device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes
 
 // CLUSTER: calls in place; else a row in place, which the caller may mix in, is one CTA's work
 template <int D, bool K8, bool CLUSTER>
-__global__ void __launch_bounds__(kMoveThreads, D == 128 ? 4 : 2) move_kernel(const EvictParams p) {
+__global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const EvictParams p) {
   using Gm = EvGeo<D, K8>;
-  constexpr int PB = Gm::PB, NP = Gm::NP;
+  constexpr int PB = Gm::PB, NP = Gm::NP, T = Gm::TOK;
   extern __shared__ __align__(128) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, wp = tid >> 5, h = blockIdx.y, b = blockIdx.z;
   const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_len), n = min(L, p.keep);      // (older than the preceding launch)
@@ -281,42 +293,42 @@ __global__ void __launch_bounds__(kMoveThreads, D == 128 ? 4 : 2) move_kernel(co
   const long long dh = h * p.dsh, sh = h * p.ssh;
   uint8_t* const mine = smem + wp * Gm::WARP;
   const uint32_t tiles_a = smem_u32(mine);
-  long long* const places = reinterpret_cast<long long*>(mine + 2 * Gm::TILE);           // [tile][codes, scales][16]
+  long long* const places = reinterpret_cast<long long*>(mine + 2 * Gm::TILE);           // [tile][codes, scales][T]
   // piece x of a tile: its row, its place in the row, and where that lies in shared memory
   auto row_of = [](int x) { return x / NP; };
   auto base_of = [&](int row, int pc) -> uint8_t* {
     if (K8) return pc < 16 ? p.kd + pc * 16 : pc == 24 ? p.vsf : p.vd + (pc - 16) * 16;
-    return pc == 8 ? (row < 16 ? p.ksf : p.vsf) : (row < 16 ? p.kd : p.vd) + pc * PB;
+    return pc == 8 ? (row < T ? p.ksf : p.vsf) : (row < T ? p.kd : p.vd) + pc * PB;
   };
   auto at = [&](int x, int row, int pc) {           // (split: codes and scales have regions of their own)
-    return K8 || !p.split ? x * PB : pc < 8 ? row * 8 * PB + pc * PB : (32 * 8 + row) * PB;
+    return K8 || !p.split ? x * PB : pc < 8 ? row * 8 * PB + pc * PB : (2 * T * 8 + row) * PB;
   };
   // The old place of a token hangs on two loads one after the other (position, page), its rows on those: the positions are
   // fetched two tiles ahead, the rows one. (Every CTA of a cluster takes every round, so that all of them meet at its barrier.)
-  const int stride = ctas * kMoveWarps * 16;
-  int rt = (blockIdx.x * kMoveWarps + wp) * 16;
-  auto position = [&](int r) { return lane < 16 && r + lane < n ? __ldg(kept + r + lane) : -1; };
+  const int stride = ctas * kMoveWarps * T;
+  int rt = (blockIdx.x * kMoveWarps + wp) * T;
+  auto position = [&](int r) { return lane < T && r + lane < n ? __ldg(kept + r + lane) : -1; };
   int j = position(rt);
   float wv = 0.0f, wn = 0.0f;
   bool still = false, still_n = false;              // (the tile stays where it is)
-  auto gather = [&](int buf, int r, float& weight, bool& same) {      // the rows of tokens r .. r + 15, at positions j
+  auto gather = [&](int buf, int r, float& weight, bool& same) {      // the rows of tokens r .. r + T - 1, at positions j
     const int left = n - r;
     // (positions ascend: the tile's last one tells whether all of them are their ranks)
-    same = own_pages && left >= 16 && __shfl_sync(0xffffffffu, j, 15) == r + 15;
+    same = own_pages && left >= T && __shfl_sync(0xffffffffu, j, T - 1) == r + T - 1;
     if (left > 0 && !same) {
       if (j >= 0) {
         const long long pg = __ldg(bt + (j >> p.lps));
         const int so = j & PSM;
-        places[buf * 32 + lane] = pg * p.dsp + so * p.dst + dh;
-        places[buf * 32 + 16 + lane] = pg * p.ssp + so * p.sst + sh;
+        places[buf * 2 * T + lane] = pg * p.dsp + so * p.dst + dh;
+        places[buf * 2 * T + T + lane] = pg * p.ssp + so * p.sst + sh;
       }
       __syncwarp();
 #pragma unroll
       for (int u = 0; u < Gm::TURNS; ++u) {
-        const int x = u * 32 + lane, row = row_of(x), pc = x - row * NP, i = row & 15;
+        const int x = u * 32 + lane, row = row_of(x), pc = x - row * NP, i = row & (T - 1);
         const bool scales = pc == NP - 1;
         if ((Gm::PIECES % 32 == 0 || x < Gm::PIECES) && i < left)
-          cp_async<PB>(tiles_a + buf * Gm::TILE + at(x, row, pc), base_of(row, pc) + places[buf * 32 + (scales ? 16 : 0) + i]);
+          cp_async<PB>(tiles_a + buf * Gm::TILE + at(x, row, pc), base_of(row, pc) + places[buf * 2 * T + (scales ? T : 0) + i]);
       }
     }
     if (j >= 0) weight = w[j];
@@ -341,23 +353,23 @@ __global__ void __launch_bounds__(kMoveThreads, D == 128 ? 4 : 2) move_kernel(co
       const int oo = rt & PSM;
       const long long to = og * p.dsp + oo * p.dst + dh, to_s = og * p.ssp + oo * p.sst + sh;
       const uint32_t tile = tiles_a + buf * Gm::TILE;
-      if (p.bulk && left >= 16) {
+      if (p.bulk && left >= T) {
         fence_proxy_async();
         __syncwarp();
         if (K8) {
           if (lane == 0) bulk_s2g(p.kd + to, tile, Gm::TILE);
         } else if (!p.split) {
-          if (lane < 2) bulk_s2g((lane ? p.vd : p.kd) + to, tile + lane * 16 * NP * PB, 16 * NP * PB);
+          if (lane < 2) bulk_s2g((lane ? p.vd : p.kd) + to, tile + lane * T * NP * PB, T * NP * PB);
         } else if (lane < 2) {
-          bulk_s2g((lane ? p.vd : p.kd) + to, tile + lane * 16 * 8 * PB, 16 * 8 * PB);
-          bulk_s2g((lane ? p.vsf : p.ksf) + to_s, tile + (32 * 8 + lane * 16) * PB, 16 * PB);
+          bulk_s2g((lane ? p.vd : p.kd) + to, tile + lane * T * 8 * PB, T * 8 * PB);
+          bulk_s2g((lane ? p.vsf : p.ksf) + to_s, tile + (2 * T * 8 + lane * T) * PB, T * PB);
         }
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
       } else {
         __syncwarp();
 #pragma unroll 3
         for (int u = 0; u < Gm::TURNS; ++u) {
-          const int x = u * 32 + lane, row = row_of(x), pc = x - row * NP, i = row & 15;
+          const int x = u * 32 + lane, row = row_of(x), pc = x - row * NP, i = row & (T - 1);
           if ((Gm::PIECES % 32 == 0 || x < Gm::PIECES) && i < left) {
             uint8_t* d = base_of(row, pc) + (pc == NP - 1 ? to_s + i * p.sst : to + i * p.dst);
             const uint32_t s = tile + at(x, row, pc);
@@ -367,7 +379,7 @@ __global__ void __launch_bounds__(kMoveThreads, D == 128 ? 4 : 2) move_kernel(co
         }
       }
     }
-    if (lane < 16 && rt + lane < n) ow[rt + lane] = wv;
+    if (lane < T && rt + lane < n) ow[rt + lane] = wv;
     wv = wn;
     still = still_n;
   }
@@ -444,7 +456,7 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   p.max_len = (int)(reach < W ? reach : W);               // (a length beyond the table or the weights is cut there)
   const long long pairs = (long long)B * KVH;
   int nc = kEvCluster;
-  while (nc > 1 && (pairs * nc > 600 || p.max_len < nc * 2048)) nc /= 2;
+  while (nc > 1 && (pairs * nc > 600 || p.max_len < nc * 2048 || p.max_len <= 8192)) nc /= 2;
   cudaStream_t st = (cudaStream_t)stream;
   int rc = launch_clusters(select_kernel, p, nc, KVH, B, nc, kSelThreads, 0, st);
   if (rc != HKV_OK) return rc;
@@ -458,7 +470,7 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   if (rc != HKV_OK) return rc;
   if (cluster) return launch_clusters(mk, p, kEvCluster, KVH, B, kEvCluster, kMoveThreads, smem, st);
   // as many CTAs per (request, kv head) as find work at once
-  const long long most = keep < p.max_len ? keep : p.max_len, round = kMoveWarps * 16;
+  const long long most = keep < p.max_len ? keep : p.max_len, round = kMoveWarps * (D == 128 ? 16 : 8);
   const long long x = std::max(1ll, std::min((most + round - 1) / round, (kMoveCtas + pairs - 1) / pairs));
   return record_cuda(launch_pdl(mk, dim3((unsigned)x, (unsigned)KVH, (unsigned)B), dim3(kMoveThreads), smem, st, p));
 }
