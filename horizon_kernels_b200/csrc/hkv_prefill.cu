@@ -28,6 +28,12 @@ constexpr int kPfReqs = 32;            // requests per launch (the tables below 
 constexpr int kPfCtas = 160;           // CTAs per launch
 constexpr int kKeys = 128;             // keys per tile
 constexpr int kPieceCost = 3;          // cost of starting and ending a piece, in key tiles (of about 1 us)
+// Over a window a row tile has ten tiles where a prompt has two hundred, and the maximum of a warp's 32 rows moves at nearly every
+// one of the first ten: the output's rescaling, between one value product and the next, is what a tile waits for. With 16-bit
+// outputs the maximum therefore lags by up to 2^8, as in the decode kernel: probabilities stay within f16's range at its 2^-11 of
+// each, and what is lost against a largest probability of exactly 1, about 2e-4 of the output (2-norm), lies a factor of eight
+// below the output's own rounding. MEASURE. fp32 outputs keep the exact maximum.
+constexpr float kPfLag = 8.0f;
 constexpr int kMinPiece = 2;           // no piece of a divided row tile is shorter, in key tiles
 constexpr int kStageBytes = 32768;
 constexpr int kStages = 5;
@@ -73,6 +79,7 @@ struct PrefillParams {
   int first_chunk;
   int window, sinks;                   // WIN: a token at position x sees the keys j <= x with j > x - window or j < sinks (window 0: all)
   float* lse;                          // the rows' log-sum-exps, or null
+  float lag;                           // WIN: the running maximum moves when a score exceeds it by more (log2 domain)
   PfReq req[kPfReqs];
   PfStart start[kPfCtas + 1];
   PfSplit split[kPfCtas];
@@ -520,21 +527,27 @@ struct Tiles {
   __device__ __forceinline__ PfSpan span(int* whole, int* tile0) const {
     return pf_span(r, rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, whole, tile0);
   }
-  __device__ __forceinline__ void enter() {
+  __device__ __forceinline__ void enter(const PfSpan& x) {           // WIN: at the row tile of span x
     first = true;
     const bool c = cut();
     end = c && kt >= last.kt;
+    e1 = x.e1;
+    s2 = x.s2;
+    hi = c ? last.kt : x.e2 > x.s2 ? x.e2 : x.e1;
+    if (hi == s2 && kt < e1) hi = e1;               // (cut between the sinks and the window)
+  }
+  __device__ __forceinline__ void enter() {
     if constexpr (WIN) {
-      if (req >= p.n_req) return;
       int whole, tile0;
-      const PfSpan x = span(&whole, &tile0);
-      e1 = x.e1;
-      s2 = x.s2;
-      hi = c ? last.kt : x.e2 > x.s2 ? x.e2 : x.e1;
-      if (hi == s2 && kt < e1) hi = e1;             // (cut between the sinks and the window)
-    } else {
-      hi = c ? last.kt : tile_hi();
+      PfSpan x{0, 0, 0};
+      if (req < p.n_req) x = span(&whole, &tile0);
+      enter(x);
+      return;
     }
+    first = true;
+    const bool c = cut();
+    end = c && kt >= last.kt;
+    hi = c ? last.kt : tile_hi();
   }
   __device__ __forceinline__ void next_piece() {
     if (cut()) {
@@ -542,6 +555,7 @@ struct Tiles {
       return;
     }
     kt = p.kt_lo;
+    PfSpan x{0, 0, 0};
     bool none;
     do {
       if (++rt >= n_rt) {
@@ -552,11 +566,11 @@ struct Tiles {
           enter_request();
         }
       }
-      none = false;
       if constexpr (WIN) {
+        none = false;
         if (req < p.n_req) {
           int whole, tile0;
-          const PfSpan x = span(&whole, &tile0);
+          x = span(&whole, &tile0);
           none = x.count(p.kt_lo) <= 0;
           kt = x.begin(p.kt_lo);
         } else {
@@ -567,7 +581,8 @@ struct Tiles {
       }
     } while (req < p.n_req && none);                      // (no keys in this chunk)
     ++piece;
-    enter();
+    if constexpr (WIN) enter(x);
+    else enter();
   }
   __device__ __forceinline__ void next() {
     first = false;
@@ -908,16 +923,36 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
       // keys below this one are seen by every live row of the tile (rows that do not exist may take any value)
       const int whole = max(0, min(r.L, r.L - r.ql + x.rt * p.tok + 1));
       const uint32_t g_end = g0 + x.left();
-      // WIN: the piece's tile i lies at x.kt + i, from `jump` on at i + beyond; keys below win_hi are out of the last row's window
-      const int jump = WIN && x.kt < x.e1 ? x.e1 - x.kt : 0;
-      const int beyond = WIN ? (x.kt < x.e1 ? x.s2 - jump : x.kt) + pf_keys(r, p.window, p.sinks).skip : 0;
-      const int win_hi = WIN ? pf_from(r, min(r.ql, (x.rt + 1) * p.tok) - 1, p.window) : 0;
       volatile float* top_now = xm + (x.piece & 1) * 128 + row;
       float m = -INFINITY;                                // the running maximum as this thread knows it
       unsigned long long l2 = 0;                          // two partial sums
       bool any_tile = false;
       for (; g < g_end; g += SETS, ++turn) {
-        const int key = (WIN && (int)(g - g0) >= jump ? beyond + (int)(g - g0) : x.kt + (int)(g - g0)) * kKeys;
+        int key = x.kt + (int)(g - g0);                   // (of the request's tiles, below of its keys)
+        // WIN: parts of 32 keys that some row of the warp sees (the others have no scores to look at and zeros for
+        // probabilities), and, in the upper four bits, those that not every row sees. The tile's place is worked out anew for
+        // every tile: kept in registers over the piece, its parts would push others out, and a spilled register costs an L2
+        // access here (with 44 spilled ones, 6144 tokens without a window took 391 us instead of 304).
+        uint32_t parts = 15;
+        if constexpr (WIN) {
+          int window = p.window;
+          asm volatile("" : "+r"(window));
+          if (x.kt < x.e1 && key >= x.e1) key += x.s2 - x.e1;
+          const PfKeys kk = pf_keys(r, window, p.sinks);
+          key = (key >= kk.su ? key + kk.skip : key) * kKeys;
+          const int t0 = r.L - r.ql + x.rt * p.tok + 1;   // keys below it are seen by every row, those from it to t0 - window by none
+          if (key + kKeys > t0 || (window > 0 && key < t0 + p.tok - 1 - window)) {
+            const int last = __reduce_max_sync(0xffffffffu, lim), lo = window > 0 ? __shfl_sync(0xffffffffu, lim, 0) - window : 0;
+            parts = 0;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int k = key + 32 * c;
+              if (k < last && (k + 32 > lo || k < p.sinks)) parts |= 17u << c;
+            }
+          }
+        } else {
+          key *= kKeys;
+        }
         const bool head = g == g0;
         ok = all_wait(s_bar, turn);
         if (!ok) break;
@@ -928,11 +963,14 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
           tm_ld32(s0, s_addr + 32 * c);
           tm_wait_ld();
           tm_ready(s0);
-          if (WIN && (key + 32 * c + 32 > whole || (key + 32 * c < win_hi && key + 32 * c + 32 > p.sinks))) {
-            const int rel = lim - key - 32 * c, from = p.window > 0 ? rel - p.window : 0, sinks = p.sinks - key - 32 * c;
+          if (WIN && (parts >> (4 + c) & 1)) {
+            // (a bit per key: half the instructions of a comparison or three per key)
+            auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1; };
+            const int rel = lim - key - 32 * c, from = p.window > 0 ? rel - p.window : 0;
+            const uint32_t sees = below(rel) & ~(below(from) & ~below(p.sinks - key - 32 * c));
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (i >= rel || (i < from && i >= sinks)) s0[i] = 0xff800000u;
+              if (!(sees & (1u << i))) s0[i] = 0xff800000u;
           }
           if (!WIN && key + 32 * c + 32 > whole) {
             const int rel = lim - key - 32 * c;
@@ -947,6 +985,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
 #pragma unroll 1
         for (int c = 0; c < 4; ++c) {
           load(c);
+          if (!WIN || parts >> c & 1)
 #pragma unroll
           for (int i = 0; i < 32; i += 2)
             mx[i / 2 & 3] = fmaxf(mx[i / 2 & 3], fmaxf(__uint_as_float(s0[i]), __uint_as_float(s0[i + 1])));
@@ -956,7 +995,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
         if (g > 0) ok = all_wait(word_before, (g - 1) / SETS);
         if (!ok) break;
         const float m_old = m, m_in = head ? -INFINITY : *top_now;
-        const bool move = top > m_in;
+        const bool move = top > (WIN ? m_in + p.lag : m_in);
         m = move ? (top == INFINITY ? 0.0f : top) : m_in;
         if (move || head) *top_now = m;
         mbar_arrive_u32(my_word);
@@ -972,6 +1011,10 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
 #pragma unroll 1
         for (int c = 3;; --c) {
           uint32_t ph16[16];
+          if (WIN && !(parts >> c & 1)) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) ph16[k] = 0;
+          } else
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             float a, b;
@@ -983,7 +1026,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
           }
           tm_st16(s_addr + 64 + 16 * c, ph16);
           if (c == 0) break;
-          load(c - 1);
+          if (!WIN || (parts >> (c - 1) & 1)) load(c - 1);
         }
         if (__any_sync(0xffffffffu, al_o != 1.0f)) {
           // the output of the tiles before this one, all of whose value products must have been added first; 64 columns at a
@@ -1314,6 +1357,7 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
   p.window = win.window;
   p.sinks = win.sinks;
   p.lse = win.lse;
+  p.lag = win.window > 0 && !out_f32 ? kPfLag : 0.0f;
   p.out = out;
   p.out_f32 = out_f32;
   p.k_bf16 = !q_f16;                                      // (the cached values are exact in both types)
