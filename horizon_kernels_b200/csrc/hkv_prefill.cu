@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "hkv_common.cuh"
 
 namespace hkv {
@@ -103,9 +105,12 @@ struct PfKeys {
 __host__ __device__ inline int pf_from(const PfReq& r, int t, int window) {   // first token of the window of query token t
   return window > 0 ? max(0, r.L - r.ql + t + 1 - window) : 0;
 }
+constexpr int kKeysLog = 7;
+static_assert(1 << kKeysLog == kKeys, "keys of a tile");
+__host__ __device__ inline int pf_tiles(int keys) { return (keys + kKeys - 1) >> kKeysLog; }      // (not negative)
 __host__ __device__ inline PfKeys pf_keys(const PfReq& r, int window, int sinks) {
-  const int lo = pf_from(r, 0, window), su = (min(lo, sinks) + kKeys - 1) / kKeys;
-  return PfKeys{su, max(0, lo / kKeys - su)};
+  const int lo = pf_from(r, 0, window), su = pf_tiles(min(lo, sinks));
+  return PfKeys{su, max(0, (lo >> kKeysLog) - su)};
 }
 // the tiles of a chunk [kt_lo, kt_hi) that a row tile sees: [kt_lo, e1), the sinks, and [s2, e2), the window
 struct PfSpan {
@@ -113,12 +118,12 @@ struct PfSpan {
   __host__ __device__ int count(int kt_lo) const { return e1 - kt_lo + e2 - s2; }
   __host__ __device__ int begin(int kt_lo) const { return e1 > kt_lo ? kt_lo : s2; }
 };
-// (whole: one past the last tile that it sees at all; first: the first one)
-__host__ __device__ inline PfSpan pf_span(const PfReq& r, int rt, int tok, int kt_lo, int kt_hi, int window, int sinks, int* whole,
-                                          int* first) {
-  const int skip = pf_keys(r, window, sinks).skip, lo = pf_from(r, rt * tok, window), s = (min(lo, sinks) + kKeys - 1) / kKeys;
-  const int t_end = min(r.ql, (rt + 1) * tok), vis = max(1, min(r.L, r.L - r.ql + t_end));
-  const int a = max(s, lo / kKeys - skip), b = (vis + kKeys - 1) / kKeys - skip;
+// (skip: of the request; whole: one past the last tile that it sees at all; first: the first one)
+__host__ __device__ inline PfSpan pf_span(const PfReq& r, int skip, int rt, int tok, int kt_lo, int kt_hi, int window, int sinks,
+                                          int* whole, int* first) {
+  const int t0 = rt * tok, lo = pf_from(r, t0, window), s = pf_tiles(min(lo, sinks));
+  const int vis = max(1, min(r.L, r.L - r.ql + min(r.ql, t0 + tok)));
+  const int a = max(s, (lo >> kKeysLog) - skip), b = pf_tiles(vis) - skip;
   *whole = max(s, b);
   *first = s > 0 ? 0 : a;
   PfSpan x;
@@ -128,41 +133,10 @@ __host__ __device__ inline PfSpan pf_span(const PfReq& r, int rt, int tok, int k
   return x;
 }
 
-template <bool WIN>
 struct Walk {
   int req, h, rt, kt;
-  int window, sinks;
-  __host__ __device__ bool same_tile(const PfStart& e) const { return req == e.req && h == e.h && rt == e.rt; }
   // the next row tile that has keys in this chunk
-  // tiles of the row tile from kt on
-  __host__ __device__ int left(const PfReq* r, int tok, int kt_lo, int kt_hi) const {
-    if (!WIN) return pf_hi(r[req], rt, tok, kt_hi) - kt;
-    int whole, first;
-    const PfSpan x = pf_span(r[req], rt, tok, kt_lo, kt_hi, window, sinks, &whole, &first);
-    return kt < x.e1 ? x.e1 - kt + x.e2 - x.s2 : x.e2 - kt;
-  }
-  __host__ __device__ void step(const PfReq* r, int tok, int kt_lo, int kt_hi, int n) {      // n tiles further in the row tile
-    if (WIN) {
-      int whole, first;
-      const PfSpan x = pf_span(r[req], rt, tok, kt_lo, kt_hi, window, sinks, &whole, &first);
-      if (kt < x.e1 && kt + n >= x.e1) n += x.s2 - x.e1;
-    }
-    kt += n;
-  }
-  __host__ __device__ void advance(const PfReq* r, int n_req, int KVH, int tok, int kt_lo, int kt_hi) {
-    if (WIN) {
-      while (true) {
-        if (++rt >= pf_row_tiles(r[req], tok)) {
-          rt = 0;
-          if (++h >= KVH) { h = 0; ++req; }
-        }
-        if (req >= n_req) return;
-        int whole, first;
-        const PfSpan x = pf_span(r[req], rt, tok, kt_lo, kt_hi, window, sinks, &whole, &first);
-        kt = x.begin(kt_lo);
-        if (x.count(kt_lo) > 0) return;
-      }
-    }
+  void advance(const PfReq* r, int n_req, int KVH, int tok, int kt_lo, int kt_hi) {
     kt = kt_lo;
     do {
       if (++rt >= pf_row_tiles(r[req], tok)) {
@@ -170,6 +144,36 @@ struct Walk {
         if (++h >= KVH) { h = 0; ++req; }
       }
     } while (req < n_req && pf_hi(r[req], rt, tok, kt_hi) <= kt_lo);
+  }
+  int left(const PfReq* r, int tok, int, int kt_hi) const { return pf_hi(r[req], rt, tok, kt_hi) - kt; }
+  void step(const PfReq*, int, int, int, int n) { kt += n; }
+};
+// the same over a window
+struct WinWalk {
+  int req, h, rt, kt;
+  int window, sinks, skip;
+  PfSpan x;
+  void advance(const PfReq* r, int n_req, int KVH, int tok, int kt_lo, int kt_hi) {
+    do {
+      if (rt < 0) skip = pf_keys(r[req], window, sinks).skip;         // (the first row tile of all)
+      if (++rt >= pf_row_tiles(r[req], tok)) {
+        rt = 0;
+        if (++h >= KVH) {
+          h = 0;
+          if (++req >= n_req) return;
+          skip = pf_keys(r[req], window, sinks).skip;
+        }
+      }
+      int whole, first;
+      x = pf_span(r[req], skip, rt, tok, kt_lo, kt_hi, window, sinks, &whole, &first);
+    } while (x.count(kt_lo) <= 0);
+    kt = x.begin(kt_lo);
+  }
+  // tiles of the row tile from kt on
+  int left(const PfReq*, int, int, int) const { return kt < x.e1 ? x.e1 - kt + x.e2 - x.s2 : x.e2 - kt; }
+  void step(const PfReq*, int, int, int, int n) {                     // n tiles further in the row tile
+    if (kt < x.e1 && kt + n >= x.e1) n += x.s2 - x.e1;
+    kt += n;
   }
 };
 
@@ -505,6 +509,7 @@ struct Tiles {
   PfReq r;
   int n_rt;                            // row tiles of the request
   int e1, s2;                          // WIN: after tile e1 - 1 comes s2 (PfSpan)
+  int skip;                            // .. of the request's tiles (PfKeys)
   uint32_t piece;
   bool first, end;                     // first tile of its piece; nothing left
   __device__ __forceinline__ explicit Tiles(const PrefillParams& p_) : p(p_), last(p_.start[blockIdx.x + 1]), piece(0) {
@@ -520,12 +525,13 @@ struct Tiles {
     if (req < p.n_req) {
       r = p.req[req];
       n_rt = pf_row_tiles(r, p.tok);
+      if constexpr (WIN) skip = pf_keys(r, p.window, p.sinks).skip;
     }
   }
   __device__ __forceinline__ bool cut() const { return rt == last.rt && h == last.h && req == last.req; }   // goes on in the next CTA
   __device__ __forceinline__ int tile_hi() const { return pf_hi(r, rt, p.tok, p.kt_hi); }
   __device__ __forceinline__ PfSpan span(int* whole, int* tile0) const {
-    return pf_span(r, rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, whole, tile0);
+    return pf_span(r, skip, rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, whole, tile0);
   }
   __device__ __forceinline__ void enter(const PfSpan& x) {           // WIN: at the row tile of span x
     first = true;
@@ -647,7 +653,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
       bool ok = *abort == 0;
       auto fetch = [&](Tiles<WIN>& x, int side) {
         const PfReq& r = x.r;
-        const int n_t = min(p.kt_hi, (r.L + kKeys - 1) / kKeys - (WIN ? pf_keys(r, p.window, p.sinks).skip : 0)) - p.kt_lo;
+        const int n_t = min(p.kt_hi, (r.L + kKeys - 1) / kKeys - (WIN ? x.skip : 0)) - p.kt_lo;
         const uint8_t* from = p.tiles + ((size_t)r.tile0 * p.KVH + (size_t)x.h * n_t + (x.kt - p.kt_lo)) * 2 * IMAGE + side * IMAGE;
         for (int i = 0; ok && i < PER; ++i) {
           if (LOSE && fill == 3) ok = false;
@@ -1124,7 +1130,7 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Pref
     m = mm;
   };
   int end, tile0 = 0;
-  if constexpr (WIN) pf_span(r, t.rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, &end, &tile0);
+  if constexpr (WIN) pf_span(r, pf_keys(r, p.window, p.sinks).skip, t.rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, &end, &tile0);
   else end = (max(1, min(r.L, r.L - r.ql + min(r.ql, (t.rt + 1) * p.tok))) + kKeys - 1) / kKeys;
   if (state && (WIN ? tile0 < p.kt_lo : !p.first_chunk)) add(p.state_ml[2 * st_row], p.state_ml[2 * st_row + 1], p.state_o + st_row * D + ch);
   for (int c = sp.c1; c <= sp.c2; ++c) {
@@ -1157,14 +1163,19 @@ __global__ void __launch_bounds__(256) merge_kernel(const __grid_constant__ Pref
 template <bool WIN>
 static int plan(PrefillParams& p, int n_cta, int* n_split) {
   long long total = 0;
-  Walk<WIN> w0{0, 0, -1, 0, p.window, p.sinks};
+  typename std::conditional<WIN, WinWalk, Walk>::type w0{};
+  w0.rt = -1;
+  if constexpr (WIN) {
+    w0.window = p.window;
+    w0.sinks = p.sinks;
+  }
   w0.advance(p.req, p.n_req, p.KVH, p.tok, p.kt_lo, p.kt_hi);      // the first row tile with keys in the chunk
   for (int r = 0; r < p.n_req; ++r) {
     long long head = 0;
-    const int n_rt = pf_row_tiles(p.req[r], p.tok);
+    const int n_rt = pf_row_tiles(p.req[r], p.tok), skip = WIN ? pf_keys(p.req[r], p.window, p.sinks).skip : 0;
     for (int rt = 0; rt < n_rt; ++rt) {
       int whole, first;
-      const int n = WIN ? pf_span(p.req[r], rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, &whole, &first).count(p.kt_lo)
+      const int n = WIN ? pf_span(p.req[r], skip, rt, p.tok, p.kt_lo, p.kt_hi, p.window, p.sinks, &whole, &first).count(p.kt_lo)
                         : pf_hi(p.req[r], rt, p.tok, p.kt_hi) - p.kt_lo;
       if (n > 0) head += kPieceCost + n;
     }
@@ -1173,7 +1184,7 @@ static int plan(PrefillParams& p, int n_cta, int* n_split) {
   long long cap = (total + n_cta - 1) / n_cta;
   if (cap < kPieceCost + 4) cap = kPieceCost + 4;
   for (;; cap += cap / 64 + 1) {
-    Walk<WIN> w = w0;
+    auto w = w0;
     int c = 0;
     *n_split = 0;
     int part_c1 = -1, part_slot1 = 0, pieces = 0;         // the divided row tile being cut; pieces of the current CTA
