@@ -21,8 +21,8 @@ int noalloc_workspace(void** ws);
 
 constexpr int kWtWarps = 4;
 constexpr int kWtThreads = kWtWarps * 32;
-constexpr int kWtCost = 4;           // what a sequence costs a warp beyond its units (its queries and log-sum-exps), in units
-constexpr int kWtMin = 2;            // least units of a warp
+constexpr int kWtCost = 2;           // what a sequence costs a warp beyond its units (its queries and log-sum-exps), in units
+constexpr int kWtMin = 1;            // least units of a warp
 
 struct WeightsParams {
   const __nv_bfloat16* q;
@@ -54,7 +54,7 @@ struct WtGeo {
   static constexpr int ROW = LAYOUT == 1 ? SD : SD + SS;             // byte stride between token rows of a stage
   static constexpr int SF_BASE = LAYOUT == 1 ? UT * SD : SD, SF_ROW = LAYOUT == 1 ? SS : ROW;
   static constexpr int STAGE = UT * (SD + SS);
-  static constexpr int NS = 4;
+  static constexpr int NS = 2;
   static constexpr int KS = D / 16, NBL = D / 64, KB = K8 ? 16 : 8;
   // 72-byte rows: as in the decode kernel, so that the lanes' loads touch every bank once
   __device__ static constexpr int tok(int i) {
@@ -83,7 +83,7 @@ __device__ __forceinline__ WtReq wt_req(const WeightsParams& p, int b) {
 }
 
 template <int D, int LAYOUT, int QT>
-__global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams p) {
+__global__ void __launch_bounds__(kWtThreads, D == 128 ? (QT == 1 ? 4 : 3) : QT == 1 ? 3 : 2) weights_kernel(const WeightsParams p) {
   using Gm = WtGeo<D, LAYOUT>;
   constexpr int NS = Gm::NS, UT = Gm::UT;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -95,52 +95,76 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
   pdl_wait();
   pdl_launch_dependents();
 
-  // prefix of the requests' weights (units + cost) per kv head, 32 requests at a time
+  // the part [lo, hi) of this warp in the stream of weights (units + cost of the requests, kv head by kv head), the request b0
+  // that holds lo, and the weight of the requests before it, per kv head
   auto wt = [](int U) { return U > 0 ? U + kWtCost : 0; };
-  const int ngrp = (B + 31) >> 5;
-  for (int grp = wp; grp < ngrp; grp += kWtWarps) {
-    const int b = grp * 32 + lane;
-    int u = b < B ? wt(wt_req(p, b).U) : 0;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
-    if (lane == 0) coarse[grp + 1] = u;
-  }
-  __syncthreads();
-  if (wp == 0) {
-    const int per_lane = (ngrp + 31) >> 5;
-    int s = 0;
-    for (int i = 0; i < per_lane; ++i) {
-      const int k = lane * per_lane + i;
-      s += k < ngrp ? coarse[k + 1] : 0;
-    }
-    int incl = s;
+  const long long parts = (long long)gridDim.x * kWtWarps;
+  long long lo, hi;
+  auto part = [&](long long total) {
+    const long long per = max((long long)(kWtMin + kWtCost), (total + parts - 1) / parts);
+    lo = ((long long)blockIdx.x + (long long)wp * gridDim.x) * per;
+    hi = min(total, lo + per);
+  };
+  int b0, base0;
+  WtReq first;                         // of b0
+  fence_barrier_init();
+  if (B <= 32) {                       // a lane per request, every warp for itself
+    const WtReq r = wt_req(p, min(lane, B - 1));
+    const int u = lane < B ? wt(r.U) : 0;
+    int incl = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    int run = incl - s;
-    for (int i = 0; i < per_lane; ++i) {
-      const int k = lane * per_lane + i;
-      if (k < ngrp) {
-        run += coarse[k + 1];
-        coarse[k + 1] = run;
-      }
+    __syncthreads();                   // (the barriers are set up)
+    part((long long)__shfl_sync(0xffffffffu, incl, 31) * KVH);
+    if (lo >= hi) return;
+    b0 = __ffs(__ballot_sync(0xffffffffu, (long long)incl * KVH > lo)) - 1;
+    base0 = __shfl_sync(0xffffffffu, incl - u, b0);
+    first.U = __shfl_sync(0xffffffffu, r.U, b0);
+    first.L = __shfl_sync(0xffffffffu, r.L, b0);
+    first.ql = __shfl_sync(0xffffffffu, r.ql, b0);
+    first.q0 = __shfl_sync(0xffffffffu, r.q0, b0);
+    first.su = __shfl_sync(0xffffffffu, r.su, b0);
+    first.skip = __shfl_sync(0xffffffffu, r.skip, b0);
+  } else {
+    // prefix over groups of 32 requests
+    const int ngrp = (B + 31) >> 5;
+    for (int grp = wp; grp < ngrp; grp += kWtWarps) {
+      const int b = grp * 32 + lane;
+      int u = b < B ? wt(wt_req(p, b).U) : 0;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) u += __shfl_xor_sync(0xffffffffu, u, o);
+      if (lane == 0) coarse[grp + 1] = u;
     }
-    if (lane == 0) coarse[0] = 0;
-  }
-  fence_barrier_init();
-  __syncthreads();
-
-  const long long total = (long long)coarse[ngrp] * KVH;
-  const long long parts = (long long)gridDim.x * kWtWarps;
-  const long long per = max((long long)(kWtMin + kWtCost), (total + parts - 1) / parts);
-  const long long lo = ((long long)blockIdx.x + (long long)wp * gridDim.x) * per, hi = min(total, lo + per);
-  if (lo >= hi) return;
-
-  // the sequence that holds stream position lo
-  int b0, base0;
-  {
+    __syncthreads();
+    if (wp == 0) {
+      const int per_lane = (ngrp + 31) >> 5;
+      int s = 0;
+      for (int i = 0; i < per_lane; ++i) {
+        const int k = lane * per_lane + i;
+        s += k < ngrp ? coarse[k + 1] : 0;
+      }
+      int incl = s;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+      }
+      int run = incl - s;
+      for (int i = 0; i < per_lane; ++i) {
+        const int k = lane * per_lane + i;
+        if (k < ngrp) {
+          run += coarse[k + 1];
+          coarse[k + 1] = run;
+        }
+      }
+      if (lane == 0) coarse[0] = 0;
+    }
+    __syncthreads();
+    part((long long)coarse[ngrp] * KVH);
+    if (lo >= hi) return;
     int lo_g = 0, hi_g = ngrp;
     while (hi_g - lo_g > 1) {
       const int m = (lo_g + hi_g) >> 1;
@@ -154,10 +178,10 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
       const int t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
-    const unsigned hit = __ballot_sync(0xffffffffu, (long long)(coarse[lo_g] + incl) * KVH > lo);
-    const int j = __ffs(hit) - 1;
+    const int j = __ffs(__ballot_sync(0xffffffffu, (long long)(coarse[lo_g] + incl) * KVH > lo)) - 1;
     b0 = lo_g * 32 + j;
     base0 = coarse[lo_g] + __shfl_sync(0xffffffffu, incl - u, j);
+    first = wt_req(p, b0);
   }
   // A walk over the units of [lo, hi): the fetching side runs NS units ahead of the computing one
   struct Walk {
@@ -189,7 +213,7 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
   };
   Walk cw;
   cw.b = b0;
-  cw.r = wt_req(p, b0);
+  cw.r = first;
   cw.h = (int)((lo - (long long)base0 * KVH) / wt(cw.r.U));
   cw.seq0 = (long long)base0 * KVH + (long long)cw.h * wt(cw.r.U);
   bool more = enter(cw, lo);
@@ -198,55 +222,70 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
 
   const uint32_t ring_a = smem_u32(smem + wp * NS * Gm::STAGE), bars_a = smem_u32(bars + wp * NS);
   const int PSM = (1 << p.lps) - 1;
-  unsigned f_n = 0, c_n = 0;
+  // units fetched ahead; the next stage to fetch into and to consume, and the latter's phase
+  int ahead = 0, f_st = 0, c_st = 0;
+  uint32_t c_par = 0;
+  const uint8_t *f_kd, *f_ks;          // keys of the fetching side's kv head
+  auto f_head = [&]() {
+    f_kd = p.kd + (long long)fw.h * p.dsh;
+    f_ks = p.ksf + (long long)fw.h * p.ssh;
+  };
+  f_head();
+  // page ids of the next 16 units (two 16-token blocks each) of the fetching side's sequence, a lane each; -1: no row sees the block
+  int pg = 0, pg_first = 0, pg_end = -1;
+  auto look_up = [&]() {
+    const int u = fw.u + (lane >> 1), t = (u + (u >= fw.r.su ? fw.r.skip : 0)) * UT + 16 * (lane & 1);
+    const int lo_w = p.window > 0 ? max(0, fw.r.L - fw.r.ql + p.row0 / G - p.window + 1) : 0;
+    pg = u < fw.end && t < fw.r.L && (t + 16 > lo_w || t < p.sinks) ? __ldg(p.bt + (long long)fw.b * p.MP + (t >> p.lps)) : -1;
+    pg_first = fw.u;
+    pg_end = min(fw.end, fw.u + 16);
+  };
   // fetches the next unit, 16-token blocks that hold a visible token only
   auto fetch = [&]() {
-    const uint32_t bar = bars_a + 8 * (f_n % NS), st = ring_a + (f_n % NS) * Gm::STAGE;
+    const uint32_t bar = bars_a + 8 * f_st, st = ring_a + f_st * Gm::STAGE;
     const int tok0 = (fw.u + (fw.u >= fw.r.su ? fw.r.skip : 0)) * UT;
-    const int lo_w = p.window > 0 ? max(0, fw.r.L - fw.r.ql + p.row0 / G - p.window + 1) : 0;
-    bool blk[2];
+    if (fw.u >= pg_end) look_up();
     int page[2];
 #pragma unroll
-    for (int bi = 0; bi < 2; ++bi) {
-      const int t = tok0 + 16 * bi;
-      blk[bi] = t < fw.r.L && (t + 16 > lo_w || t < p.sinks);
-      page[bi] = blk[bi] ? __ldg(p.bt + (long long)fw.b * p.MP + (t >> p.lps)) : 0;
-    }
-    const uint8_t* kd = p.kd + (long long)fw.h * p.dsh;
-    const uint8_t* ks = p.ksf + (long long)fw.h * p.ssh;
+    for (int bi = 0; bi < 2; ++bi) page[bi] = __shfl_sync(0xffffffffu, pg, 2 * (fw.u - pg_first) + bi);
     if (Gm::ROWCOPY) {
       // two lanes per token row (of a 16-token block)
       constexpr int CB = D == 128 ? 8 : 16, N = (Gm::SD + Gm::SS) / CB;
       const int row = lane >> 1;
 #pragma unroll
       for (int bi = 0; bi < 2; ++bi)
-        if (blk[bi]) {
-          const uint8_t* src = kd + (unsigned long long)(unsigned)page[bi] * p.dsp + (((tok0 + 16 * bi) & PSM) + row) * p.dst;
+        if (page[bi] >= 0) {
+          const uint8_t* src = f_kd + (unsigned long long)(unsigned)page[bi] * p.dsp + (((tok0 + 16 * bi) & PSM) + row) * p.dst;
           const uint32_t d = st + (16 * bi + row) * Gm::ROW;
           for (int j = lane & 1; j < N; j += 2) cp_async<CB>(d + j * CB, src + j * CB);
         }
       cp_async_mbar_arrive_noinc(bar);
     } else if (elect_one()) {
-      const int nb = (int)blk[0] + (int)blk[1];
+      const int nb = (page[0] >= 0) + (page[1] >= 0);
       mbar_expect_tx_u32(bar, nb * 16 * (Gm::SD + Gm::SS));
 #pragma unroll
       for (int bi = 0; bi < 2; ++bi)
-        if (blk[bi]) {
+        if (page[bi] >= 0) {
           const unsigned pos = (tok0 + 16 * bi) & PSM;
-          const uint8_t* src = kd + (unsigned long long)(unsigned)page[bi] * p.dsp + pos * (unsigned)Gm::ROW;
+          const uint8_t* src = f_kd + (unsigned long long)(unsigned)page[bi] * p.dsp + pos * (unsigned)Gm::ROW;
           if (LAYOUT == 0) {
             bulk_g2s_u32(st + bi * 16 * Gm::ROW, src, 16 * Gm::ROW, bar);
           } else {
             bulk_g2s_u32(st + bi * 16 * Gm::SD, src, 16 * Gm::SD, bar);
-            bulk_g2s_u32(st + UT * Gm::SD + bi * 16 * Gm::SS, ks + (unsigned long long)(unsigned)page[bi] * p.ssp + pos * (unsigned)Gm::SS,
+            bulk_g2s_u32(st + UT * Gm::SD + bi * 16 * Gm::SS, f_ks + (unsigned long long)(unsigned)page[bi] * p.ssp + pos * (unsigned)Gm::SS,
                          16 * Gm::SS, bar);
           }
         }
     }
-    ++f_n;
-    if (++fw.u == fw.end) f_more = enter(fw, fw.seq0 + kWtCost + fw.end);
+    ++ahead;
+    if (++f_st == NS) f_st = 0;
+    if (++fw.u == fw.end) {
+      f_more = enter(fw, fw.seq0 + kWtCost + fw.end);
+      f_head();
+      pg_end = -1;
+    }
   };
-  while (f_more && f_n < NS) fetch();
+  while (f_more && ahead < NS) fetch();
 
   const int r0 = Gm::tok(g), r1 = Gm::tok(g + 8);
   const uint32_t koff_d = r0 * Gm::ROW + Gm::KB * Gm::NBL * c, koff_s = Gm::SF_BASE + r0 * Gm::SF_ROW + Gm::NBL * c;
@@ -256,12 +295,23 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
     // the queries of this sequence: rows 8 q + g, channels of this lane's key blocks, as f16; rows 2 c, 2 c + 1 of the scores
     const int L = cw.r.L, ql = cw.r.ql, q0 = cw.r.q0, h = cw.h;
     const int R = min(8 * QT, G * ql - p.row0);
+    float le[QT][2];
+    int lim[QT][2];
+#pragma unroll
+    for (int q = 0; q < QT; ++q)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const int r = 8 * q + 2 * c + k, row = p.row0 + r;
+        const bool is = r < R;
+        const int tr = is ? row / G : 0;
+        le[q][k] = is ? __ldg(p.lse + (long long)(q0 + tr) * (KVH * G) + h * G + row - tr * G)
+                      : __int_as_float(0x7f800000);              // (a row that does not exist: its scores are 0 - inf)
+        lim[q][k] = is ? L - ql + tr + 1 : 0;       // sees the keys below this one
+      }
     const float sc_signed = p.scale_log2 * __ldg(p.gk + h);
     const bool flip = sc_signed < 0.0f;
     const float sc = fabsf(sc_signed);
     uint32_t qa[QT][Gm::KS][2];
-    float le[QT][2];
-    int lim[QT][2], from[QT][2];
 #pragma unroll
     for (int q = 0; q < QT; ++q) {
       const bool have = g + 8 * q < R;
@@ -310,31 +360,26 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
         const float a = flip ? -qf[2 * i] : qf[2 * i], b = flip ? -qf[2 * i + 1] : qf[2 * i + 1];
         qa[q][i >> 1][i & 1] = pack_f16x2_sat(a, b);
       }
+    }
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const int r = 8 * q + 2 * c + k, row = p.row0 + r;
-        const bool is = r < R;
-        const int tr = is ? row / G : 0;
-        le[q][k] = is ? __ldg(p.lse + (long long)(q0 + tr) * (KVH * G) + h * G + row - tr * G) * 1.4426950408889634f
-                       : __int_as_float(0x7f800000);              // (a row that does not exist: its scores are 0 - inf)
-        lim[q][k] = is ? L - ql + tr + 1 : 0;       // sees the keys below this one
-        from[q][k] = is && p.window > 0 ? L - ql + tr + 1 - p.window : 0;
-      }
+    for (int q = 0; q < QT; ++q) {
+      le[q][0] *= 1.4426950408889634f;
+      le[q][1] *= 1.4426950408889634f;
     }
     // tokens of [w_hi, t_lo) and whole sinks are seen by every row that exists
     const int t_lo = L - ql + p.row0 / G + 1;
     const int w_hi = p.window > 0 ? L - ql + (p.row0 + R - 1) / G + 1 - p.window : 0;
+    const int lo_w = p.window > 0 ? L - ql + p.row0 / G + 1 - p.window : 0;
     float* wrow = p.w + (long long)cw.b * p.w_b + (long long)h * p.w_h;
     while (true) {
-      const uint32_t bar = bars_a + 8 * (c_n % NS), st = ring_a + (c_n % NS) * Gm::STAGE;
+      const uint32_t bar = bars_a + 8 * c_st, st = ring_a + c_st * Gm::STAGE;
       const int tok0 = (cw.u + (cw.u >= cw.r.su ? cw.r.skip : 0)) * UT;
       // this lane's token of the unit, whose weight it adds to: block c / 2, row r0 or r1
       const int mine = tok0 + 16 * (c >> 1) + (c & 1 ? r1 : r0);
       const bool masked = tok0 + UT > t_lo || (tok0 < w_hi && tok0 + UT > p.sinks);
-      const int lo_w = p.window > 0 ? L - ql + p.row0 / G + 1 - p.window : 0;
       const bool add = mine < L && (mine >= lo_w || mine < p.sinks);
       float old = add ? wrow[mine] : 0.0f;
-      if (!mbar_try_wait_u32(bar, (c_n / NS) & 1) && !mbar_wait_bounded_u32(bar, (c_n / NS) & 1)) {
+      if (!mbar_try_wait_u32(bar, c_par) && !mbar_wait_bounded_u32(bar, c_par)) {
         if (lane == 0) atomicExch(p.status, HKV_ERR_DEVICE_WAIT);
         dead = true;
         break;
@@ -410,8 +455,9 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
           for (int k = 0; k < 2; ++k) {
             float pa = fast_exp2(fmaf(x[q][k], sc, -le[q][k])), pb = fast_exp2(fmaf(x[q][2 + k], sc, -le[q][k]));
             if (masked) {                           // (warp-uniform)
-              pa = ta < lim[q][k] && (ta >= from[q][k] || ta < p.sinks) ? pa : 0.0f;
-              pb = tb < lim[q][k] && (tb >= from[q][k] || tb < p.sinks) ? pb : 0.0f;
+              auto sees = [&](int t) { return t < lim[q][k] && (p.window == 0 || t >= lim[q][k] - p.window || t < p.sinks); };
+              pa = sees(ta) ? pa : 0.0f;
+              pb = sees(tb) ? pb : 0.0f;
             }
             sum[bi][0] += pa;
             sum[bi][1] += pb;
@@ -425,7 +471,11 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
       s1 += __shfl_xor_sync(0xffffffffu, up ? sum[0][1] : sum[1][1], 2);
       const float s = (odd ? s1 : s0) + __shfl_xor_sync(0xffffffffu, odd ? s0 : s1, 1);
       if (add) wrow[mine] = old + s;
-      ++c_n;
+      --ahead;
+      if (++c_st == NS) {
+        c_st = 0;
+        c_par ^= 1;
+      }
       __syncwarp();
       if (f_more) fetch();                          // (into the stage just read)
       if (++cw.u == cw.end) {
@@ -435,7 +485,13 @@ __global__ void __launch_bounds__(kWtThreads) weights_kernel(const WeightsParams
     }
   }
   if (dead)                                         // nothing of this warp's may still be on its way when the CTA ends
-    for (; c_n < f_n; ++c_n) (void)mbar_wait_bounded_u32(bars_a + 8 * (c_n % NS), (c_n / NS) & 1);
+    for (; ahead > 0; --ahead) {
+      (void)mbar_wait_bounded_u32(bars_a + 8 * c_st, c_par);
+      if (++c_st == NS) {
+        c_st = 0;
+        c_par ^= 1;
+      }
+    }
 }
 
 template <int D, int LAYOUT, int QT>
@@ -451,6 +507,13 @@ static int launch_weights(const WeightsParams& p, cudaStream_t st) {
   if (e != cudaSuccess) return record_cuda(e);
   if (ctas < 1) return HKV_ERR_UNSUPPORTED;
   return record_cuda(launch_pdl(k, dim3((unsigned)(sms * ctas)), dim3(kWtThreads), smem, st, p));
+}
+
+template <int QT>
+static int launch_weights_any(const WeightsParams& p, int D, int layout, cudaStream_t st) {
+  if (D == 128) return layout == 0 ? launch_weights<128, 0, QT>(p, st) : layout == 1 ? launch_weights<128, 1, QT>(p, st) : launch_weights<128, 3, QT>(p, st);
+  return layout == 0 ? launch_weights<256, 0, QT>(p, st) : layout == 1 ? launch_weights<256, 1, QT>(p, st)
+         : layout == 2 ? launch_weights<256, 2, QT>(p, st) : launch_weights<256, 3, QT>(p, st);
 }
 
 }  // namespace hkv
@@ -506,18 +569,11 @@ extern "C" int hkv_accumulate_weights(const void* q, const void* kd, const void*
   p.scale_log2 = sm_scale * 1.4426950408889634f;
   p.rot_scale = (float)(1.0 / sqrt((double)D));
   cudaStream_t st = (cudaStream_t)stream;
-  const bool two = G * qlmax > 8;
-  for (p.row0 = 0; p.row0 < G * qlmax; p.row0 += two ? 16 : 8) {
-    int rc;
-    if (D == 128)
-      rc = layout == 0 ? (two ? launch_weights<128, 0, 2>(p, st) : launch_weights<128, 0, 1>(p, st))
-           : layout == 1 ? (two ? launch_weights<128, 1, 2>(p, st) : launch_weights<128, 1, 1>(p, st))
-                         : (two ? launch_weights<128, 3, 2>(p, st) : launch_weights<128, 3, 1>(p, st));
-    else
-      rc = layout == 0 ? (two ? launch_weights<256, 0, 2>(p, st) : launch_weights<256, 0, 1>(p, st))
-           : layout == 1 ? (two ? launch_weights<256, 1, 2>(p, st) : launch_weights<256, 1, 1>(p, st))
-           : layout == 2 ? (two ? launch_weights<256, 2, 2>(p, st) : launch_weights<256, 2, 1>(p, st))
-                         : (two ? launch_weights<256, 3, 2>(p, st) : launch_weights<256, 3, 1>(p, st));
+  // query rows of a pass: 8, 16 or 32
+  const int QT = G * qlmax <= 8 ? 1 : G * qlmax <= 16 ? 2 : 4;
+  for (p.row0 = 0; p.row0 < G * qlmax; p.row0 += 8 * QT) {
+    const int rc = QT == 1 ? launch_weights_any<1>(p, D, layout, st) : QT == 2 ? launch_weights_any<2>(p, D, layout, st)
+                                                                         : launch_weights_any<4>(p, D, layout, st);
     if (rc != HKV_OK) return rc;
   }
   return HKV_OK;
