@@ -228,6 +228,12 @@ def _build_classes():
             # prefill rows (backend.py:229, :16-25 of the reference): fp16 compute dtype, context chunk in tokens
             self.pf16 = _env("HORIZON_KVFP4_PF16", "1") == "1"
             self.prefill_chunk = max(16, int(_env("HORIZON_KVFP4_CHUNK", "65536")))
+            # HORIZON_KVFP4_WINDOW=n: a model trained with full attention is served over its last n tokens and the first
+            # HORIZON_KVFP4_SINKS ones (a server's choice, not the model's: `sliding_window` above stays refused)
+            self.window = int(_env("HORIZON_KVFP4_WINDOW", "0"))
+            self.sinks = int(_env("HORIZON_KVFP4_SINKS", "4")) if self.window else 0
+            if self.window < 0 or self.sinks < 0:
+                raise ValueError("HORIZON_KVFP4_WINDOW and HORIZON_KVFP4_SINKS are numbers of tokens, not negative")
             self._gk = self._gv = None
             self._views = None
             nspec, max_reqs = 0, int(kwargs.get("max_num_seqs", 0) or 0)
@@ -339,7 +345,7 @@ def _build_classes():
             gk, gv = (self._gk, self._gv) if self._gk is not None else self._scales(layer, query.device)
             decode = m.has_decode and m.num_reqs > 0
             self._keep_to(kv_cache)
-            if decode:                                # as in do_kv_cache_update: the usual arguments as they are
+            if decode and not self.window:            # as in do_kv_cache_update: the usual arguments as they are
                 rc = (_lib._host or _lib.host()).layer_decode(
                     query, kv_cache, m.block_table, m.seq_lens, m.query_start_loc, T, self.scale, float(layer._v_scale_float),
                     gk, gv, m.qlmax, output, st["ws"], self.cps, self.num_heads, self.head_size,
@@ -357,7 +363,11 @@ def _build_classes():
             if not q.is_contiguous():
                 q = q.contiguous()
             out = output.view(output.shape[0], self.num_heads, self.head_size) if output.dim() == 2 else output
-            if decode:
+            if decode and self.window:
+                K.decode_window(q, v["flat"], v["strides"], v["PS"], m.block_table, m.seq_lens, m.query_start_loc,
+                                self.scale, float(layer._v_scale_float), gk, gv, m.qlmax, out, st["ws"], self.window, self.sinks,
+                                splits=self.cps or None, signs=self._rot(q.device), k8=self.k8)
+            elif decode:
                 K.decode_ragged(q, v["flat"], v["strides"], v["PS"], m.block_table, m.seq_lens, m.query_start_loc,
                                 self.scale, float(layer._v_scale_float), gk, gv, m.qlmax, out, st["ws"],
                                 splits=self.cps or None, signs=self._rot(q.device), k8=self.k8)
@@ -388,9 +398,13 @@ def _build_classes():
             direct = out.is_contiguous() and out.data_ptr() % 16 == 0 and out.dtype in (torch.bfloat16, torch.float32)
             o = out if direct else torch.empty(out.shape, dtype=torch.float32, device=out.device)
             bt = m.block_table if m.block_table.is_contiguous() else m.block_table.contiguous()
-            K.prefill(q, v["flat"], v["strides"], v["PS"], bt, rows, self.scale * float(layer._k_scale_float),
-                      float(layer._v_scale_float), self.num_kv_heads, o, chunk=self.prefill_chunk, signs=signs, k8=self.k8,
-                      workspace=self._state(q.device)["ws"])
+            args = (q, v["flat"], v["strides"], v["PS"], bt, rows, self.scale * float(layer._k_scale_float),
+                    float(layer._v_scale_float), self.num_kv_heads, o)
+            more = dict(chunk=self.prefill_chunk, signs=signs, k8=self.k8, workspace=self._state(q.device)["ws"])
+            if self.window:
+                K.prefill_window(*args, self.window, self.sinks, **more)
+            else:
+                K.prefill(*args, **more)
             if not direct:
                 for _, q0, q1, _ in rows:
                     out[q0:q1].copy_(o[q0:q1])

@@ -8,6 +8,9 @@ module is what the ncu summaries of the other kernels and variants are captured 
     python -m horizon_kernels_b200.microbench pipes
     python -m horizon_kernels_b200.microbench decode  [--batch 192] [--kvh 2] [--g 8] [--d 256] [--min-len 128]
                                                       [--max-len 32768] [--iters 10] [--had] [--k8] [--nhd] [--ql 1]
+                                                      [--window 0] [--sinks 4]
+    python -m horizon_kernels_b200.microbench weights (the arguments of decode)
+    python -m horizon_kernels_b200.microbench evict   (the arguments of decode) [--keep 2048] [--recent 256]
 """
 import argparse
 import json
@@ -91,7 +94,7 @@ def dequant(a):
 
 
 def decode(a):
-    """One decode step over a hybrid batch: context lengths log-uniform in [min-len, max-len], pages scattered over the
+    """One decode step (or the weights that its queries leave, or an eviction to new pages) over a hybrid batch: context lengths log-uniform in [min-len, max-len], pages scattered over the
     pool, the cache filled by the write kernel. Every iteration reads the whole cache of the batch once; the batch is
     sized by --batch so that this is several times the L2."""
     B, KVH, G, D, PS = a.batch, a.kvh, a.g, a.d, 16
@@ -101,10 +104,12 @@ def decode(a):
             for x in u]
     pages = [(n + PS - 1) // PS for n in lens]
     tot, MP = sum(pages), max(pages)
-    NP = tot + tot // 4 + 8
+    OMP = (a.keep + PS - 1) // PS if a.kernel == "evict" else 0
+    NP = tot + tot // 4 + 8 + B * OMP
     flat, st, pool = _pool(NP, KVH, D, PS, a.k8, a.nhd)
     signs = K.hadamard_signs(D, device="cuda") if a.had else None
-    perm = torch.randperm(NP, generator=g, device="cuda")[:tot]
+    perm = torch.randperm(NP - 1, generator=g, device="cuda") + 1
+    fresh, perm = perm[tot:tot + B * OMP].to(torch.int32).view(B, OMP), perm[:tot]
     bt = torch.zeros((B, MP), dtype=torch.int32, device="cuda")
     o = 0
     for b, n in enumerate(pages):
@@ -127,15 +132,41 @@ def decode(a):
     qsl = torch.arange(B + 1, dtype=torch.int32, device="cuda") * ql
     out = torch.empty_like(q)
     ws = K.alloc_workspace(B, KVH, G, D, ql, "cuda")
-    ms = _time(lambda: K.decode_ragged(q, flat, st, PS, bt, sl, qsl, D ** -0.5, 1.0, gk, gv, ql, out, ws, signs=signs,
-                                       k8=a.k8), a.iters)
-    if K.workspace_status(ws) != 0 or not bool(torch.isfinite(out.float()).all()):
+    more = {}
+    if a.kernel == "decode" and not a.window:
+        def call():
+            K.decode_ragged(q, flat, st, PS, bt, sl, qsl, D ** -0.5, 1.0, gk, gv, ql, out, ws, signs=signs, k8=a.k8)
+    else:
+        lse = torch.empty(q.shape[:2], device="cuda")
+
+        def call():
+            K.decode_window(q, flat, st, PS, bt, sl, qsl, D ** -0.5, 1.0, gk, gv, ql, out, ws, a.window, a.sinks, signs=signs, k8=a.k8, lse=lse)
+    seen = [n if not a.window else min(n, a.window + ql - 1) + min(max(0, n - a.window - ql + 1), a.sinks) for n in lens]
+    byts = sum(seen) * KVH * _token_bytes(D, a.k8)
+    if a.kernel != "decode":
+        call()
+        w = torch.zeros((B, KVH, max(lens)), device="cuda")
+
+        def call():
+            K.accumulate_weights(q, flat, st, PS, bt, sl, qsl, D ** -0.5, gk, ql, lse, w, window=a.window, sinks=a.sinks, signs=signs, k8=a.k8)
+        byts = sum(seen) * KVH * ((D if a.k8 else Lt.slot_bytes(D)) + 8)
+    if a.kernel == "evict":
+        call()
+        kept, nl = torch.empty((B, KVH, a.keep), dtype=torch.int32, device="cuda"), torch.empty((B,), dtype=torch.int32, device="cuda")
+        nw = torch.empty((B, KVH, a.keep), device="cuda")
+
+        def call():
+            K.evict(flat, st, PS, D, bt, sl, w, a.keep, a.sinks, a.recent, kept, nl, out_tables=fresh, out_weights=nw, k8=a.k8)
+        byts = sum(KVH * (4 * n + min(n, a.keep) * (2 * _token_bytes(D, a.k8) + 8)) for n in lens)
+        more = {"keep": a.keep, "recent": a.recent}
+    ms = _time(call, a.iters)
+    if K.workspace_status(ws) != 0 or K.workspace_status(None) != 0 or not bool(torch.isfinite(out.float()).all()):
         raise RuntimeError("decode reported a wait that ran out, or a non-finite output")
-    byts = sum(lens) * KVH * _token_bytes(D, a.k8)
-    print(json.dumps({"kernel": "decode", "batch": B, "kv_heads": KVH, "group": G, "head_dim": D,
+    print(json.dumps({"kernel": a.kernel, "batch": B, "kv_heads": KVH, "group": G, "head_dim": D,
                       "rotated": a.had, "k8": a.k8, "positions_outermost_pages": a.nhd, "query_tokens": ql,
                       "query_rows_per_kv_head": G * ql, "cached_tokens": sum(lens), "cache_mb": byts / 1e6,
-                      "us": ms * 1e3, "algorithmic_gbs": byts / ms / 1e6}))
+                      "us": ms * 1e3, "algorithmic_gbs": byts / ms / 1e6,
+                      **({"window": a.window, "sinks": a.sinks} if a.window else {}), **more}))
 
 
 def pipes(a):
@@ -163,7 +194,7 @@ def pipes(a):
 
 def main():
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("kernel", choices=["write", "dequant", "decode", "pipes"])
+    ap.add_argument("kernel", choices=["write", "dequant", "decode", "weights", "evict", "pipes"])
     ap.add_argument("--tokens", type=int, default=None)
     ap.add_argument("--kvh", type=int, default=None)
     ap.add_argument("--d", type=int, default=None, choices=[128, 256])
@@ -175,16 +206,20 @@ def main():
     ap.add_argument("--k8", action="store_true", help="the FP8-key slot (head_dim 256)")
     ap.add_argument("--ql", type=int, default=1, help="decode: query tokens per request (group x ql rows per kv head)")
     ap.add_argument("--nhd", action="store_true", help="decode: pages with positions outermost (row-copy path)")
+    ap.add_argument("--window", type=int, default=0, help="decode, weights: a query token sees its last WINDOW tokens and the first SINKS")
+    ap.add_argument("--sinks", type=int, default=4)
+    ap.add_argument("--keep", type=int, default=2048, help="evict: tokens that stay, the first SINKS and the last RECENT among them")
+    ap.add_argument("--recent", type=int, default=256)
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--f16", action="store_true")
     a = ap.parse_args()
     if a.tokens is None:
         a.tokens = 32768 if a.kernel == "write" else 262144
     if a.kvh is None:
-        a.kvh = 2 if a.kernel == "decode" else 8
+        a.kvh = 2 if a.kernel in ("decode", "weights", "evict") else 8
     if a.d is None:
-        a.d = 256 if (a.kernel == "decode" or a.k8) else 128
-    {"write": write, "dequant": dequant, "decode": decode, "pipes": pipes}[a.kernel](a)
+        a.d = 256 if (a.kernel in ("decode", "weights", "evict") or a.k8) else 128
+    {"write": write, "dequant": dequant, "decode": decode, "weights": decode, "evict": decode, "pipes": pipes}[a.kernel](a)
 
 
 if __name__ == "__main__":

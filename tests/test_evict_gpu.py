@@ -191,3 +191,69 @@ def test_lengths_beyond_the_table_and_the_weights_are_cut():
     assert ol.tolist() == [32, 0] and (kept[1] == -1).all()
     for h in range(2):
         assert np.array_equal(kept[0, h].cpu().numpy(), R.kept_positions(w0[0, h].cpu().numpy(), 32, 0, 0))
+
+
+@pytest.mark.parametrize("where", ["new", "own"])
+@pytest.mark.parametrize("D,offset,pad", [(128, 8, 0), (128, 0, 8), (128, 24, 40), (256, 16, 48), (256, 48, 16)])
+def test_caches_off_the_16_byte_grid(D, offset, pad, where):
+    """a cache that begins at, or whose pages are apart by, an odd multiple of 8 bytes (head_dim 128), where no bulk copy may go"""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    KVH, PS, pages, keep, L = 2, 16, 60, 70, 400
+    slot = Lt.slot_bytes(D)
+    page = 2 * KVH * PS * slot + pad
+    mem = torch.randint(0, 256, (offset + pages * page,), dtype=torch.uint8, device="cuda", generator=g)
+    cache = torch.as_strided(mem, (pages, 2 * KVH, PS, slot), (page, PS * slot, slot, 1), offset)
+    flat, st = Lt.flat_views(*Lt.slot_views(cache, KVH, D))
+    bt = torch.arange(1, 26, dtype=torch.int32, device="cuda").view(1, 25)
+    ot = torch.arange(30, 35, dtype=torch.int32, device="cuda").view(1, 5) if where == "new" else None
+    w = torch.rand(1, KVH, L, device="cuda", generator=g)
+    w0, before = w.cpu(), mem.cpu().clone()
+    kept, ol = torch.zeros((1, KVH, keep), dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    K.evict(flat, st, PS, D, bt, torch.tensor([L], dtype=torch.int32, device="cuda"), w, keep, 2, 9, kept, ol, out_tables=ot,
+            out_weights=None if ot is None else torch.zeros(1, KVH, keep, device="cuda"))
+    want = before.clone()
+    old, new = (torch.as_strided(m, cache.shape, cache.stride(), offset) for m in (before, want))
+    tab = (bt if ot is None else ot).cpu().long()[0]
+    r = torch.arange(keep)
+    for h in range(KVH):
+        j = torch.from_numpy(R.kept_positions(w0[0, h].numpy(), keep, 2, 9))
+        for side in (h, KVH + h):
+            new[tab[r // PS], side, r % PS] = old[bt.cpu().long()[0][j // PS], side, j % PS]
+    assert torch.equal(mem.cpu(), want)
+
+
+def test_pages_shared_by_requests_move_to_new_ones():
+    """a prefix that two requests share is read by both and stays as it is"""
+    g = torch.Generator(device="cuda").manual_seed(6)
+    phys, flat, st = cache_of("hnd", 60, 16, 2, 128, g)
+    bt = torch.tensor([list(range(1, 21)), list(range(1, 11)) + list(range(21, 31))], dtype=torch.int32, device="cuda")
+    ot = torch.arange(40, 50, dtype=torch.int32, device="cuda").view(2, 5)
+    w = torch.rand(2, 2, 320, device="cuda", generator=g)
+    kept, ol = torch.zeros((2, 2, 80), dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    ow, before = torch.zeros(2, 2, 80, device="cuda"), phys.cpu().clone()
+    K.evict(flat, st, 16, 128, bt, torch.tensor([320, 311], dtype=torch.int32, device="cuda"), w, 80, 4, 16, kept, ol, out_tables=ot, out_weights=ow)
+    after = phys.cpu()
+    assert torch.equal(after[:40], before[:40])
+    r = torch.arange(80)
+    for b in range(2):
+        for h in range(2):
+            j = kept[b, h].long().cpu()
+            for side in (h, 2 + h):
+                assert torch.equal(after[ot[b].long().cpu()[r // 16], side, r % 16], before[bt[b].long().cpu()[j // 16], side, j % 16])
+
+
+def test_weights_that_are_rows_of_a_wider_tensor():
+    g = torch.Generator(device="cuda").manual_seed(8)
+    phys, flat, st = cache_of("hnd", 40, 16, 2, 128, g)
+    bt = torch.arange(1, 33, dtype=torch.int32, device="cuda").view(2, 16)
+    big = torch.rand(2, 3, 2, 300, device="cuda", generator=g)
+    w, rest = big[:, 1, :, 20:276], big.clone()
+    kept, ol = torch.zeros((2, 2, 64), dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+    sl = torch.tensor([256, 100], dtype=torch.int32, device="cuda")
+    K.evict(flat, st, 16, 128, bt, sl, w, 64, 1, 5, kept, ol)
+    for b, L in enumerate(sl.tolist()):
+        for h in range(2):
+            old = rest[b, 1, h, 20:276].clone()
+            assert torch.equal(w[b, h, :64], old[kept[b, h].long()]) and bool((w[b, h, 64:L] == 0).all()) and torch.equal(w[b, h, L:], old[L:])
+    big[:, 1, :, 20:276] = rest[:, 1, :, 20:276]
+    assert torch.equal(big, rest)
