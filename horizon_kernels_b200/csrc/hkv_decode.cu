@@ -119,7 +119,10 @@ struct Smem {
 };
 
 // WIN: over a sliding window and the first tokens. The units between them are not part of the stream, those at their edges are
-// masked like the last unit of a sequence; the rows' log-sum-exps are stored too when the caller wants them.
+// masked like the last unit of a sequence; the rows' log-sum-exps are stored too when the caller wants them. Against a decode of as
+// many tokens, which bounds it: 64 requests, 8 kv heads x 128, window 4096 and 4 sinks 75.9 us, 4100 tokens 71.2; 96 requests, 2 x 256,
+// group 8, 2047 and 5: 42.0 and 39.3 us, with two query tokens 59.2 and 54.1; four requests, 1024 and 4: 13.9 and 12.5 (a unit more
+// at either end of the window, three masked ones instead of one).
 template <int D, int LAYOUT, int QT, bool WIN>
 __device__ __forceinline__ void decode_body(const DecodeParams& p) {
   using Gm = Geo<D, LAYOUT>;

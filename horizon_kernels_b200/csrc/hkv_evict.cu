@@ -28,7 +28,6 @@ constexpr int kEvBins = 2048;
 constexpr int kEvCluster = 8;
 constexpr int kSelRegs = 32;                        // weights of a thread that stay in registers
 constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
-constexpr int kMoveCtas = 592;
 
 struct EvictParams {
   uint8_t* kd;
@@ -59,6 +58,7 @@ __device__ __forceinline__ uint32_t cluster_rank() {
   return r;
 }
 __device__ __forceinline__ void cluster_sync() {
+  __syncwarp();                                     // (.aligned: the warp's lanes come together)
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ int peer_load(const int* p, uint32_t rank) {   // *p of another CTA of the cluster
@@ -94,6 +94,10 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 // A warp has a run of the CTA's tokens, 32 at a time, a lane one of them: the order of (warp, turn, lane) is that of the tokens.
 // The first kSelRegs turns stay in registers from pass to pass, further ones (contexts beyond 8 x 16384 tokens) are read again.
+// What bounds it: the longest context's chain of phases. One CTA, 14400 tokens (clocks): 7000 for the loads, 13000 for the first
+// pass (shared-memory atomics; a weight's leading bits agree with several of its neighbours'), 1000 for each look at the bins, 1000
+// for the second pass, 5000 for counts and ranks. Loads behind a branch each took 23000. 256 threads (one wave of CTAs where 512 take
+// two) took 41 us instead of 27 for 64 requests of 1.5k to 16k tokens, 1024 threads 31 to 36: the long ones decide.
 __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParams p) {
   __shared__ __align__(16) int hist[kEvBins];
   __shared__ int wsum[kSelWarps], counts[2 * kSelWarps], totals[2], found[3], slice;
@@ -251,8 +255,10 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
 // piece by piece (PB bytes: 8 at head_dim 128, whose rows are 8-byte aligned, 16 at 256; a row is 8 pieces of codes, FP8 keys
 // 16 before them, and one of scales), and writes the tile out: with one bulk copy a side where rows lie back to back in the
 // cache, else piece by piece. The rows hold no registers on their way, so that a warp has the next tile in flight while it
-// writes this one. 64 requests of 1.5k to 16k tokens to 2048, 8 kv heads x 128: 75 us with the rows in registers and 8-byte
-// stores (bound by the L1's work on them and the address arithmetic), MEASURE now.
+// writes this one. 64 requests of 1.5k to 16k tokens cut to 2048, 8 kv heads x 128 (302 MB moved): 83 us with the rows in
+// registers and 8-byte stores, which the L1 and the address arithmetic bound; 67 now (profiled), for 350 MB of DRAM traffic: rows
+// of 72 bytes here and there cost whole 32-byte sectors. In one piece (nothing evicted) the launch moves the 302 MB in 54 us. Eight
+// tokens a tile at head_dim 256, where sixteen leave room for fewer warps: 71 -> 65 us (8 requests of 131072 to 16384, 2 x 256).
 template <int D, bool K8>
 struct EvGeo {
   static constexpr int PB = D == 128 ? 8 : 16;
@@ -455,8 +461,15 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   const long long reach = (long long)MP * PS;
   p.max_len = (int)(reach < W ? reach : W);               // (a length beyond the table or the weights is cut there)
   const long long pairs = (long long)B * KVH;
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return record_cuda(e);
+  // CTAs per (request, kv head) for the selection. A cluster divides the work of a long context but meets four times a pass: 8192
+  // tokens of 8 heads take 13.4 us with one CTA each (both launches), 14.9 with four; 30000 tokens of 2 heads 31.8 with one, 20.3,
+  // 17.3 and 16.8 with two, four and eight. With more (request, kv head) pairs than SMs one CTA each: 512 pairs 107 us, two each 121.
   int nc = kEvCluster;
-  while (nc > 1 && (pairs * nc > 600 || p.max_len < nc * 2048 || p.max_len <= 8192)) nc /= 2;
+  while (nc > 1 && (pairs * nc > 4 * sms || p.max_len < nc * 2048 || p.max_len <= 8192)) nc /= 2;
   cudaStream_t st = (cudaStream_t)stream;
   int rc = launch_clusters(select_kernel, p, nc, KVH, B, nc, kSelThreads, 0, st);
   if (rc != HKV_OK) return rc;
@@ -469,8 +482,9 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   rc = record_cuda(cudaFuncSetAttribute((const void*)mk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (rc != HKV_OK) return rc;
   if (cluster) return launch_clusters(mk, p, kEvCluster, KVH, B, kEvCluster, kMoveThreads, smem, st);
-  // as many CTAs per (request, kv head) as find work at once
+  // one wave of four CTAs an SM, or as many as find work at once (64 requests, 8 kv heads, to 2048 tokens: 592 CTAs 112.6 us, 740 (in
+  // 1.3 waves) 113, 5920 120; with the launch of an earlier step)
   const long long most = keep < p.max_len ? keep : p.max_len, round = kMoveWarps * (D == 128 ? 16 : 8);
-  const long long x = std::max(1ll, std::min((most + round - 1) / round, (kMoveCtas + pairs - 1) / pairs));
+  const long long x = std::max(1ll, std::min((most + round - 1) / round, (4 * sms + pairs - 1) / pairs));
   return record_cuda(launch_pdl(mk, dim3((unsigned)x, (unsigned)KVH, (unsigned)B), dim3(kMoveThreads), smem, st, p));
 }

@@ -8,6 +8,9 @@
 //                   handed to the value product through tensor memory
 //   merge_kernel    joins the parts of row tiles whose keys were divided among CTAs (only when there are any)
 //
+// WIN: over a sliding window and the first tokens. Key tiles between a request's sinks and the window of its first token are never
+// made; a row tile goes over its sink tiles and those of its window, in one piece (PfSpan).
+//
 // Replaces the reference's library attention over dequantised tokens (backend.py:438-543).
 //
 // Layer steps on a B200 (write launch included): a fresh prompt of 6144 tokens, 32 query heads over 8 kv heads, head_dim 128:
@@ -34,7 +37,8 @@ constexpr int kPieceCost = 3;          // cost of starting and ending a piece, i
 // one of the first ten: the output's rescaling, between one value product and the next, is what a tile waits for. With 16-bit
 // outputs the maximum therefore lags by up to 2^8, as in the decode kernel: probabilities stay within f16's range at its 2^-11 of
 // each, and what is lost against a largest probability of exactly 1, about 2e-4 of the output (2-norm), lies a factor of eight
-// below the output's own rounding. MEASURE. fp32 outputs keep the exact maximum.
+// below the output's own rounding (1.7e-3 against 64 bits with and without). 6144 tokens, window 1024: 151.8 us with the exact
+// maximum, 149.4 with the lag; 2048 tokens over 30000 at head_dim 256, window 4096: 150.2 and 143. fp32 outputs keep the exact one.
 constexpr float kPfLag = 8.0f;
 constexpr int kMinPiece = 2;           // no piece of a divided row tile is shorter, in key tiles
 constexpr int kStageBytes = 32768;

@@ -21,6 +21,7 @@ int noalloc_workspace(void** ws);
 
 constexpr int kWtWarps = 4;
 constexpr int kWtThreads = kWtWarps * 32;
+// (cost / least units of 4 / 2, 2 / 2 and 2 / 1: four requests of 2048 tokens, 8 kv heads x 128, 9.2, 7.6 and 6.8 us; 8 / 2: 12.5)
 constexpr int kWtCost = 2;           // what a sequence costs a warp beyond its units (its queries and log-sum-exps), in units
 constexpr int kWtMin = 1;            // least units of a warp
 
@@ -28,7 +29,7 @@ struct WeightsParams {
   const __nv_bfloat16* q;
   const uint8_t* kd;
   const uint8_t* ksf;
-  long long dst, dsh, sst, ssh;
+  long long dst, dsh, ssh;
   unsigned dsp, ssp;
   const int* bt;
   const int* seq_lens;
@@ -54,7 +55,7 @@ struct WtGeo {
   static constexpr int ROW = LAYOUT == 1 ? SD : SD + SS;             // byte stride between token rows of a stage
   static constexpr int SF_BASE = LAYOUT == 1 ? UT * SD : SD, SF_ROW = LAYOUT == 1 ? SS : ROW;
   static constexpr int STAGE = UT * (SD + SS);
-  static constexpr int NS = 2;
+  static constexpr int NS = 2;         // (8 requests of 131072, 8 x 128: 139.2 us with two stages, 139.8 with three or four)
   static constexpr int KS = D / 16, NBL = D / 64, KB = K8 ? 16 : 8;
   // 72-byte rows: as in the decode kernel, so that the lanes' loads touch every bank once
   __device__ static constexpr int tok(int i) {
@@ -82,6 +83,14 @@ __device__ __forceinline__ WtReq wt_req(const WeightsParams& p, int b) {
   return r;
 }
 
+// QT: 8-row query tiles of a pass. Four (32 rows, their fragments in registers, two CTAs per SM at head_dim 256) against two passes of
+// two: 32 requests of 1k to 16k tokens, 2 x 256, group 8 x 4 tokens 34 us against 50.
+//
+// What bounds it (8 requests of 131072 tokens, 8 x 128, group 8; 0.74 of the copy peak): instruction issue, 65 % used, and dependency
+// latency; 186 warp instructions per 16 tokens, 64 of them the conversions and scale products of the keys (ALU pipe 53 %). More CTAs
+// at fewer registers are slower: 126 registers 139 us, 96 165, 80 169. With 32 rows at head_dim 256 a launch is start-up: of 54000
+// clocks 4000 locate and fetch, 11000 load the queries, 3900 are each unit's (tensor pipe 25 %). Rolling a unit's two blocks, for the
+// instruction cache, gained nothing (16 rows over 131072: 188 -> 197 us).
 template <int D, int LAYOUT, int QT>
 __global__ void __launch_bounds__(kWtThreads, D == 128 ? (QT == 1 ? 4 : 3) : QT == 1 ? 3 : 2) weights_kernel(const WeightsParams p) {
   using Gm = WtGeo<D, LAYOUT>;
@@ -554,7 +563,7 @@ extern "C" int hkv_accumulate_weights(const void* q, const void* kd, const void*
   WeightsParams p;
   p.q = (const __nv_bfloat16*)q;
   p.kd = (const uint8_t*)kd; p.ksf = (const uint8_t*)ksf;
-  p.dsp = (unsigned)dsp; p.ssp = (unsigned)ssp; p.dst = dst; p.dsh = dsh; p.sst = sst; p.ssh = ssh;
+  p.dsp = (unsigned)dsp; p.ssp = (unsigned)ssp; p.dst = dst; p.dsh = dsh; p.ssh = ssh;
   p.bt = block_tables; p.seq_lens = seq_lens; p.qsl = query_start_loc; p.gk = gk; p.lse = lse; p.signs = signs;
   p.w = weights; p.w_b = w_b; p.w_h = w_h;
   p.status = &((Header*)workspace)->status;

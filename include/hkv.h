@@ -204,7 +204,7 @@ int hkv_dequant_k8(const void* kd, const void* vd, const void* vsf, const int64_
 /*
  * Process-wide options. No counterpart in the reference.
  *   HKV_OPT_EARLY_METADATA (0 = off, the default; 1 = on): the caller states that `seq_lens` and `query_start_loc` of
- *     every later hkv_decode / hkv_decode_noalloc call are complete before the kernel that PRECEDES the call on its
+ *     every later hkv_decode / hkv_decode_window / hkv_decode_noalloc call are complete before the kernel that PRECEDES the call on its
  *     stream starts (an inference engine writes them once per step, long before the attention layers run; hkv_write never
  *     writes them). hkv_decode then reads these two arrays while the preceding kernel is still running and waits for
  *     it only afterwards, before it touches the block tables, the cache, the queries or the workspace. With the option
