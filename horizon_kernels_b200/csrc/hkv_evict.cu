@@ -27,6 +27,7 @@ constexpr int kSelThreads = 512, kSelWarps = kSelThreads / 32;
 constexpr int kEvBins = 2048;
 constexpr int kEvCluster = 8;
 constexpr int kSelRegs = 32;                        // weights of a thread that stay in registers
+constexpr int kSmall = 32 * kSelRegs;               // tokens that one warp selects from
 constexpr int kMoveThreads = 256, kMoveWarps = kMoveThreads / 32;
 
 struct EvictParams {
@@ -43,7 +44,7 @@ struct EvictParams {
   float* ow;
   long long w_b, w_h, ow_b, ow_h;                   // element strides of the weights
   int* kept;
-  int MP, OMP, lps, KVH, keep, sinks, recent, max_len, OW;
+  int B, MP, OMP, lps, KVH, keep, sinks, recent, max_len, OW;
   int bulk, split;                                  // a tile's new rows lie back to back and 16-byte aligned; codes apart from scales
 };
 
@@ -90,6 +91,79 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   if (w != w) return 0xffffffffu;
   if (u == 0x80000000u) return 0x80000000u;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+// The tokens of a context of at most kSmall, by one warp: the threshold bit by bit, every bit a count over the lanes' registers, no
+// barrier. Right for more (request, kv head) pairs than the CTAs of select_kernel fill SMs in one wave: 2048 pairs of 300 tokens, 100 stay,
+// 36 us against 80 (both launches), of 800 and 300 78 against 113; 512 of 300 19 against 22. A few pairs of 1000: 19 against 12.
+__device__ __forceinline__ void select_small(const float* w, int* kept, int lane, int L, int keep, int sinks, int recent) {
+  const int n = min(L, keep);
+  if (L <= keep) {
+    for (int r = lane; r < keep; r += 32) kept[r] = r < n ? r : -1;
+    return;
+  }
+  for (int i = lane; i < sinks; i += 32) kept[i] = i;
+  for (int i = lane; i < recent; i += 32) kept[keep - recent + i] = L - recent + i;
+  const int cnt = L - sinks - recent, need = keep - sinks - recent, turns = (cnt + 31) >> 5;
+  if (need == 0) return;
+  w += sinks;
+  uint32_t key[kSelRegs];
+#pragma unroll
+  for (int g = 0; g < kSelRegs; g += 8) {
+    float x[8];
+    if (g < turns) {
+#pragma unroll
+      for (int u = 0; u < 8; ++u) x[u] = w[min(32 * (g + u) + lane, cnt - 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) key[g + u] = g < turns && 32 * (g + u) + lane < cnt ? weight_key(x[u]) : 0u;
+  }
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int g = 0; g < kSelRegs; g += 4)
+      if (g < turns) {
+#pragma unroll
+        for (int u = g; u < g + 4; ++u) f(u, key[u]);
+      }
+  };
+  uint32_t low = 0;                                 // the need-th largest key, and whether others are equal to it
+  bool ties = true;
+#pragma unroll 1
+  for (uint32_t bit = 0x80000000u; bit != 0 && ties; bit >>= 1) {
+    int c = 0;
+    each([&](int, uint32_t k) { c += k >= (low | bit); });
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (c >= need) low |= bit;
+    ties = c != need;                               // (else exactly those stay)
+  }
+  int left = 0;
+  if (ties) {
+    int c = 0;
+    each([&](int, uint32_t k) { c += k > low; });
+    left = need - __reduce_add_sync(0xffffffffu, c);
+  } else {
+    --low;
+  }
+  const unsigned below = (1u << lane) - 1;
+  int gb = 0, eb = 0;
+  kept += sinks;
+  each([&](int u, uint32_t k) {
+    const unsigned bg = __ballot_sync(0xffffffffu, k > low), be = __ballot_sync(0xffffffffu, ties && k == low);
+    const int e = eb + __popc(be & below);
+    if (k > low || (ties && k == low && e < left)) kept[gb + __popc(bg & below) + min(e, left)] = sinks + 32 * u + lane;
+    gb += __popc(bg);
+    eb += __popc(be);
+  });
+}
+__global__ void __launch_bounds__(kMoveThreads) select_small_kernel(const EvictParams p) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, pair = blockIdx.x * kMoveWarps + (threadIdx.x >> 5);
+  const int b = pair / p.KVH, h = pair - b * p.KVH;
+  if (b >= p.B) return;
+  const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_len);
+  if (h == 0 && lane == 0) p.out_lens[b] = min(L, p.keep);
+  select_small(p.w + b * p.w_b + h * p.w_h, p.kept + (long long)pair * p.keep, lane, L, p.keep, p.sinks, p.recent);
 }
 
 // A warp has a run of the CTA's tokens, 32 at a time, a lane one of them: the order of (warp, turn, lane) is that of the tokens.
@@ -268,7 +342,6 @@ struct EvGeo {
   static constexpr int PIECES = ROWS * NP, TURNS = (PIECES + 31) / 32;
   static constexpr int TILE = PIECES * PB;
   static constexpr int WARP = 2 * (TILE + 16 * TOK);               // shared memory of a warp: two tiles, the rows' old places (codes, scales)
-  static constexpr int SMEM = kMoveWarps * WARP;
 };
 
 __device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
@@ -276,8 +349,8 @@ __device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes
 }
 
 // CLUSTER: calls in place; else a row in place, which the caller may mix in, is one CTA's work
-template <int D, bool K8, bool CLUSTER>
-__global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const EvictParams p) {
+template <int D, bool K8, bool CLUSTER, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) move_kernel(const EvictParams p) {
   using Gm = EvGeo<D, K8>;
   constexpr int PB = Gm::PB, NP = Gm::NP, T = Gm::TOK;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -311,8 +384,8 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const EvictParams
   };
   // The old place of a token hangs on two loads one after the other (position, page), its rows on those: the positions are
   // fetched two tiles ahead, the rows one. (Every CTA of a cluster takes every round, so that all of them meet at its barrier.)
-  const int stride = ctas * kMoveWarps * T;
-  int rt = (blockIdx.x * kMoveWarps + wp) * T;
+  const int stride = ctas * WARPS * T;
+  int rt = (blockIdx.x * WARPS + wp) * T;
   auto position = [&](int r) { return lane < T && r + lane < n ? __ldg(kept + r + lane) : -1; };
   int j = position(rt);
   float wv = 0.0f, wn = 0.0f;
@@ -392,7 +465,7 @@ __global__ void __launch_bounds__(kMoveThreads, 4) move_kernel(const EvictParams
   asm volatile("cp.async.wait_all;" ::: "memory");
   asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   // (in place: the last barrier lies behind every read)
-  for (int r = n + blockIdx.x * kMoveThreads + tid; r < min(L, p.OW); r += ctas * kMoveThreads) ow[r] = 0.0f;
+  for (int r = n + blockIdx.x * 32 * WARPS + tid; r < min(L, p.OW); r += ctas * 32 * WARPS) ow[r] = 0.0f;
 }
 
 template <typename K>
@@ -445,7 +518,7 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   p.bt = block_tables; p.out_bt = out_tables; p.seq_lens = seq_lens; p.out_lens = out_lens;
   p.w = weights; p.ow = out_weights; p.w_b = w_b; p.w_h = w_h; p.ow_b = ow_b; p.ow_h = ow_h;
   p.kept = kept;
-  p.MP = MP; p.OMP = OMP; p.KVH = KVH; p.keep = keep; p.sinks = sinks; p.recent = recent; p.OW = OW;
+  p.B = B; p.MP = MP; p.OMP = OMP; p.KVH = KVH; p.keep = keep; p.sinks = sinks; p.recent = recent; p.OW = OW;
   // rows back to back, and bulk copies' 16-byte alignment (a tile begins at a multiple of 16 tokens)
   const int64_t SD = k8 ? D + D / 2 : D / 2, SS = D / 16, row = SD + SS;
   const bool al16 = (((uintptr_t)kd | (uintptr_t)vd | (uintptr_t)strides[0] | (uintptr_t)strides[2]) & 15) == 0;
@@ -471,20 +544,36 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   int nc = kEvCluster;
   while (nc > 1 && (pairs * nc > 4 * sms || p.max_len < nc * 2048 || p.max_len <= 8192)) nc /= 2;
   cudaStream_t st = (cudaStream_t)stream;
-  int rc = launch_clusters(select_kernel, p, nc, KVH, B, nc, kSelThreads, 0, st);
+  int rc = p.max_len <= kSmall && pairs > 2 * sms ? record_cuda(launch_pdl(select_small_kernel, dim3((unsigned)((pairs + kMoveWarps - 1) / kMoveWarps)),
+                                                        dim3(kMoveThreads), 0, st, p))
+                               : launch_clusters(select_kernel, p, nc, KVH, B, nc, kSelThreads, 0, st);
   if (rc != HKV_OK) return rc;
-  const bool cluster = out_tables == block_tables || out_weights == weights;
+  const int T = D == 128 ? 16 : 8, warp_smem = k8 ? EvGeo<256, true>::WARP : D == 128 ? EvGeo<128, false>::WARP : EvGeo<256, false>::WARP;
+  const long long most = keep < p.max_len ? keep : p.max_len;
   void (*mk)(const EvictParams) = nullptr;
-  if (k8) mk = cluster ? move_kernel<256, true, true> : move_kernel<256, true, false>;
-  else if (D == 128) mk = cluster ? move_kernel<128, false, true> : move_kernel<128, false, false>;
-  else mk = cluster ? move_kernel<256, false, true> : move_kernel<256, false, false>;
-  const int smem = k8 ? EvGeo<256, true>::SMEM : D == 128 ? EvGeo<128, false>::SMEM : EvGeo<256, false>::SMEM;
+  if (out_tables == block_tables || out_weights == weights) {
+    // In place: a cluster per (request, kv head), no larger than a round's work and no more CTAs than fill the GPU (512 pairs to 2048
+    // tokens: 105 us with two CTAs a cluster, 112 with eight). A round waits for its slowest read, so few pairs with many rounds take
+    // as many warps as fit: 16 pairs to 16384 tokens at head_dim 256 167 -> 125 us (to other pages 65), to 7000 at 128 36 -> 31; two
+    // rounds gain nothing (2048 tokens: 18.9 -> 21.5).
+    int nm = kEvCluster;
+    while (nm > 1 && (nm / 2 * kMoveWarps * T >= most || pairs * nm > 4 * sms)) nm /= 2;
+    const bool wide = pairs * nm <= sms && most > 4 * nm * kMoveWarps * T;
+    if (k8) mk = wide ? move_kernel<256, true, true, 32> : move_kernel<256, true, true, kMoveWarps>;
+    else if (D == 128) mk = wide ? move_kernel<128, false, true, 32> : move_kernel<128, false, true, kMoveWarps>;
+    else mk = wide ? move_kernel<256, false, true, 32> : move_kernel<256, false, true, kMoveWarps>;
+    const int warps = wide ? 32 : kMoveWarps;
+    rc = record_cuda(cudaFuncSetAttribute((const void*)mk, cudaFuncAttributeMaxDynamicSharedMemorySize, warps * warp_smem));
+    return rc != HKV_OK ? rc : launch_clusters(mk, p, nm, KVH, B, nm, 32 * warps, (size_t)warps * warp_smem, st);
+  }
+  if (k8) mk = move_kernel<256, true, false, kMoveWarps>;
+  else mk = D == 128 ? move_kernel<128, false, false, kMoveWarps> : move_kernel<256, false, false, kMoveWarps>;
+  const int smem = kMoveWarps * warp_smem;
   rc = record_cuda(cudaFuncSetAttribute((const void*)mk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (rc != HKV_OK) return rc;
-  if (cluster) return launch_clusters(mk, p, kEvCluster, KVH, B, kEvCluster, kMoveThreads, smem, st);
   // one wave of four CTAs an SM, or as many as find work at once (64 requests, 8 kv heads, to 2048 tokens: 592 CTAs 112.6 us, 740 (in
   // 1.3 waves) 113, 5920 120; with the launch of an earlier step)
-  const long long most = keep < p.max_len ? keep : p.max_len, round = kMoveWarps * (D == 128 ? 16 : 8);
+  const long long round = kMoveWarps * T;
   const long long x = std::max(1ll, std::min((most + round - 1) / round, (4 * sms + pairs - 1) / pairs));
   return record_cuda(launch_pdl(mk, dim3((unsigned)x, (unsigned)KVH, (unsigned)B), dim3(kMoveThreads), smem, st, p));
 }
