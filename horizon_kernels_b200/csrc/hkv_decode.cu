@@ -1003,7 +1003,8 @@ struct DeviceInfo {
   int sms = 0;
   int ctas_per_sm[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};    // [D == 256][LAYOUT]
   int ctas_two_tiles[2] = {0, 0};                    // [D == 256] decode_kernel<D, 0, 2>: sixteen query rows per pass
-  int win_per_sm[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}}, win_two_tiles[2] = {0, 0};   // the same of window_kernel, at most as many
+  int win_per_sm[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};  // the same of window_kernel, at most as many
+  int win_two_tiles[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};                 // [D == 256][LAYOUT]: sixteen rows over more layouts
   std::atomic<bool> ready{false};                    // set (release) after the fields above, under g_setup_mutex
 };
 static DeviceInfo g_dev[64];
@@ -1024,6 +1025,16 @@ static cudaError_t setup_variant(int& ctas, int& win) {
   return cudaSuccess;
 }
 
+// window_kernel<D, LAYOUT, 2>, at most as many CTAs as the two-tile decode has (the workspace is sized by that)
+template <int D, int LAYOUT>
+static cudaError_t setup_window(int most, int& win) {
+  auto k = window_kernel<D, LAYOUT, 2>;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D, LAYOUT, 2>::TOTAL);
+  if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&win, k, NTHREADS, Smem<D, LAYOUT, 2>::TOTAL);
+  win = std::min(win, most);
+  return e;
+}
+
 static int device_info(DeviceInfo** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -1042,8 +1053,11 @@ static int device_info(DeviceInfo** out) {
       if ((e = setup_variant<256, 2>(di.ctas_per_sm[1][2], di.win_per_sm[1][2])) != cudaSuccess) return record_cuda(e);
       if ((e = setup_variant<128, 3>(di.ctas_per_sm[0][3], di.win_per_sm[0][3])) != cudaSuccess) return record_cuda(e);
       if ((e = setup_variant<256, 3>(di.ctas_per_sm[1][3], di.win_per_sm[1][3])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<128, 0, 2>(di.ctas_two_tiles[0], di.win_two_tiles[0])) != cudaSuccess) return record_cuda(e);
-      if ((e = setup_variant<256, 0, 2>(di.ctas_two_tiles[1], di.win_two_tiles[1])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<128, 0, 2>(di.ctas_two_tiles[0], di.win_two_tiles[0][0])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_variant<256, 0, 2>(di.ctas_two_tiles[1], di.win_two_tiles[1][0])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_window<128, 3>(di.ctas_two_tiles[0], di.win_two_tiles[0][3])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_window<256, 2>(di.ctas_two_tiles[1], di.win_two_tiles[1][2])) != cudaSuccess) return record_cuda(e);
+      if ((e = setup_window<256, 3>(di.ctas_two_tiles[1], di.win_two_tiles[1][3])) != cudaSuccess) return record_cuda(e);
       di.ready.store(true, std::memory_order_release);
     }
   }
@@ -1130,19 +1144,22 @@ static int decode_impl(const void* q, const void* kd, const void* ksf, const voi
   DeviceInfo* di;
   int rc = device_info(&di);
   if (rc != HKV_OK) return rc;
-  // head-major slot pages, more than 8 query rows per kv head: the two-tile kernel serves 16 rows per pass
+  // head-major slot pages, more than 8 query rows per kv head: the two-tile kernel serves 16 rows per pass; over a window also
+  // positions-outermost pages (32 requests, 8 x 128, group 4 x 4 tokens: 98 us in two passes, 46 in one; 96, 2 x 256, group 8 x 2: 107
+  // and 74) and the slot with FP8 keys (the latter: 83 and 54)
   const int(&per_sm)[2][4] = win ? di->win_per_sm : di->ctas_per_sm;
-  const int(&two_tiles)[2] = win ? di->win_two_tiles : di->ctas_two_tiles;
-  bool two = layout == 0 && G * qlmax > RPAD && two_tiles[D == 256] > 0;
+  // (over a window the other slot layouts have it too)
+  const int two_tiles = win ? di->win_two_tiles[D == 256][layout] : layout == 0 ? di->ctas_two_tiles[D == 256] : 0;
+  bool two = G * qlmax > RPAD && two_tiles > 0;
   auto parts_of = [&](int cps) {
     long long n = std::min<long long>((long long)di->sms * cps, kMaxParts);
     if (splits > 0) n = std::min<long long>(n, (long long)B * KVH * splits);
     return n < 1 ? 1 : n;
   };
   // (at head_dim 256 its partials may not fit a workspace that is enough for eight rows per pass, e.g. the built-in one)
-  if (two && D == 256 && workspace_bytes < WorkspaceLayout((int)parts_of(two_tiles[1]), 2 * RPAD, D).total) two = false;
+  if (two && D == 256 && workspace_bytes < WorkspaceLayout((int)parts_of(two_tiles), 2 * RPAD, D).total) two = false;
   const int rows_per_pass = two ? 2 * RPAD : RPAD;
-  const int cps = two ? two_tiles[D == 256] : per_sm[D == 256][layout];
+  const int cps = two ? two_tiles : per_sm[D == 256][layout];
   if (cps < 1) return HKV_ERR_UNSUPPORTED;
   const long long n_parts = parts_of(cps);
   if (workspace_bytes < WorkspaceLayout((int)n_parts, rows_per_pass, D).total) return HKV_ERR_WORKSPACE;
@@ -1168,7 +1185,8 @@ static int decode_impl(const void* q, const void* kd, const void* ksf, const voi
   cudaStream_t st = (cudaStream_t)stream;
   const unsigned grid = (unsigned)n_parts;
   void (*k)(const DecodeParams) =
-      win ? (two ? (D == 128 ? window_kernel<128, 0, 2> : window_kernel<256, 0, 2>) :
+      win ? (two ? (D == 128 ? (layout == 0 ? window_kernel<128, 0, 2> : window_kernel<128, 3, 2>)
+                             : layout == 0 ? window_kernel<256, 0, 2> : layout == 2 ? window_kernel<256, 2, 2> : window_kernel<256, 3, 2>) :
              D == 128 ? (layout == 0 ? window_kernel<128, 0> : layout == 1 ? window_kernel<128, 1> : window_kernel<128, 3>)
                       : (layout == 0 ? window_kernel<256, 0> : layout == 1 ? window_kernel<256, 1>
                          : layout == 2 ? window_kernel<256, 2> : window_kernel<256, 3>)) :
@@ -1176,10 +1194,11 @@ static int decode_impl(const void* q, const void* kd, const void* ksf, const voi
       D == 128 ? (layout == 0 ? decode_kernel<128, 0> : layout == 1 ? decode_kernel<128, 1> : decode_kernel<128, 3>)
                : (layout == 0 ? decode_kernel<256, 0> : layout == 1 ? decode_kernel<256, 1>
                   : layout == 2 ? decode_kernel<256, 2> : decode_kernel<256, 3>);
-  const size_t smem_bytes = two ? (size_t)(D == 128 ? Smem<128, 0, 2>::TOTAL : Smem<256, 0, 2>::TOTAL) : D == 128 ? (size_t)Smem<128, 0>::TOTAL
+  const size_t smem_bytes = two ? (size_t)(D == 128 ? Smem<128, 0, 2>::TOTAL : layout == 2 ? Smem<256, 2, 2>::TOTAL : Smem<256, 0, 2>::TOTAL) : D == 128 ? (size_t)Smem<128, 0>::TOTAL
                                      : layout == 2 ? (size_t)Smem<256, 2>::TOTAL : (size_t)Smem<256, 0>::TOTAL;
   static_assert(Smem<128, 0>::TOTAL == Smem<128, 1>::TOTAL && Smem<256, 0>::TOTAL == Smem<256, 1>::TOTAL &&
-                Smem<128, 0>::TOTAL == Smem<128, 3>::TOTAL && Smem<256, 0>::TOTAL == Smem<256, 3>::TOTAL,
+                Smem<128, 0>::TOTAL == Smem<128, 3>::TOTAL && Smem<256, 0>::TOTAL == Smem<256, 3>::TOTAL &&
+                Smem<128, 0, 2>::TOTAL == Smem<128, 3, 2>::TOTAL && Smem<256, 0, 2>::TOTAL == Smem<256, 3, 2>::TOTAL,
                 "layouts share a size");
   // More query rows per kv head than a pass serves (large groups, several draft tokens) take several passes: every
   // pass is one launch over the cache (split sequences are merged inside it).

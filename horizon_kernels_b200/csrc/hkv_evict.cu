@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
   if (nc > 1) cluster_sync();                       // (the totals have been read)
 }
 
-// A tile of moves: 16 tokens (8 at head_dim 256) whose new places lie in one 16-token block of a page. A warp gathers their rows into shared memory,
-// piece by piece (PB bytes: 8 at head_dim 128, whose rows are 8-byte aligned, 16 at 256; a row is 8 pieces of codes, FP8 keys
+// A tile of moves: 16 tokens (8 at head_dim 256) whose new places lie in one 16-token block of a page. A warp gathers their rows
+// into shared memory, piece by piece (PB bytes: 8 at head_dim 128, whose rows are 8-byte aligned, 16 at 256; a row is 8 pieces of codes, FP8 keys
 // 16 before them, and one of scales), and writes the tile out: with one bulk copy a side where rows lie back to back in the
 // cache, else piece by piece. The rows hold no registers on their way, so that a warp has the next tile in flight while it
 // writes this one. 64 requests of 1.5k to 16k tokens cut to 2048, 8 kv heads x 128 (302 MB moved): 83 us with the rows in

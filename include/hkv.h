@@ -270,7 +270,7 @@ int hkv_selftest_prefill_timeout(const void* q, int q_f16, const void* kd, const
  *           -inf for a row that sees no key
  * A 16-token block (prefill: a token) that no row of a request sees is not read, and its page may be gone: the table entry may
  * be any number within int32's range, the page's contents anything.
- * The workspace is hkv_decode's; the scratch of the prefill has hkv_prefill_window_scratch_bytes(..) bytes (0: refused arguments),
+ * The decode serves sixteen query rows per kv head a pass over any slot pages, eight over regions. The workspace is hkv_decode's; the scratch of the prefill has hkv_prefill_window_scratch_bytes(..) bytes (0: refused arguments),
  * and `chunk` counts the tokens that some row sees.
  */
 int hkv_decode_window(const void* q, const void* kd, const void* ksf, const void* vd, const void* vsf,
