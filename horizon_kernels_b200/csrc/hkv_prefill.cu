@@ -40,6 +40,10 @@ constexpr int kPieceCost = 3;          // cost of starting and ending a piece, i
 // below the output's own rounding (1.7e-3 against 64 bits with and without). 6144 tokens, window 1024: 151.8 us with the exact
 // maximum, 149.4 with the lag; 2048 tokens over 30000 at head_dim 256, window 4096: 150.2 and 143. fp32 outputs keep the exact one.
 constexpr float kPfLag = 8.0f;
+// Over a window: how much larger, in key tiles, shares of undivided row tiles may be than divided ones, which cost a launch more. 2048
+// tokens over 3000, window 700: 61.7 us divided, 56.0 with 2 or 4, 55.6 with 7, 68.7 with 12; four prompts of 90 to 1500 tokens, window
+// 500: 72.6, 70.0 with 2, 74 to 75 with 4 and 7; 6144 tokens, window 1024: 148.0, 146.0 with 2, 147 with 7.
+constexpr int kMergeCost = 2;
 constexpr int kMinPiece = 2;           // no piece of a divided row tile is shorter, in key tiles
 constexpr int kStageBytes = 32768;
 constexpr int kStages = 5;
@@ -1187,13 +1191,13 @@ static int plan(PrefillParams& p, int n_cta, int* n_split) {
   }
   long long cap = (total + n_cta - 1) / n_cta;
   if (cap < kPieceCost + 4) cap = kPieceCost + 4;
-  for (;; cap += cap / 64 + 1) {
+  // fills shares of at most `cap` in order; without `divide` a row tile that does not fit goes to the next CTA whole
+  auto share = [&](bool divide) -> int {
     auto w = w0;
     int c = 0;
     *n_split = 0;
     int part_c1 = -1, part_slot1 = 0, pieces = 0;         // the divided row tile being cut; pieces of the current CTA
     long long room = cap;
-    bool fits = true;
     auto begin = [&]() { p.start[c] = PfStart{w.kt, w.rt, (short)w.h, (short)w.req}; room = cap; pieces = 0; };
     if (w.req < p.n_req) begin();
     while (w.req < p.n_req) {
@@ -1211,20 +1215,29 @@ static int plan(PrefillParams& p, int n_cta, int* n_split) {
       }
       long long u = room - kPieceCost;
       if (n - u < kMinPiece) u = n - kMinPiece;
-      if (u >= kMinPiece) {
+      if (divide && u >= kMinPiece) {
         if (part_c1 < 0) { part_c1 = c; part_slot1 = pieces == 0 ? 0 : 1; }
         w.step(p.req, p.tok, p.kt_lo, p.kt_hi, (int)u);
-      } else if (pieces == 0) {                           // (cannot happen: cap holds kPieceCost + 2 * kMinPiece)
-        fits = false;
-        break;
+      } else if (pieces == 0) {                           // (divided, it cannot happen: cap holds kPieceCost + 2 * kMinPiece)
+        return 0;
       }
-      if (++c >= n_cta) { fits = false; break; }
+      if (++c >= n_cta) return 0;
       begin();
     }
-    if (!fits) continue;
     p.start[c + 1] = PfStart{p.kt_lo, 0, 0, (short)p.n_req};
     return c + 1;
+  };
+  int used;
+  while ((used = share(true)) == 0) cap += cap / 64 + 1;
+  if (WIN && p.window > 0 && *n_split > 0) {
+    // row tiles over a window are short: whole ones spare the launch that joins their parts, if shares grow by less than it costs
+    cap += kMergeCost;
+    const int whole = share(false);
+    if (whole > 0) return whole;
+    cap -= kMergeCost;
+    used = share(true);
   }
+  return used;
 }
 
 static size_t a256(size_t x) { return align_up(x, 256); }
