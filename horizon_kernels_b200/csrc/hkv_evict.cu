@@ -540,9 +540,10 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   if (e != cudaSuccess) return record_cuda(e);
   // CTAs per (request, kv head) for the selection. A cluster divides the work of a long context but meets four times a pass: 8192
   // tokens of 8 heads take 13.4 us with one CTA each (both launches), 14.9 with four; 30000 tokens of 2 heads 31.8 with one, 20.3,
-  // 17.3 and 16.8 with two, four and eight. With more (request, kv head) pairs than SMs one CTA each: 512 pairs 107 us, two each 121.
+  // 17.3 and 16.8 with two, four and eight. No more CTAs than two an SM, which run at once: 128 pairs to 20000 tokens take 50.9 us with
+  // two each, 60.8 with four; 512 pairs 107 with one each, 121 with two.
   int nc = kEvCluster;
-  while (nc > 1 && (pairs * nc > 4 * sms || p.max_len < nc * 2048 || p.max_len <= 8192)) nc /= 2;
+  while (nc > 1 && (pairs * nc > 2 * sms || p.max_len < nc * 2048 || p.max_len <= 8192)) nc /= 2;
   cudaStream_t st = (cudaStream_t)stream;
   int rc = p.max_len <= kSmall && pairs > 2 * sms ? record_cuda(launch_pdl(select_small_kernel, dim3((unsigned)((pairs + kMoveWarps - 1) / kMoveWarps)),
                                                         dim3(kMoveThreads), 0, st, p))
@@ -571,9 +572,10 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   const int smem = kMoveWarps * warp_smem;
   rc = record_cuda(cudaFuncSetAttribute((const void*)mk, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (rc != HKV_OK) return rc;
-  // one wave of four CTAs an SM, or as many as find work at once (64 requests, 8 kv heads, to 2048 tokens: 592 CTAs 112.6 us, 740 (in
-  // 1.3 waves) 113, 5920 120; with the launch of an earlier step)
-  const long long round = kMoveWarps * T;
-  const long long x = std::max(1ll, std::min((most + round - 1) / round, (4 * sms + pairs - 1) / pairs));
+  // As many CTAs as run at once, four an SM, or as find work at once; rounded down, since a few behind the first wave cost as much as
+  // another wave (160 pairs to 20000 tokens: 592 / 160 up 70.4 us, down 59.9; 128 pairs 50.9, 44.4), but two a pair while there are
+  // fewer than four pairs an SM (512 pairs to 2048 tokens: one each 104.5, two 98.2).
+  const long long round = kMoveWarps * T, fit = std::max(4 * sms / pairs, std::min(2ll, (4 * sms + pairs - 1) / pairs));
+  const long long x = std::max(1ll, std::min((most + round - 1) / round, fit));
   return record_cuda(launch_pdl(mk, dim3((unsigned)x, (unsigned)KVH, (unsigned)B), dim3(kMoveThreads), smem, st, p));
 }
