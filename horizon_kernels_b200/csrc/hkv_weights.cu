@@ -531,6 +531,7 @@ __global__ void __launch_bounds__(kWtThreads, D == 128 ? (QT == 1 ? 4 : 3) : QT 
 // 29.3 so. What bounds it: of 45000 clocks 9000 locate, fetch and prepare, then a unit takes a warp 4400 with the tensor pipe two
 // thirds busy (mma.sync; 128 instructions a unit). Two CTAs an SM 29.8 us, three 29.3, four 30.6 (128 registers, spills); with the
 // blocks of channels rolled 30.1; queries prefetched before the pages are looked up 30.5; a sequence's cost at 5 to 8 units 29.4 to 30.
+// Passes of 16 rows gain little by it (the same with two tokens 22.9 -> 22.1, 300 requests to 300 tokens 12.7 -> 14.5) and keep theirs.
 constexpr int kWdCost = 3;           // what a sequence costs a CTA beyond its units, in units
 constexpr int kWdMin = 4;
 
