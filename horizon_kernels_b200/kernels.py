@@ -31,6 +31,12 @@ def _need_cuda(*ts):
             raise RuntimeError("hkv kernels need CUDA tensors: there is no CPU path")
 
 
+def _one_device(first, *ts):
+    """a kernel must not be given another device's pointer (None: an argument that is not there)"""
+    if any(t is not None and t.device != first.device for t in ts):
+        raise ValueError("tensors on more than one device")
+
+
 def num_sms(device=None) -> int:
     d = torch.cuda.current_device() if device is None else torch.device(device).index
     if d not in _SMS:
@@ -124,6 +130,7 @@ def write(key, value, flat, strides, PS, slot_mapping, gk, gv, search=True, sign
     _check_scales(gk, gv, key.shape[1])
     _need_cuda(key, value, slot_mapping, gk, gv, *flat)
     _check_signs(signs, key.shape[2])
+    _one_device(key, value, slot_mapping, gk, gv, signs, *flat)
     KVH, D = key.shape[1], key.shape[2]
     kd, ksf, vd, vsf = flat
     st = (C.c_int64 * 6)(*strides)
@@ -161,6 +168,7 @@ def _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gv, 
         raise ValueError("query heads must be a multiple of the kv heads")
     _need_cuda(query, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, *flat)
     _check_signs(signs, query.shape[2])
+    _one_device(query, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, signs, *flat)
     return KVH, HQ // KVH
 
 
@@ -207,6 +215,7 @@ def decode_ragged(query, flat, strides, PS, block_tables, seq_lens, query_start_
 
 def _dequant(flat, strides, PS, block_tables, MP, rows, cu, n_rows, start, n_tokens, out_k, out_v, k8):
     _need_cuda(block_tables, out_k, out_v, *flat)
+    _one_device(out_k, out_v, block_tables, rows, cu, *flat)
     if out_k.dtype not in (torch.bfloat16, torch.float16) or out_v.dtype != out_k.dtype:
         raise TypeError("out_k / out_v must both be bf16 or both fp16")
     if not out_k.is_contiguous() or not out_v.is_contiguous() or out_k.shape != out_v.shape:
@@ -278,6 +287,7 @@ def _check_prefill(query, flat, PS, block_tables, rows, KVH, out, signs, workspa
             raise ValueError(f"prefill row {(row, q0, q1, L)} of {B} requests and {NT} query tokens")
     _need_cuda(query, block_tables, out, *flat)
     _check_signs(signs, D)
+    _one_device(query, block_tables, out, signs, *flat)
     if workspace is not None:
         _need_cuda(workspace)
         if workspace.device != query.device or workspace.nbytes < WORKSPACE_HEADER_BYTES:
@@ -351,6 +361,7 @@ def decode_window(query, flat, strides, PS, block_tables, seq_lens, query_start_
     _check_window(window, sinks)
     KVH, G = _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, signs)
     _check_lse(lse, query.shape[0], query.shape[1])
+    _one_device(query, lse)
     (B, MP), D = block_tables.shape, query.shape[2]
     kd, ksf, vd, vsf = flat
     with torch.cuda.device(query.device):
@@ -381,6 +392,7 @@ def prefill_window(query, flat, strides, PS, block_tables, rows, qk_scale, out_s
     _check_prefill(query, flat, PS, block_tables, rows, KVH, out, signs, workspace)
     (B, MP), (NT, HQ, D) = block_tables.shape, query.shape
     _check_lse(lse, NT, HQ)
+    _one_device(query, lse)
     n = len(rows)
     host_rows = (C.c_int32 * (4 * n))(*[int(x) for r in rows for x in r])
     lib = _lib.load()
@@ -434,6 +446,7 @@ def accumulate_weights(query, flat, strides, PS, block_tables, seq_lens, query_s
     _check_weights(weights, B)
     if weights.shape[1] != KVH:
         raise ValueError("weights (requests, kv heads, positions)")
+    _one_device(query, lse, weights)
     if workspace is not None:
         _need_cuda(workspace)
         if workspace.device != query.device or workspace.nbytes < WORKSPACE_HEADER_BYTES:
@@ -493,8 +506,7 @@ def evict(flat, strides, PS, D, block_tables, seq_lens, weights, keep, sinks, re
         raise ValueError("out_weights (requests, kv heads, >= keep positions)")
     if keep > out_tables.shape[1] * PS:
         raise ValueError("keep is more than the new pages hold")
-    if any(t.device != weights.device for t in (block_tables, out_tables, seq_lens, out_lens, kept, out_weights, *flat)):
-        raise ValueError("tensors on more than one device")
+    _one_device(weights, block_tables, out_tables, seq_lens, out_lens, kept, out_weights, *flat)
     same = out_weights.data_ptr() == weights.data_ptr() and out_weights.stride() == weights.stride()
     (a0, a1), (b0, b1) = _extent(weights), _extent(out_weights)
     if not same and a0 < b1 and b0 < a1:
