@@ -10,6 +10,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "hkv_common.cuh"
@@ -40,7 +41,7 @@ struct WeightsParams {
   float* w;
   long long w_b, w_h;
   int* status;
-  int MP, B, KVH, G, qlmax, lps, row0, max_len, window, sinks;
+  int MP, B, KVH, G, qlmax, lps, row0, max_len, W, window, sinks;
   float scale_log2, rot_scale;
 };
 
@@ -74,9 +75,9 @@ __device__ __forceinline__ WtReq wt_req(const WeightsParams& p, int b) {
   ql = (ql < 0 || ql > p.qlmax || p.G * ql <= p.row0) ? 0 : ql;
   r.ql = ql;
   r.L = ql > 0 ? min(max(__ldg(p.seq_lens + b), 0), p.max_len) : 0;
-  const int all = (r.L + 31) >> 5;
+  const int all = (min(r.L, p.W) + 31) >> 5;        // (tokens behind the weights gather nothing)
   const int lo = p.window > 0 ? max(0, r.L - ql + p.row0 / p.G - p.window + 1) : 0;      // first token of the first row's window
-  const int su = (min(lo, p.sinks) + 31) >> 5, wu = lo >> 5;
+  const int su = min(all, (min(lo, p.sinks) + 31) >> 5), wu = min(all, lo >> 5);
   r.su = su;
   r.skip = max(0, wu - su);
   r.U = all - r.skip;
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kWtThreads, D == 128 ? (QT == 1 ? 4 : 3) : QT 
   auto look_up = [&]() {
     const int u = fw.u + (lane >> 1), t = (u + (u >= fw.r.su ? fw.r.skip : 0)) * UT + 16 * (lane & 1);
     const int lo_w = p.window > 0 ? max(0, fw.r.L - fw.r.ql + p.row0 / G - p.window + 1) : 0;
-    pg = u < fw.end && t < fw.r.L && (t + 16 > lo_w || t < p.sinks) ? __ldg(p.bt + (long long)fw.b * p.MP + (t >> p.lps)) : -1;
+    pg = u < fw.end && t < min(fw.r.L, p.W) && (t + 16 > lo_w || t < p.sinks) ? __ldg(p.bt + (long long)fw.b * p.MP + (t >> p.lps)) : -1;
     pg_first = fw.u;
     pg_end = min(fw.end, fw.u + 16);
   };
@@ -407,7 +408,7 @@ __global__ void __launch_bounds__(kWtThreads, D == 128 ? (QT == 1 ? 4 : 3) : QT 
       // this lane's token of the unit, whose weight it adds to: block c / 2, row r0 or r1
       const int mine = tok0 + 16 * (c >> 1) + (c & 1 ? r1 : r0);
       const bool masked = tok0 + UT > t_lo || (tok0 < w_hi && tok0 + UT > p.sinks);
-      const bool add = mine < L && (mine >= lo_w || mine < p.sinks);
+      const bool add = mine < min(L, p.W) && (mine >= lo_w || mine < p.sinks);
       float old = add ? wrow[mine] : 0.0f;
       if (!mbar_try_wait_u32(bar, c_par) && !mbar_wait_bounded_u32(bar, c_par)) {
         if (lane == 0) atomicExch(p.status, HKV_ERR_DEVICE_WAIT);
@@ -629,7 +630,7 @@ __global__ void __launch_bounds__(kWtThreads, LAYOUT == 2 ? 2 : 3) wide_weights_
     if (fu >= pg_end) {
       const int u = fu + W * (lane >> 1), t = (u + (u >= fw.r.su ? fw.r.skip : 0)) * UT + 16 * (lane & 1);
       const int lo_w = p.window > 0 ? max(0, fw.r.L - fw.r.ql + p.row0 / G - p.window + 1) : 0;
-      pg = u < fw.end && t < fw.r.L && (t + 16 > lo_w || t < p.sinks) ? __ldg(p.bt + (long long)fw.b * p.MP + (t >> p.lps)) : -1;
+      pg = u < fw.end && t < min(fw.r.L, p.W) && (t + 16 > lo_w || t < p.sinks) ? __ldg(p.bt + (long long)fw.b * p.MP + (t >> p.lps)) : -1;
       pg_first = fu;
       pg_end = fu + W * 16;
     }
@@ -714,7 +715,7 @@ __global__ void __launch_bounds__(kWtThreads, LAYOUT == 2 ? 2 : 3) wide_weights_
       // this lane's token of the unit, whose weight it adds to: block c / 2, row r0 or r1
       const int mine = tok0 + 16 * (c >> 1) + (c & 1 ? r1 : r0);
       const bool masked = tok0 + UT > t_lo || (tok0 < w_hi && tok0 + UT > p.sinks);
-      const bool add = mine < L && (mine >= lo_w || mine < p.sinks);
+      const bool add = mine < min(L, p.W) && (mine >= lo_w || mine < p.sinks);
       const float old = add ? wrow[mine] : 0.0f;
       if (!mbar_try_wait_u32(bar, c_par) && !mbar_wait_bounded_u32(bar, c_par)) {
         if (lane == 0) atomicExch(p.status, HKV_ERR_DEVICE_WAIT);
@@ -912,8 +913,8 @@ extern "C" int hkv_accumulate_weights(const void* q, const void* kd, const void*
   p.MP = MP; p.B = B; p.KVH = KVH; p.G = G; p.qlmax = qlmax;
   p.lps = 0;
   while ((1 << p.lps) < PS) ++p.lps;
-  const long long reach = (long long)MP * PS;
-  p.max_len = (int)(reach < W ? reach : W);               // (a length beyond the table or the weights is cut there)
+  p.max_len = (int)std::min((long long)MP * PS, 0x7fffff00ll);      // (a length beyond the table is cut there)
+  p.W = W;
   p.window = window >= p.max_len ? 0 : window;            // (everything is seen)
   p.sinks = sinks;
   if (p.window > (1 << 30)) return HKV_ERR_RANGE;

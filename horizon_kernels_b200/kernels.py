@@ -424,7 +424,7 @@ def accumulate_weights(query, flat, strides, PS, block_tables, seq_lens, query_s
                        window=0, sinks=0, signs=None, k8=False, workspace=None):
     """weights[b, h, j] += the sum over the query rows of request b and kv head h that see key j (masks as in decode_window) of
     exp(score - lse): the attention that the cached tokens get from this call's queries, which `evict` goes by. weights
-    (B, KVH, W) fp32 with a contiguous last dimension; a context is taken up to W, entries that no row sees stay. lse
+    (B, KVH, W) fp32 with a contiguous last dimension; tokens from W on gather nothing, entries that no row sees stay. lse
     (NT, HQ) fp32, as decode_window and prefill_window leave it for the same queries, masks and scales. Requests with no or more
     than qlmax query tokens are skipped; (HQ / KVH) * qlmax <= 64. The result does not depend on the order in which the GPU
     works. query .. query_start_loc, gk, signs, k8 as in decode_window; of the cache only the keys are read."""

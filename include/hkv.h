@@ -294,7 +294,8 @@ int hkv_prefill_window(const void* q, int q_f16, const void* kd, const void* ksf
  * is written by one thread in a fixed order: repeated calls give the same bits.
  *   q .. seq_lens, query_start_loc, signs, k8   as hkv_decode_window; requests with 0 or more than qlmax query tokens are skipped
  *   lse       fp32 (n_tokens, KVH * G) contiguous, natural logarithm, as hkv_decode_window and hkv_prefill_window leave it
- *   weights   fp32, entry (b, h, j) at b * w_b + h * w_h + j, W of them per (b, h): a context is taken up to min(MP * PS, W)
+ *   weights   fp32, entry (b, h, j) at b * w_b + h * w_h + j, W of them per (b, h): tokens from W on gather nothing, the query
+ *             tokens are the last ones of the whole context all the same (a context is taken up to MP * PS)
  *   workspace a decode workspace whose status word a wait that ran out would set, or NULL: the built-in one's
  * G * qlmax <= 64; a pass over the keys serves 8 query rows per kv head, or 16 when there are more than 8.
  */
