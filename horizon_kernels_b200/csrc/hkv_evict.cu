@@ -44,7 +44,7 @@ struct EvictParams {
   float* ow;
   long long w_b, w_h, ow_b, ow_h;                   // element strides of the weights
   int* kept;
-  int B, MP, OMP, lps, KVH, keep, sinks, recent, max_len, OW;
+  int B, MP, OMP, lps, KVH, keep, sinks, recent, max_len, W, OW;
   int bulk, split;                                  // a tile's new rows lie back to back and 16-byte aligned; codes apart from scales
 };
 
@@ -85,6 +85,9 @@ __device__ __forceinline__ int scan_warp(int v, int lane) {
   return v;
 }
 
+// The candidates are the tokens between the first and the last ones that have a weight: [sinks, this). Those without one are lighter
+// than all of them, so that where the candidates are no more than may stay, the first tokens from `sinks` on stay
+__device__ __forceinline__ int candidates_end(int L, int W, int sinks, int recent) { return min(L - recent, max(W, sinks)); }
 // fp32 -> unsigned integers of the same order; both zeros are one, every NaN lies above infinity
 __device__ __forceinline__ uint32_t weight_key(float w) {
   const uint32_t u = __float_as_uint(w);
@@ -93,10 +96,10 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// The tokens of a context of at most kSmall, by one warp: the threshold bit by bit, every bit a count over the lanes' registers, no
+// At most kSmall candidates, by one warp: the threshold bit by bit, every bit a count over the lanes' registers, no
 // barrier. Right for more (request, kv head) pairs than the CTAs of select_kernel fill SMs in one wave: 2048 pairs of 300 tokens, 100 stay,
 // 36 us against 80 (both launches), of 800 and 300 78 against 113; 512 of 300 19 against 22. A few pairs of 1000: 19 against 12.
-__device__ __forceinline__ void select_small(const float* w, int* kept, int lane, int L, int keep, int sinks, int recent) {
+__device__ __forceinline__ void select_small(const float* w, int W, int* kept, int lane, int L, int keep, int sinks, int recent) {
   const int n = min(L, keep);
   if (L <= keep) {
     for (int r = lane; r < keep; r += 32) kept[r] = r < n ? r : -1;
@@ -104,8 +107,11 @@ __device__ __forceinline__ void select_small(const float* w, int* kept, int lane
   }
   for (int i = lane; i < sinks; i += 32) kept[i] = i;
   for (int i = lane; i < recent; i += 32) kept[keep - recent + i] = L - recent + i;
-  const int cnt = L - sinks - recent, need = keep - sinks - recent, turns = (cnt + 31) >> 5;
-  if (need == 0) return;
+  const int cnt = candidates_end(L, W, sinks, recent) - sinks, need = keep - sinks - recent, turns = (cnt + 31) >> 5;
+  if (need >= cnt || need == 0) {
+    for (int i = lane; i < need; i += 32) kept[sinks + i] = sinks + i;
+    return;
+  }
   w += sinks;
   uint32_t key[kSelRegs];
 #pragma unroll
@@ -163,7 +169,7 @@ __global__ void __launch_bounds__(kMoveThreads) select_small_kernel(const EvictP
   if (b >= p.B) return;
   const int L = min(max(__ldg(p.seq_lens + b), 0), p.max_len);
   if (h == 0 && lane == 0) p.out_lens[b] = min(L, p.keep);
-  select_small(p.w + b * p.w_b + h * p.w_h, p.kept + (long long)pair * p.keep, lane, L, p.keep, p.sinks, p.recent);
+  select_small(p.w + b * p.w_b + h * p.w_h, p.W, p.kept + (long long)pair * p.keep, lane, L, p.keep, p.sinks, p.recent);
 }
 
 // A warp has a run of the CTA's tokens, 32 at a time, a lane one of them: the order of (warp, turn, lane) is that of the tokens.
@@ -190,8 +196,12 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
   }
   for (int i = t0; i < p.sinks; i += step) kept[i] = i;
   for (int i = t0; i < p.recent; i += step) kept[p.keep - p.recent + i] = L - p.recent + i;
-  const int mid = L - p.sinks - p.recent, need = p.keep - p.sinks - p.recent;        // candidates, of which so many stay
-  if (need == 0) return;
+  // candidates, of which so many stay
+  const int mid = candidates_end(L, p.W, p.sinks, p.recent) - p.sinks, need = p.keep - p.sinks - p.recent;
+  if (need >= mid || need == 0) {                   // (again the whole cluster)
+    for (int i = t0; i < need; i += step) kept[p.sinks + i] = p.sinks + i;
+    return;
+  }
   const int share = (mid + nc - 1) / nc, m0 = min(mid, cr * share), cnt = min(mid, m0 + share) - m0;
   const int turns = ((cnt + kSelWarps - 1) / kSelWarps + 31) >> 5;                   // of a warp
   const int i0 = wp * turns * 32 + lane, first = p.sinks + m0 + i0;                  // this lane's first token, of the CTA's and of all
@@ -410,7 +420,7 @@ __global__ void __launch_bounds__(32 * WARPS, 32 / WARPS) move_kernel(const Evic
           cp_async<PB>(tiles_a + buf * Gm::TILE + at(x, row, pc), base_of(row, pc) + places[buf * 2 * T + (scales ? T : 0) + i]);
       }
     }
-    if (j >= 0) weight = w[j];
+    if (j >= 0) weight = j < p.W ? w[j] : 0.0f;
     asm volatile("cp.async.commit_group;" ::: "memory");
     j = position(r + stride);
   };
@@ -531,8 +541,9 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   p.split = p.split && p.bulk;
   p.lps = 0;
   while ((1 << p.lps) < PS) ++p.lps;
-  const long long reach = (long long)MP * PS;
-  p.max_len = (int)(reach < W ? reach : W);               // (a length beyond the table or the weights is cut there)
+  p.max_len = (int)std::min((long long)MP * PS, 0x7fffff00ll);      // (a length beyond the table is cut there)
+  p.W = W;
+  const int widest = p.max_len < W ? p.max_len : W;       // tokens to select from
   const long long pairs = (long long)B * KVH;
   int dev = 0, sms = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -543,9 +554,9 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   // 17.3 and 16.8 with two, four and eight. No more CTAs than two an SM, which run at once: 128 pairs to 20000 tokens take 50.9 us with
   // two each, 60.8 with four; 512 pairs 107 with one each, 121 with two.
   int nc = kEvCluster;
-  while (nc > 1 && (pairs * nc > 2 * sms || p.max_len < nc * 2048 || p.max_len <= 8192)) nc /= 2;
+  while (nc > 1 && (pairs * nc > 2 * sms || widest < nc * 2048 || widest <= 8192)) nc /= 2;
   cudaStream_t st = (cudaStream_t)stream;
-  int rc = p.max_len <= kSmall && pairs > 2 * sms ? record_cuda(launch_pdl(select_small_kernel, dim3((unsigned)((pairs + kMoveWarps - 1) / kMoveWarps)),
+  int rc = widest <= kSmall && pairs > 2 * sms ? record_cuda(launch_pdl(select_small_kernel, dim3((unsigned)((pairs + kMoveWarps - 1) / kMoveWarps)),
                                                         dim3(kMoveThreads), 0, st, p))
                                : launch_clusters(select_kernel, p, nc, KVH, B, nc, kSelThreads, 0, st);
   if (rc != HKV_OK) return rc;

@@ -476,7 +476,8 @@ def evict(flat, strides, PS, D, block_tables, seq_lens, weights, keep, sinks, re
     then); otherwise the pages of a row must be read by nobody in the call, which is what pages shared between requests need.
     kept (B, KVH, keep) int32 takes the old positions of what stays, -1 from n on; out_lens (B,) int32, another tensor than
     seq_lens, the new lengths; out_weights (None: the weights themselves) the weights of what stays, and 0 from n to
-    min(L, its width) - 1. Slots from n on keep their bytes. A context is taken up to W."""
+    min(L, its width) - 1. Slots from n on keep their bytes. Tokens from W on have no weight and are
+    lighter than all that have one; out_weights takes 0 for them."""
     rc = (_lib._host or _lib.host()).evict(flat, strides, PS, D, block_tables, seq_lens, weights, keep, sinks, recent, kept, out_lens,
                                            out_tables, out_weights, k8)
     if rc is not None:

@@ -318,7 +318,8 @@ int hkv_accumulate_weights(const void* q, const void* kd, const void* ksf, const
  *               Either the weights themselves (the same address and strides) or memory that does not overlap them
  *   cache       any layout hkv_write accepts whose pointers and strides are multiples of 8 (head_dim 128) or 16 bytes; k8: the
  *               K8V4 slot, ksf unused but not NULL
- * A context is taken up to min(MP * PS, W). Slots from n on keep their bytes. keep <= OMP * PS, sinks + recent <= keep.
+ * A context is taken up to MP * PS. Its tokens from W on have no weight: they are lighter than all that have one, and
+ * out_weights takes 0 for them. Slots from n on keep their bytes. keep <= OMP * PS, sinks + recent <= keep.
  */
 int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t strides[6], int PS, const int32_t* block_tables, int MP,
               const int32_t* seq_lens, int B, int KVH, int D, int k8, const float* weights, int64_t w_b, int64_t w_h, int W,
