@@ -33,13 +33,6 @@ constexpr int kPfReqs = 32;            // requests per launch (the tables below 
 constexpr int kPfCtas = 160;           // CTAs per launch
 constexpr int kKeys = 128;             // keys per tile
 constexpr int kPieceCost = 3;          // cost of starting and ending a piece, in key tiles (of about 1 us)
-// Over a window a row tile has ten tiles where a prompt has two hundred, and the maximum of a warp's 32 rows moves at nearly every
-// one of the first ten: the output's rescaling, between one value product and the next, is what a tile waits for. With 16-bit
-// outputs the maximum therefore lags by up to 2^8, as in the decode kernel: probabilities stay within f16's range at its 2^-11 of
-// each, and what is lost against a largest probability of exactly 1, about 2e-4 of the output (2-norm), lies a factor of eight
-// below the output's own rounding (1.7e-3 against 64 bits with and without). 6144 tokens, window 1024: 151.8 us with the exact
-// maximum, 149.4 with the lag; 2048 tokens over 30000 at head_dim 256, window 4096: 150.2 and 143. fp32 outputs keep the exact one.
-constexpr float kPfLag = 8.0f;
 // Over a window: how much larger, in key tiles, shares of undivided row tiles may be than divided ones, which cost a launch more. 2048
 // tokens over 3000, window 700: 61.7 us divided, 56.0 with 2 or 4, 55.6 with 7, 68.7 with 12; four prompts of 90 to 1500 tokens, window
 // 500: 72.6, 70.0 with 2, 74 to 75 with 4 and 7; 6144 tokens, window 1024: 148.0, 146.0 with 2, 147 with 7.
@@ -89,7 +82,6 @@ struct PrefillParams {
   int first_chunk;
   int window, sinks;                   // WIN: a token at position x sees the keys j <= x with j > x - window or j < sinks (window 0: all)
   float* lse;                          // the rows' log-sum-exps, or null
-  float lag;                           // WIN: the running maximum moves when a score exceeds it by more (log2 domain)
   PfReq req[kPfReqs];
   PfStart start[kPfCtas + 1];
   PfSplit split[kPfCtas];
@@ -506,7 +498,8 @@ __device__ __forceinline__ void store_out(const PrefillParams& p, long long elem
 // largest probability is any number: the error against 64 bits (before the output's own rounding) was 1.9e-4 where this has
 // 6.5e-5 (a prompt of 6144 tokens, head_dim 128) and 2.0e-4 where this has 8.3e-5 (2048 tokens over 30000, head_dim 256);
 // the torch path before had 8.0e-5 and 1.06e-4. With the lag the steps took 361 and 862 us, now 372 and 915; with the rescaling
-// before the exponentials 1.6 and 1.3 times as long.
+// before the exponentials 1.6 and 1.3 times as long. The same over a window, whose row tiles move the maximum at nearly every tile (a lag of
+// up to 2^8: 6144 tokens, window 1024, 153.0 us, exact 155.0; 2048 tokens over 30000 at head_dim 256, window 4096, 153.6 and 158.8).
 // A walk over the CTA's key tiles, piece by piece. A step to the next row tile of a request costs a few instructions: every
 // role takes it at every piece, two of them in a single thread.
 template <bool WIN>
@@ -1009,7 +1002,7 @@ __global__ void __launch_bounds__(PfShape<D>::THREADS, 1) attend_kernel(const __
         if (g > 0) ok = all_wait(word_before, (g - 1) / SETS);
         if (!ok) break;
         const float m_old = m, m_in = head ? -INFINITY : *top_now;
-        const bool move = top > (WIN ? m_in + p.lag : m_in);
+        const bool move = top > m_in;
         m = move ? (top == INFINITY ? 0.0f : top) : m_in;
         if (move || head) *top_now = m;
         mbar_arrive_u32(my_word);
@@ -1252,6 +1245,12 @@ struct PfWindow {
   int window = 0, sinks = 0;
   float* lse = nullptr;
 };
+// 0 where every context lies within the window: the same result, and cut among the CTAs as without one
+static int window_of(const int32_t* rows, int n_rows, int window) {
+  for (int i = 0; rows && i < n_rows; ++i)
+    if (rows[4 * i + 3] > window) return window;
+  return 0;
+}
 static int key_tiles(const int32_t* row, const PfWindow& w) {
   const PfReq r{row[1], row[2] - row[1], row[3], 0};
   return (r.L + kKeys - 1) / kKeys - pf_keys(r, w.window, w.sinks).skip;
@@ -1336,7 +1335,7 @@ extern "C" size_t hkv_prefill_window_scratch_bytes(const int32_t* rows, int n_ro
   using namespace hkv;
   if (n_rows < 1 || window < 0 || sinks < 0 || check_rows(rows, n_rows, n_tokens, KVH, G, D) != HKV_OK) return 0;
   PfWindow w;
-  w.window = window > 0x3fffff00 ? 0 : window;
+  w.window = window_of(rows, n_rows, window);
   w.sinks = sinks;
   return prefill_scratch(rows, n_rows, n_tokens, KVH, G, D, chunk_tiles_of(chunk), rotated, w).total;
 }
@@ -1385,7 +1384,6 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
   p.window = win.window;
   p.sinks = win.sinks;
   p.lse = win.lse;
-  p.lag = win.window > 0 && !out_f32 ? kPfLag : 0.0f;
   p.out = out;
   p.out_f32 = out_f32;
   p.k_bf16 = !q_f16;                                      // (the cached values are exact in both types)
@@ -1488,7 +1486,7 @@ extern "C" int hkv_prefill_window(const void* q, int q_f16, const void* kd, cons
   if (window < 0 || sinks < 0) return HKV_ERR_RANGE;
   if ((uintptr_t)lse & 3) return HKV_ERR_ALIGN;
   hkv::PfWindow w;
-  w.window = window > 0x3fffff00 ? 0 : window;            // (no context is longer)
+  w.window = hkv::window_of(rows, n_rows, window);
   w.sinks = sinks;
   w.lse = lse;
   return prefill_impl<true>(q, q_f16, kd, ksf, vd, vsf, strides, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D,
