@@ -515,12 +515,20 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   if (B > kMaxBatch) return HKV_ERR_RANGE;
   if (keep < 1 || sinks < 0 || recent < 0 || (int64_t)sinks + recent > keep) return HKV_ERR_RANGE;
   if ((int64_t)keep > (int64_t)OMP * PS || keep > OW) return HKV_ERR_RANGE;      // the new pages, the new weights
-  if (seq_lens == out_lens) return HKV_ERR_UNSUPPORTED;   // other heads read the old length while the new one is written
+  auto apart = [](uintptr_t x, int64_t nx, uintptr_t y, int64_t ny) {      // of so many 4-byte numbers each
+    return x + 4 * (uintptr_t)nx <= y || y + 4 * (uintptr_t)ny <= x;
+  };
+  // other heads read the old length while the new one is written
+  if (!apart((uintptr_t)seq_lens, B, (uintptr_t)out_lens, B)) return HKV_ERR_UNSUPPORTED;
   const uintptr_t a = (uintptr_t)kd | (uintptr_t)vd | (uintptr_t)vsf | (k8 ? 0 : (uintptr_t)ksf) | (uintptr_t)strides[0] |
                       (uintptr_t)strides[1] | (uintptr_t)strides[2] | (uintptr_t)strides[3] | (uintptr_t)strides[4] |
                       (uintptr_t)strides[5];
   if (a & (D == 128 ? 7 : 15)) return HKV_ERR_ALIGN;
   if (((uintptr_t)weights | (uintptr_t)out_weights) & 3) return HKV_ERR_ALIGN;
+  // new weights where the old ones are read: only in place, rank by rank
+  const bool same = weights == out_weights && (B == 1 || w_b == ow_b) && (KVH == 1 || w_h == ow_h);
+  if (!same && !apart((uintptr_t)weights, (B - 1) * w_b + (KVH - 1) * w_h + W, (uintptr_t)out_weights, (B - 1) * ow_b + (KVH - 1) * ow_h + OW))
+    return HKV_ERR_UNSUPPORTED;
   EvictParams p;
   p.kd = (uint8_t*)kd; p.ksf = (uint8_t*)ksf; p.vd = (uint8_t*)vd; p.vsf = (uint8_t*)vsf;
   p.dsp = strides[0]; p.dst = strides[1]; p.dsh = strides[2];

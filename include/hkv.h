@@ -310,7 +310,7 @@ int hkv_accumulate_weights(const void* q, const void* kd, const void* ksf, const
  * and, of those between, the (keep - sinks - recent) heaviest (the lowest position first among equals; a NaN counts as more
  * than any number; the two zeros are equal), in their order. A request of at most `keep` tokens keeps all of them.
  *   kept        int32 (B, KVH, keep): the old positions of the tokens that stay, ascending; -1 from n on
- *   out_lens    int32 (B): n; not the array seq_lens
+ *   out_lens    int32 (B): n; memory that does not overlap seq_lens
  *   out_tables  int32 (B, OMP): the slots of token kept[b, h, r] (codes and scales of keys and values, byte for byte) are copied
  *               to position r of this row. A row holds either the request's own first pages (in place; no other row of the call
  *               may name them), or pages that the call reads from nowhere. May be block_tables itself.
