@@ -173,7 +173,8 @@ __global__ void __launch_bounds__(kMoveThreads) select_small_kernel(const EvictP
 }
 
 // A warp has a run of the CTA's tokens, 32 at a time, a lane one of them: the order of (warp, turn, lane) is that of the tokens.
-// The first kSelRegs turns stay in registers from pass to pass, further ones (contexts beyond 8 x 16384 tokens) are read again.
+// The first kSelRegs turns stay in registers from pass to pass, further ones (contexts of more than 16384 tokens
+// a CTA of the cluster) are read again, one by one.
 // What bounds it: the longest context's chain of phases. One CTA, 14400 tokens (clocks): 7000 for the loads, 13000 for the first
 // pass (shared-memory atomics; a weight's leading bits agree with several of its neighbours'), 1000 for each look at the bins, 1000
 // for the second pass, 5000 for counts and ranks. Loads behind a branch each took 23000. 256 threads (one wave of CTAs where 512 take
@@ -557,12 +558,14 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return record_cuda(e);
-  // CTAs per (request, kv head) for the selection. A cluster divides the work of a long context but meets four times a pass: 8192
-  // tokens of 8 heads take 13.4 us with one CTA each (both launches), 14.9 with four; 30000 tokens of 2 heads 31.8 with one, 20.3,
-  // 17.3 and 16.8 with two, four and eight. No more CTAs than two an SM, which run at once: 128 pairs to 20000 tokens take 50.9 us with
-  // two each, 60.8 with four; 512 pairs 107 with one each, 121 with two.
+  // CTAs per (request, kv head) for the selection. A cluster divides the work of a long context but meets four times a pass, and one
+  // CTA holds 16384 weights in registers. Both launches, one CTA and four (us): a request of 8 heads x 128, 8192 tokens 21.2 and 21.5,
+  // 10240 21.5 and 23.5, 12288 23.7 and 25.0, 14336 25.6 and 25.6, 16384 25.6 and 23.5, 24576 42 and 26; 8 requests of 2 x 256 23.5 and
+  // 25.6, 27.6 and 27.8, 29.7 and 29.7, 29.7 and 27.7, 32.6 and 31.7, 50 and 34. Two are slower than one as long as that one's registers
+  // do (16 requests of 8 x 128, 16384 tokens 68.6 and 70.7, 24576 105 and 95). No more CTAs than two an SM, which run at once: 128 pairs
+  // to 20000 tokens take 50.9 us with two each, 60.8 with four; 512 pairs 107 with one each, 121 with two.
   int nc = kEvCluster;
-  while (nc > 1 && (pairs * nc > 2 * sms || widest < nc * 2048 || widest <= 8192)) nc /= 2;
+  while (nc > 1 && (pairs * nc > 2 * sms || widest < nc * 2048 || widest <= (nc == 2 ? kSelThreads * kSelRegs : 12288))) nc /= 2;
   cudaStream_t st = (cudaStream_t)stream;
   int rc = widest <= kSmall && pairs > 2 * sms ? record_cuda(launch_pdl(select_small_kernel, dim3((unsigned)((pairs + kMoveWarps - 1) / kMoveWarps)),
                                                         dim3(kMoveThreads), 0, st, p))

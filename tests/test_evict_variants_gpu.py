@@ -28,3 +28,9 @@ def test_layouts_of_many_short_contexts(kind, KVH, D, PS, where):
 @pytest.mark.parametrize("how", ["plain", "special"])
 def test_long_in_place(kind, KVH, D, PS, how):
     call(kind, [9000, 5000, 4500], 4400, 4, 500, KVH, D, PS, how=how, where="own", seed=KVH)
+
+
+@pytest.mark.parametrize("longest", [12288, 12289, 16384, 16385, 16400])
+@pytest.mark.parametrize("how", ["plain", "near"])
+def test_lines_between_one_cta_and_several(longest, how):
+    call("hnd", [longest, longest - 1, 9000], 3000, 4, 100, 1, 128, 16, how=how, where="new", seed=longest)
