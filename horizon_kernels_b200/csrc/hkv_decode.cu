@@ -707,7 +707,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
       auto softmax = [&](const uint32_t st, const int blk, const int bb, float (&x)[QT][BB][4], uint32_t (&pb)[QT][BB][2]) {
         const int tbase = (WIN && blk >= cw.r.su ? blk + cw.r.skip : blk) * UT;
         const bool masked = WIN ? blk >= blk_mask || (blk < win_end && blk >= p.sinks >> LOG_UT) : blk >= blk_mask;
-        if (masked) {                                 // warp-uniform: only the last unit(s) of a sequence
+        if (masked) {                                 // warp-uniform: only the last unit(s) of a sequence (WIN: and those at the window's edges)
           // rows past the context hold arbitrary bytes: their scores become -inf below, and their value scales are
           // set to zero here, in shared memory, so that the value product needs no masking code
           if (bb == 0 && lane < UT && (tbase + lane >= L || (WIN && tbase + lane < window_from(p, L, ql) && tbase + lane >= p.sinks))) {

@@ -297,7 +297,7 @@ int hkv_prefill_window(const void* q, int q_f16, const void* kd, const void* ksf
  *   weights   fp32, entry (b, h, j) at b * w_b + h * w_h + j, W of them per (b, h): tokens from W on gather nothing, the query
  *             tokens are the last ones of the whole context all the same (a context is taken up to MP * PS)
  *   workspace a decode workspace whose status word a wait that ran out would set, or NULL: the built-in one's
- * G * qlmax <= 64; a pass over the keys serves 8 query rows per kv head, or 16 when there are more than 8.
+ * G * qlmax <= 64; a pass over the keys serves 8 query rows per kv head, 16 when there are more than 8, 32 when there are more than 16.
  */
 int hkv_accumulate_weights(const void* q, const void* kd, const void* ksf, const int64_t strides[6], int PS,
                            const int32_t* block_tables, int MP, const int32_t* seq_lens, const int32_t* query_start_loc, int B,
