@@ -31,6 +31,14 @@ constexpr long long kWaitCycles = 1ll << 32;   // bound of every device-side wai
 
 __host__ __device__ inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+// whether B x KVH rows of W numbers, s_b and s_h apart, do not overlap (either stride may be the larger one)
+inline bool rows_apart(int B, int KVH, int64_t W, int64_t s_b, int64_t s_h) {
+  auto within = [W](int n, int64_t s, int m, int64_t t) {      // rows of the n inside one of the m
+    return (n <= 1 || s >= W) && (m <= 1 || t >= (n - 1) * s + W);
+  };
+  return within(KVH, KVH > 1 ? s_h : 0, B, s_b) || within(B, B > 1 ? s_b : 0, KVH, s_h);
+}
+
 struct WorkspaceLayout {
   size_t ticket_off, lse_off, opart_off, total;
   __host__ __device__ WorkspaceLayout(int n_parts, int rpad, int D) {

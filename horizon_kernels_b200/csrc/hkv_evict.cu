@@ -526,6 +526,7 @@ extern "C" int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t
                       (uintptr_t)strides[5];
   if (a & (D == 128 ? 7 : 15)) return HKV_ERR_ALIGN;
   if (((uintptr_t)weights | (uintptr_t)out_weights) & 3) return HKV_ERR_ALIGN;
+  if (!rows_apart(B, KVH, OW, ow_b, ow_h)) return HKV_ERR_UNSUPPORTED;
   // new weights where the old ones are read: only in place, rank by rank
   const bool same = weights == out_weights && (B == 1 || w_b == ow_b) && (KVH == 1 || w_h == ow_h);
   if (!same && !apart((uintptr_t)weights, (B - 1) * w_b + (KVH - 1) * w_h + W, (uintptr_t)out_weights, (B - 1) * ow_b + (KVH - 1) * ow_h + OW))

@@ -119,7 +119,10 @@ bool window_of(PyObject* window, PyObject* sinks, PyObject* lse, int64_t NT, int
 bool weight_rows(const at::Tensor* t, int64_t B, int64_t KVH, int dev) {
   if (!t || !on(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 3 || t->size(0) != B || t->size(1) != KVH || t->size(2) > INT32_MAX)
     return false;
-  return (t->stride(2) == 1 || t->size(2) <= 1) && (t->stride(1) > 0 || KVH <= 1) && (t->stride(0) > 0 || B <= 1);
+  const int64_t W = t->size(2), sb = t->stride(0), sh = t->stride(1);
+  if (sb < 0 || sh < 0 || (t->stride(2) != 1 && W > 1)) return false;
+  return ((KVH <= 1 || (sh > 0 && sh >= W)) && (B <= 1 || (sb > 0 && sb >= (KVH - 1) * sh + W))) ||
+         ((B <= 1 || (sb > 0 && sb >= W)) && (KVH <= 1 || (sh > 0 && sh >= (B - 1) * sb + W)));
 }
 
 // The launches behind the checks. Cache parts and strides as in include/hkv.h.

@@ -898,6 +898,7 @@ extern "C" int hkv_accumulate_weights(const void* q, const void* kd, const void*
   if (((uintptr_t)q & 15) || (signs && ((uintptr_t)signs & 15)) || (((uintptr_t)lse | (uintptr_t)weights) & 3) ||
       ((uintptr_t)workspace & 255))
     return HKV_ERR_ALIGN;
+  if (!rows_apart(B, KVH, W, w_b, w_h)) return HKV_ERR_UNSUPPORTED;
   if (dsp < 0 || ssp < 0 || dst < 0 || dsp >= (1ll << 31) || ssp >= (1ll << 31) || dst >= (1ll << 31)) return HKV_ERR_RANGE;
   if (!workspace) {
     const int rc = noalloc_workspace(&workspace);

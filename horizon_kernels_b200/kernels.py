@@ -416,8 +416,12 @@ def _check_weights(weights, B, name="weights"):
         raise TypeError(f"{name} must be an fp32 tensor (requests, kv heads, positions)")
     if weights.stride(2) != 1 and weights.shape[2] > 1:
         raise ValueError(f"{name} needs a contiguous last dimension")
+    (n_b, n_h, W), (s_b, s_h, _) = weights.shape, weights.stride()
     if any(s <= 0 for s, n in zip(weights.stride(), weights.shape) if n > 1):
-        raise ValueError(f"{name} must not be broadcast")
+        raise ValueError(f"{name} must not be broadcast: their rows would overlap")
+    if n_b > 0 and n_h > 0 and not ((n_h == 1 or s_h >= W) and (n_b == 1 or s_b >= (n_h - 1) * s_h + W) or
+                                    (n_b == 1 or s_b >= W) and (n_h == 1 or s_h >= (n_b - 1) * s_b + W)):
+        raise ValueError(f"rows of {name} overlap")
 
 
 def accumulate_weights(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, gk, qlmax, lse, weights,

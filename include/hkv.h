@@ -296,6 +296,7 @@ int hkv_prefill_window(const void* q, int q_f16, const void* kd, const void* ksf
  *   lse       fp32 (n_tokens, KVH * G) contiguous, natural logarithm, as hkv_decode_window and hkv_prefill_window leave it
  *   weights   fp32, entry (b, h, j) at b * w_b + h * w_h + j, W of them per (b, h): tokens from W on gather nothing, the query
  *             tokens are the last ones of the whole context all the same (a context is taken up to MP * PS)
+ *             Rows must not overlap
  *   workspace a decode workspace whose status word a wait that ran out would set, or NULL: the built-in one's
  * G * qlmax <= 64; a pass over the keys serves 8 query rows per kv head, 16 when there are more than 8, 32 when there are more than 16.
  */
