@@ -341,8 +341,8 @@ __global__ void __launch_bounds__(kSelThreads, 2) select_kernel(const EvictParam
 // 16 before them, and one of scales), and writes the tile out: with one bulk copy a side where rows lie back to back in the
 // cache, else piece by piece. The rows hold no registers on their way, so that a warp has the next tile in flight while it
 // writes this one. 64 requests of 1.5k to 16k tokens cut to 2048, 8 kv heads x 128 (302 MB moved): 83 us with the rows in
-// registers and 8-byte stores, which the L1 and the address arithmetic bound; 67 now (profiled), for 350 MB of DRAM traffic: rows
-// of 72 bytes here and there cost whole 32-byte sectors. In one piece (nothing evicted) the launch moves the 302 MB in 54 us. Eight
+// registers and 8-byte stores, which the L1 and the address arithmetic bound; 67 to 72 now (profiled), for 363 MB of DRAM traffic:
+// rows of 72 bytes here and there cost whole 32-byte sectors. In one piece (nothing evicted) the launch moves the 302 MB in 54 us. Eight
 // tokens a tile at head_dim 256, where sixteen leave room for fewer warps: 71 -> 65 us (8 requests of 131072 to 16384, 2 x 256).
 template <int D, bool K8>
 struct EvGeo {

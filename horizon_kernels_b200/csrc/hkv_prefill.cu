@@ -33,9 +33,10 @@ constexpr int kPfReqs = 32;            // requests per launch (the tables below 
 constexpr int kPfCtas = 160;           // CTAs per launch
 constexpr int kKeys = 128;             // keys per tile
 constexpr int kPieceCost = 3;          // cost of starting and ending a piece, in key tiles (of about 1 us)
-// Over a window: how much larger, in key tiles, shares of undivided row tiles may be than divided ones, which cost a launch more. 2048
-// tokens over 3000, window 700: 61.7 us divided, 56.0 with 2 or 4, 55.6 with 7, 68.7 with 12; four prompts of 90 to 1500 tokens, window
-// 500: 72.6, 70.0 with 2, 74 to 75 with 4 and 7; 6144 tokens, window 1024: 148.0, 146.0 with 2, 147 with 7.
+// Over a window: how much larger, in key tiles, shares of undivided row tiles may be than divided ones, which cost a launch more. 6144
+// tokens, window 1024: 150.5 us divided, 148.0 with 2, 148.5 with 4, 149.7 with 7, 155.7 with 12; four prompts of 90 to 1500 tokens, window
+// 500: 71.4, 67.2, 69.3, 72.7, 78.2; 2048 tokens over 3000, window 700: 58.1, 58.0, 57.2, 57.1, 57.1; three of 300 to 1500 at head_dim 256,
+// window 500, which lose by it: 51.0, 53.9, 58.0, 58.4, 60.1.
 constexpr int kMergeCost = 2;
 constexpr int kMinPiece = 2;           // no piece of a divided row tile is shorter, in key tiles
 constexpr int kStageBytes = 32768;
