@@ -15,10 +15,18 @@ EXPORTS = ("hkv_version", "hkv_error_string", "hkv_last_cuda_error", "hkv_write"
            "hkv_decode_rot", "hkv_write_k8", "hkv_decode_k8", "hkv_dequant_k8",
            "hkv_prefill", "hkv_prefill_scratch_bytes",
            "hkv_decode_window", "hkv_prefill_window", "hkv_prefill_window_scratch_bytes", "hkv_accumulate_weights", "hkv_evict",
+           "hkv_write_rotary", "hkv_write_b8", "hkv_decode_b8", "hkv_prefill_b8",
            "hkv_selftest_wait_timeout", "hkv_selftest_prefill_timeout", "hkv_selftest_codec", "hkv_probe_issue_rates")
 
 _lib = None
 _host = None
+
+
+class Rotary(C.Structure):
+    """hkv_rotary"""
+    _fields_ = [("query", C.c_void_p), ("qs0", C.c_int64), ("qs1", C.c_int64), ("query_out", C.c_void_p), ("os0", C.c_int64),
+                ("os1", C.c_int64), ("n_tokens", C.c_int64), ("positions", C.c_void_p), ("table", C.c_void_p), ("rows", C.c_int64),
+                ("HQ", C.c_int), ("rot", C.c_int), ("table_bf16", C.c_int), ("interleaved", C.c_int)]
 
 
 class HkvError(RuntimeError):
@@ -92,6 +100,14 @@ def load():
         L.hkv_evict.restype = i32
         L.hkv_evict.argtypes = [vp, vp, vp, vp, C.POINTER(i64), i32, vp, i32, vp, i32, i32, i32, i32, vp, i64, i64, i32, i32, i32,
                                 i32, vp, i32, vp, vp, vp, i64, i64, i32, vp]
+        L.hkv_write_rotary.restype = L.hkv_write_b8.restype = L.hkv_decode_b8.restype = L.hkv_prefill_b8.restype = i32
+        L.hkv_write_rotary.argtypes = L.hkv_write.argtypes[:-1] + [vp, i32, C.POINTER(Rotary), vp]
+        L.hkv_write_b8.argtypes = [vp, vp, i64, i64, i64, i64, vp, vp, C.POINTER(i64), i32, vp, i64, vp, vp, i32, i32, i32,
+                                   C.POINTER(Rotary), vp]
+        L.hkv_decode_b8.argtypes = [vp, vp, vp, C.POINTER(i64), i32, vp, i32, vp, vp, i32, i32, i32, i32, i32, f32, f32, vp, vp, vp,
+                                    C.c_size_t, i32, i32, i32, i32, vp, vp, vp]
+        L.hkv_prefill_b8.argtypes = [vp, i32, vp, vp, C.POINTER(i64), i32, vp, i32, i32, C.POINTER(i32), i32, i32, i32, i32, i32, f32,
+                                     f32, i64, i32, i32, i32, vp, vp, C.c_size_t, vp, i32, vp, vp]
         L.hkv_selftest_wait_timeout.restype = i32
         L.hkv_selftest_wait_timeout.argtypes = [vp, i64, vp]
         L.hkv_selftest_codec.restype = i32
@@ -116,6 +132,7 @@ class _NoHost:
 
     decode = prefill = layer_write = layer_decode = write
     decode_window = prefill_window = accumulate_weights = evict = write
+    write_rotary = write_b8 = write_rotary_b8 = decode_b8 = prefill_b8 = write
 
 
 def load_host(path):
@@ -144,7 +161,8 @@ def host():
             h.bind(*[C.cast(f, C.c_void_p).value for f in (
                 L.hkv_write, L.hkv_write_rot, L.hkv_write_k8, L.hkv_decode, L.hkv_decode_rot, L.hkv_decode_k8,
                 L.hkv_prefill_scratch_bytes, L.hkv_prefill, L.hkv_decode_window, L.hkv_prefill_window_scratch_bytes,
-                L.hkv_prefill_window, L.hkv_accumulate_weights, L.hkv_evict)])
+                L.hkv_prefill_window, L.hkv_accumulate_weights, L.hkv_evict, L.hkv_write_rotary, L.hkv_write_b8, L.hkv_decode_b8,
+                L.hkv_prefill_b8)])
         except (ImportError, OSError, AttributeError, TypeError) as e:       # (TypeError: it binds another set of entry points)
             warnings.warn(f"{HOST_PATH} does not load, every call takes the slower Python path: {e} (rebuild it with "
                           "`python -m horizon_kernels_b200.build`)", RuntimeWarning, stacklevel=3)

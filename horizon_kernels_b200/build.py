@@ -14,7 +14,8 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "lib")
 LIB = os.path.join(OUT_DIR, "libhkv.so")
 HOST = os.path.join(OUT_DIR, "hkv_host.so")
-SOURCES = ["hkv_write.cu", "hkv_decode.cu", "hkv_dequant.cu", "hkv_prefill.cu", "hkv_weights.cu", "hkv_evict.cu", "hkv_probe.cu"]
+SOURCES = ["hkv_write.cu", "hkv_decode.cu", "hkv_dequant.cu", "hkv_prefill.cu", "hkv_weights.cu", "hkv_evict.cu", "hkv_probe.cu",
+           "hkv_write_b8.cu", "hkv_decode_b8.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17", "-Xcompiler", "-fPIC",
               "-shared", "-cudart", "static"]
 

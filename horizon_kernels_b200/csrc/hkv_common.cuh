@@ -200,6 +200,21 @@ __device__ __forceinline__ void e4m3x4_to_f16x2(uint32_t w, uint32_t& lo, uint32
       : "=r"(lo), "=r"(hi)
       : "r"(w));
 }
+// four int8 codes -> two f16x2 (bytes 0, 1 and bytes 2, 3): 1024 + (code + 128) is the f16 with the byte in its low bits
+__device__ __forceinline__ void s8x4_to_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  const __half2 bias = __half2half2(__ushort_as_half(0x6480));        // 1152
+  const uint32_t a = __byte_perm(w, 0x64646464u, 0x4140), b = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), bias), y = __hsub2(*reinterpret_cast<const __half2*>(&b), bias);
+  lo = *reinterpret_cast<const uint32_t*>(&x);
+  hi = *reinterpret_cast<const uint32_t*>(&y);
+}
+// four codes of the 8-bit cache -> two f16x2
+template <bool INT8>
+__device__ __forceinline__ void b8_to_f16x2(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if (INT8) s8x4_to_f16x2(w, lo, hi);
+  else e4m3x4_to_f16x2(w, lo, hi);
+}
 __device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));

@@ -59,10 +59,14 @@ constexpr int RPAD = 8;          // query rows per (request, kv head) of one pas
 //   LAYOUT 2  the K8V4 slot (head_dim 256; kv_fp4_ref.py:283-293): token rows of [D signed E4M3 key bytes | D/2 value
 //             codes | D/16 value scales], heads outermost: keys and values of 16 tokens are ONE bulk copy of
 //             16 * 400 bytes; the stage holds those rows as they are
+//   LAYOUT 4  the 8-bit cache, E4M3 codes: tiles of 16 token rows of D bytes and the tile's scale (include/hkv.h); keys and
+//             values of 16 tokens are a bulk copy of 16 * D + 16 bytes each
+//   LAYOUT 5  the same with int8 codes
 template <int D, int LAYOUT>
 struct Geo {
-  static constexpr int SD = D / 2, SS = D / 16, SLOT = SD + SS;
-  static constexpr int UB = (D == 128 || LAYOUT != 2) ? 2 : 1;   // 16-token blocks per unit (1 for the K8V4 slot)
+  static constexpr bool B8 = LAYOUT >= 4;
+  static constexpr int SD = D / 2, SS = D / 16, SLOT = B8 ? D + 1 : SD + SS;
+  static constexpr int UB = B8 ? 1 : (D == 128 || LAYOUT != 2) ? 2 : 1;   // 16-token blocks per unit (1 for the K8V4 slot and the 8-bit cache)
   static constexpr int UT = 16 * UB, LOG_UT = UB == 2 ? 5 : 4;
   static constexpr int NS = D == 128 ? 3 : LAYOUT == 2 ? 3 : 2;   // stages per warp
   static constexpr int MINB = D == 128 ? 3 : 2;        // CTAs per SM the register budget is sized for
@@ -72,8 +76,8 @@ struct Geo {
   static constexpr int STAGE = K8 ? UT * SLOT8 : 2 * TILE;
   static constexpr bool SLOTROWS = LAYOUT == 0 || LAYOUT == 3;        // rows of [codes | scales] in shared memory
   static constexpr bool ROWCOPY = LAYOUT == 3;                         // fetched row by row with cp.async
-  static constexpr int ROW = K8 ? SLOT8 : SLOTROWS ? SLOT : SD;      // byte stride between token rows in shared memory
-  static constexpr int SD_ROW = ROW;                   // .. and between the rows of one head in the cache
+  static constexpr int ROW = B8 ? D : K8 ? SLOT8 : SLOTROWS ? SLOT : SD;      // byte stride between token rows in shared memory
+  static constexpr int SD_ROW = B8 ? SLOT : ROW;       // .. and between the rows of one head in the cache (B8: on average)
   static constexpr int KB = K8 ? 16 : 8;               // bytes of one 16-channel key block
   static constexpr int V_BASE = K8 ? D : TILE;         // first value byte of the stage (of row 0)
   static constexpr int SF_BASE = LAYOUT == 1 ? UT * SD : SD;        // value / key scales behind their side's codes
@@ -95,7 +99,8 @@ struct Geo {
   }
   // 16-channel block of a key row held by lane column c as its u-th block: NBL adjacent blocks per lane, so that
   // their scale bytes come with one load
-  __device__ static constexpr int kblk(int c, int u) { return NBL * c + u; }
+  // (B8: so that the 16-byte chunks of a quarter of a warp, two tokens and four lane columns, lie in different banks)
+  __device__ static constexpr int kblk(int c, int u) { return B8 ? 2 * c + (u & 1) + 8 * (u >> 1) : NBL * c + u; }
 };
 
 // QT: 8-row query tiles of one pass (1, or 2: sixteen query rows per kv head read the cache once). At head_dim 256 the two
@@ -290,6 +295,12 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
   const int t00 = Gm::tok(2 * c);
   uint32_t koff_d = r0 * Gm::ROW + Gm::KB * Gm::kblk(c, 0), koff_s = Gm::SF_BASE + r0 * Gm::SF_ROW + Gm::kblk(c, 0);
   uint32_t voff_d = Gm::V_BASE + t00 * Gm::ROW + 8 * g, voff_s = Gm::V_BASE + Gm::SF_BASE + t00 * Gm::SF_ROW + g;
+  if constexpr (Gm::B8) {                           // chunk j of token t lies at chunk j ^ (t % 8): the even and the odd chunks of
+    koff_d = g * D + ((2 * c ^ g) << 4);            // rows g and g + 8; chunk g of tokens 2c and 2c + 1 (and eight rows further)
+    koff_s = koff_d ^ 16;
+    voff_d = Gm::V_BASE + 2 * c * D + ((g ^ (2 * c)) << 4);
+    voff_s = Gm::V_BASE + (2 * c + 1) * D + ((g ^ (2 * c + 1)) << 4);
+  }
   asm volatile("" : "+r"(ring_a), "+r"(bars_a), "+r"(koff_d), "+r"(koff_s), "+r"(voff_d), "+r"(voff_s));
   constexpr int KR1 = Gm::tok(8) - Gm::tok(0);                            // r1 - r0 (the same for every g)
   constexpr int VR01 = Gm::tok(1) - Gm::tok(0), VR10 = Gm::tok(8) - Gm::tok(0),
@@ -392,7 +403,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
             const unsigned long long doff = (unsigned long long)(unsigned)page[bi] * p.dsp + pos0 * (unsigned)Gm::SD_ROW;
             if (LAYOUT == 2) {
               bulk_g2s_u32(st + bi * (16 * Gm::SLOT8), f_k + doff, 16 * Gm::SLOT8, bar);
-            } else if (LAYOUT == 0) {
+            } else if (LAYOUT == 0 || Gm::B8) {
               bulk_g2s_u32(st + bi * (16 * Gm::SLOT), f_k + doff, 16 * Gm::SLOT, bar);
               bulk_g2s_u32(st + bi * (16 * Gm::SLOT) + Gm::TILE, f_v + doff, 16 * Gm::SLOT, bar);
             } else {
@@ -511,7 +522,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
           qf[16 * u + 2 * i + 1] = __uint_as_float(ws[i] & 0xffff0000u);
         }
       }
-      if (p.signs != nullptr) {
+      if (!Gm::B8 && p.signs != nullptr) {
         // keys were written rotated: q' = bf16(FWHT(q * signs) * head_dim^-0.5), the reference's rotate_q
         // (kv_fp4_ref.py:90-92), fp32 butterflies in its stage order. The four lanes of a quad hold one row.
         const float4* sg = reinterpret_cast<const float4*>(p.signs + NQ * c);
@@ -567,7 +578,8 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
     }
 
     if (blk_first < blk_end && !dead) {
-      const float sc = fmaxf(fabsf(sc_signed), 1e-30f);
+      // (B8: the scores are multiplied by it with their block's scale, and are in log2 units from there on)
+      const float sc_abs = fmaxf(fabsf(sc_signed), 1e-30f), sc = Gm::B8 ? 1.0f : sc_abs;
       const float tau_raw = TAU / sc;
       uint32_t qa[Sm::QSM ? 1 : QT][Gm::KS][2];
       if constexpr (!Sm::QSM) {
@@ -625,6 +637,28 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
           for (int q = 0; q < QT; ++q)
 #pragma unroll
             for (int i = 0; i < Gm::NCH; ++i) sa[q][i][0] = sa[q][i][1] = sa[q][i][2] = sa[q][i][3] = 0.0f;
+          if constexpr (Gm::B8) {
+            const int tk = (bb + bi) * 16 * Gm::SLOT;
+#pragma unroll
+            for (int u = 0; u < Gm::NBL; ++u) {
+              const uint32_t ka = st + (u & 1 ? koff_s : koff_d) + tk + 128 * (u >> 1);
+              const uint4 a = lds128(ka), b = lds128(ka + 8 * D);
+              const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {           // k-step v of the chunk: channels 4v .. 4v+3 of rows r0, r1
+                uint32_t A[4];
+                b8_to_f16x2<LAYOUT == 5>(wa[v], A[0], A[2]);
+                b8_to_f16x2<LAYOUT == 5>(wb[v], A[1], A[3]);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) score_mma(sa[q][v & (Gm::NCH - 1)], A, q, 4 * u + v);
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[q][bi][i] = Gm::NCH == 2 ? sa[q][0][i] + sa[q][Gm::NCH - 1][i] : sa[q][0][i];
+            continue;
+          }
           if (Gm::K8) {
             // FP8 keys: 16 bytes per block and row, no block scale (the global scale is part of `sc`)
             const int dk8 = bi * 16 * Gm::ROW;
@@ -706,14 +740,32 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
       // operand of the second product in pb.
       auto softmax = [&](const uint32_t st, const int blk, const int bb, float (&x)[QT][BB][4], uint32_t (&pb)[QT][BB][2]) {
         const int tbase = (WIN && blk >= cw.r.su ? blk + cw.r.skip : blk) * UT;
+        // B8: a score takes its block's key scale, and in log2 units the exponent of its block's value scale. A probability is then
+        // relative to the largest product of a weight and a value scale, and the value product needs no scales; the sum of the
+        // weights takes the value scale out again (a power of two: exact).
+        float lw[BB];
+        if constexpr (Gm::B8) {
+#pragma unroll
+          for (int bi = 0; bi < BB; ++bi) {
+            const uint32_t ta = st + (bb + bi) * 16 * Gm::SLOT + 16 * D;
+            const uint32_t ks = lds32(ta) & 0x7f800000u, vs = lds32(ta + Gm::V_BASE) & 0x7f800000u;
+            const float f = sc_abs * __uint_as_float(ks), ev = (float)((int)(vs >> 23) - 127);
+            lw[bi] = __uint_as_float(0x7f000000u - vs);
+#pragma unroll
+            for (int q = 0; q < QT; ++q)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) x[q][bi][i] = fmaf(x[q][bi][i], f, ev);
+          }
+        }
         const bool masked = WIN ? blk >= blk_mask || (blk < win_end && blk >= p.sinks >> LOG_UT) : blk >= blk_mask;
         if (masked) {                                 // warp-uniform: only the last unit(s) of a sequence (WIN: and those at the window's edges)
           // rows past the context hold arbitrary bytes: their scores become -inf below, and their value scales are
           // set to zero here, in shared memory, so that the value product needs no masking code
-          if (bb == 0 && lane < UT && (tbase + lane >= L || (WIN && tbase + lane < window_from(p, L, ql) && tbase + lane >= p.sinks))) {
-            const uint32_t a = st + Gm::V_BASE + Gm::SF_BASE + lane * Gm::SF_ROW;
+          // (B8: the value codes themselves, since an E4M3 code may be a NaN; any int8 code times a weight of zero is zero)
+          if (LAYOUT != 5 && bb == 0 && lane < UT && (tbase + lane >= L || (WIN && tbase + lane < window_from(p, L, ql) && tbase + lane >= p.sinks))) {
+            const uint32_t a = st + Gm::V_BASE + (Gm::B8 ? (lane >> 4) * 16 * Gm::SLOT + (lane & 15) * D : Gm::SF_BASE + lane * Gm::SF_ROW);
 #pragma unroll
-            for (int i = 0; i < Gm::SS; i += 8) sts64_zero(a + i);
+            for (int i = 0; i < (Gm::B8 ? D : Gm::SS); i += 8) sts64_zero(a + i);
             fence_proxy_async();                      // the stage's next bulk copy overwrites these bytes
           }
           __syncwarp();
@@ -773,8 +825,13 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
           for (int bi = 0; bi < BB; ++bi) {
             const float p00 = fast_exp2(fmaf(x[q][bi][0], sc, mneg0[q])), p01 = fast_exp2(fmaf(x[q][bi][1], sc, mneg1[q])),
                         p10 = fast_exp2(fmaf(x[q][bi][2], sc, mneg0[q])), p11 = fast_exp2(fmaf(x[q][bi][3], sc, mneg1[q]));
-            l0[q] += p00 + p10;
-            l1[q] += p01 + p11;
+            if constexpr (Gm::B8) {
+              l0[q] = fmaf(p00 + p10, lw[bi], l0[q]);
+              l1[q] = fmaf(p01 + p11, lw[bi], l1[q]);
+            } else {
+              l0[q] += p00 + p10;
+              l1[q] += p01 + p11;
+            }
             // transpose the two 8x8 (token, row) tiles
             pb[q][bi][0] = movmatrix_trans(pack_f16x2(p00, p01));
             pb[q][bi][1] = movmatrix_trans(pack_f16x2(p10, p11));
@@ -788,6 +845,22 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
         for (int bi = 0; bi < BB; ++bi) {
 #pragma unroll
           for (int hf = 0; hf < Gm::NH; ++hf) {
+            if constexpr (Gm::B8) {
+              const uint32_t va = st + voff_d + (bb + bi) * 16 * Gm::SLOT + 128 * hf, vb = st + voff_s + (bb + bi) * 16 * Gm::SLOT + 128 * hf;
+              const uint4 a = lds128(va), b = lds128(vb), a8 = lds128(va + 8 * D), b8 = lds128(vb + 8 * D);   // tokens 2c, 2c + 1, .. + 8
+              const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w}, wc[4] = {a8.x, a8.y, a8.z, a8.w},
+                             wd[4] = {b8.x, b8.y, b8.z, b8.w};
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {           // channels 2i, 2i + 1 of the chunk: byte pairs over two tokens
+                const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
+                uint32_t A[4];
+                b8_to_f16x2<LAYOUT == 5>(__byte_perm(wa[i >> 1], wb[i >> 1], sel), A[0], A[1]);
+                b8_to_f16x2<LAYOUT == 5>(__byte_perm(wc[i >> 1], wd[i >> 1], sel), A[2], A[3]);
+#pragma unroll
+                for (int q = 0; q < QT; ++q) mma_f16(o[q][8 * hf + i], A[0], A[1], A[2], A[3], pb[q][bi][0], pb[q][bi][1]);
+              }
+              continue;
+            }
             const int dv = bi * 16 * Gm::ROW + 64 * hf, sv = bi * 16 * Gm::SF_ROW + 8 * hf;
             const uint2 v00 = lds64(vd_ + dv);
             const uint2 v01 = lds64(vd_ + dv + VR01 * Gm::ROW);
@@ -847,7 +920,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
 
     // ---------------- merge the TG warps' states of this piece and write it out
     {
-      const float sc = fmaxf(fabsf(sc_signed), 1e-30f);
+      const float sc = Gm::B8 ? 1.0f : fmaxf(fabsf(sc_signed), 1e-30f);
       constexpr int RM = RP / Sm::MP;                // rows of one merge pass
       float* ob = obuf + (size_t)w * RM * Sm::OROW;
       const float gvh = __ldg(p.gv + h);
@@ -996,9 +1069,11 @@ __global__ void __launch_bounds__(NTHREADS, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB) 
   decode_body<D, LAYOUT, QT, true>(p);
 }
 
-// ----------------------------------------------------------------------------------------------------- host side
 int record_cuda(cudaError_t e);
+int early_metadata();                              // HKV_OPT_EARLY_METADATA
 
+#ifndef HKV_DECODE_BODY_ONLY                       // (hkv_decode_b8.cu makes its kernels from the body above)
+// ----------------------------------------------------------------------------------------------------- host side
 struct DeviceInfo {
   int sms = 0;
   int ctas_per_sm[2][4] = {{0, 0, 0, 0}, {0, 0, 0, 0}};    // [D == 256][LAYOUT]
@@ -1010,6 +1085,7 @@ struct DeviceInfo {
 static DeviceInfo g_dev[64];
 static std::mutex g_setup_mutex;                     // serialises the once-per-device set-up of concurrent host threads
 static std::atomic<int> g_early_metadata{0};
+int early_metadata() { return g_early_metadata.load(std::memory_order_relaxed); }
 
 template <int D, int LAYOUT, int QT = 1>
 static cudaError_t setup_variant(int& ctas, int& win) {
@@ -1172,7 +1248,7 @@ static int decode_impl(const void* q, const void* kd, const void* ksf, const voi
   p.ws = (uint8_t*)workspace;
   p.out = (__nv_bfloat16*)out;
   p.MP = MP; p.B = B; p.KVH = KVH; p.G = G; p.qlmax = qlmax; p.PS = PS;
-  p.early_meta = g_early_metadata.load(std::memory_order_relaxed);
+  p.early_meta = early_metadata();
   p.max_len = (int)std::min<long long>((long long)MP * PS, 0x7fffffffll);
   if (signs && ((uintptr_t)signs & 15)) return HKV_ERR_ALIGN;
   p.signs = signs;
@@ -1382,3 +1458,6 @@ extern "C" int hkv_decode_noalloc_status(int* status, void* stream) {
   }
   return hkv_workspace_status(ws, status, stream);
 }
+#else
+}  // namespace hkv
+#endif  // HKV_DECODE_BODY_ONLY

@@ -1,5 +1,5 @@
-// Native side of kernels.write, kernels.decode_ragged, kernels.prefill, their window forms, kernels.accumulate_weights and
-// kernels.evict, and of the backend's cache update and decode: takes the callers' Python arguments as they are, checks them and calls the C ABI (include/hkv.h). What the wrappers do per call in
+// Native side of kernels.write, kernels.decode_ragged, kernels.prefill, their window forms, kernels.accumulate_weights,
+// kernels.evict, the writes with a rotation, the calls of the 8-bit cache, and of the backend's cache update and decode: takes the callers' Python arguments as they are, checks them and calls the C ABI (include/hkv.h). What the wrappers do per call in
 // Python (about forty attribute reads and checks, a device context, the conversion of 25 ctypes arguments) costs 20 to 25
 // microseconds, longer than a small decode step runs on the GPU; here it costs two.
 //
@@ -36,6 +36,10 @@ struct Abi {                       // entry points of the loaded libhkv.so, hand
   decltype(&hkv_prefill_window) prefill_window = nullptr;
   decltype(&hkv_accumulate_weights) accumulate_weights = nullptr;
   decltype(&hkv_evict) evict = nullptr;
+  decltype(&hkv_write_rotary) write_rotary = nullptr;
+  decltype(&hkv_write_b8) write_b8 = nullptr;
+  decltype(&hkv_decode_b8) decode_b8 = nullptr;
+  decltype(&hkv_prefill_b8) prefill_b8 = nullptr;
 } abi;
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
@@ -123,6 +127,54 @@ bool weight_rows(const at::Tensor* t, int64_t B, int64_t KVH, int dev) {
   if (sb < 0 || sh < 0 || (t->stride(2) != 1 && W > 1)) return false;
   return ((KVH <= 1 || (sh > 0 && sh >= W)) && (B <= 1 || (sb > 0 && sb >= (KVH - 1) * sh + W))) ||
          ((B <= 1 || (sb > 0 && sb >= W)) && (KVH <= 1 || (sh > 0 && sh >= (B - 1) * sb + W)));
+}
+
+// the 8-bit cache: key tiles and value tiles, strides (page, head)
+struct Tiles {
+  void *k, *v;
+  int64_t strides[2];
+};
+bool tiles_of(PyObject* flat, PyObject* strides, int dev, Tiles* c) {
+  if (!PyTuple_CheckExact(flat) || PyTuple_GET_SIZE(flat) != 2 || !PyTuple_CheckExact(strides) || PyTuple_GET_SIZE(strides) != 2) return false;
+  const at::Tensor *k = tensor(PyTuple_GET_ITEM(flat, 0)), *v = tensor(PyTuple_GET_ITEM(flat, 1));
+  if (!k || !v || !on(*k, dev) || !on(*v, dev)) return false;
+  c->k = k->data_ptr();
+  c->v = v->data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    long long s;
+    if (!integer(PyTuple_GET_ITEM(strides, i), &s)) return false;
+    c->strides[i] = s;
+  }
+  return true;
+}
+bool format_of(PyObject* o, int* fmt) {
+  if (!PyUnicode_CheckExact(o)) return false;
+  *fmt = PyUnicode_CompareWithASCIIString(o, "e4m3") == 0 ? HKV_B8_E4M3 : PyUnicode_CompareWithASCIIString(o, "int8") == 0 ? HKV_B8_INT8 : -1;
+  return *fmt >= 0;
+}
+// keys and values of a write, and their slots
+bool new_rows(const at::Tensor* k, const at::Tensor* v, const at::Tensor* slots, int dev) {
+  return k && v && slots && on(*k, dev) && on(*v, dev) && on(*slots, dev) && k->scalar_type() == at::kBFloat16 &&
+         v->scalar_type() == at::kBFloat16 && k->dim() == 3 && v->sizes() == k->sizes() && k->stride(2) == 1 && v->stride(2) == 1 &&
+         slots->scalar_type() == at::kLong && slots->dim() == 1 && slots->is_contiguous() && slots->size(0) <= k->size(0) &&
+         k->size(1) <= INT32_MAX && k->size(2) <= INT32_MAX;
+}
+// query, positions, table and where the turned queries go (the C call refuses rows that overlap)
+bool rotary_of(const at::Tensor* q, const at::Tensor* k, const at::Tensor* slots, PyObject* positions, PyObject* table, PyObject* out,
+               PyObject* interleaved, int dev, hkv_rotary* r) {
+  const at::Tensor *pos = tensor(positions), *t = tensor(table), *o = tensor(out);
+  bool pairs;
+  if (!q || !pos || !t || !o || !on(*q, dev) || !on(*pos, dev) || !on(*t, dev) || !on(*o, dev) || !boolean(interleaved, &pairs) ||
+      q->scalar_type() != at::kBFloat16 || o->scalar_type() != at::kBFloat16 || q->dim() != 3 || o->sizes() != q->sizes() ||
+      q->size(2) != k->size(2) || q->stride(2) != 1 || o->stride(2) != 1 || pos->scalar_type() != at::kLong || pos->dim() != 1 ||
+      !pos->is_contiguous() || pos->size(0) != q->size(0) || slots->size(0) > q->size(0) || t->dim() != 2 || !t->is_contiguous() ||
+      (t->scalar_type() != at::kFloat && t->scalar_type() != at::kBFloat16) || t->size(1) % 16 || t->size(1) < 16 ||
+      t->size(1) > k->size(2) || q->size(1) > INT32_MAX)
+    return false;
+  *r = hkv_rotary{q->data_ptr(), q->stride(0), q->stride(1), o->data_ptr(), o->stride(0), o->stride(1), q->size(0),
+                  static_cast<const int64_t*>(pos->data_ptr()), t->data_ptr(), t->size(0), (int)q->size(1), (int)t->size(1),
+                  t->scalar_type() == at::kBFloat16, pairs};
+  return true;
 }
 
 // The launches behind the checks. Cache parts and strides as in include/hkv.h.
@@ -263,6 +315,122 @@ PyObject* decode_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (WIN && !window_of(a[17], a[18], a[19], q->size(0), HQ, dev, &w)) Py_RETURN_NONE;
     return run_decode(q->data_ptr(), c, (int)PS, *bt, *lens, *qsl, HQ, D, s1, s2, *gk, *gv, (int)qlmax, out->data_ptr(), *ws, (int)splits, signs,
                       k8, dev, WIN ? &w : nullptr);
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// write_rotary(query, key, value, flat, strides, PS, slot_mapping, positions, cos_sin, gk, gv, query_out, interleaved, search, signs, k8)
+PyObject* write_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  try {
+    if (n != 16 || !abi.write_rotary) Py_RETURN_NONE;
+    const at::Tensor *q = tensor(a[0]), *k = tensor(a[1]), *v = tensor(a[2]), *slots = tensor(a[6]), *gk = tensor(a[9]), *gv = tensor(a[10]);
+    if (!k || !k->is_cuda()) Py_RETURN_NONE;
+    const int dev = k->device().index();
+    long long PS;
+    bool search, k8;
+    const float* signs;
+    Cache c;
+    hkv_rotary r;
+    if (dev != c10::cuda::current_device() || !new_rows(k, v, slots, dev) || !integer(a[5], &PS) || PS != (int)PS || !boolean(a[13], &search) ||
+        !boolean(a[15], &k8) || !scales(gk, gv, k->size(1), dev) || !sign_vector(a[14], k->size(2), dev, &signs) || (k8 && signs) ||
+        !cache_of(a[3], a[4], dev, &c) || !rotary_of(q, k, slots, a[7], a[8], a[11], a[12], dev, &r))
+      Py_RETURN_NONE;
+    const void *kp = k->data_ptr(), *vp = v->data_ptr();
+    const int64_t k0 = k->stride(0), k1 = k->stride(1), v0 = v->stride(0), v1 = v->stride(1), n_slots = slots->size(0);
+    const int64_t* sl = static_cast<const int64_t*>(slots->data_ptr());
+    const float *gkp = static_cast<const float*>(gk->data_ptr()), *gvp = static_cast<const float*>(gv->data_ptr());
+    const int KVH = (int)k->size(1), D = (int)k->size(2);
+    void* st = c10::cuda::getCurrentCUDAStream(dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = abi.write_rotary(kp, vp, k0, k1, v0, v1, c.part[0], c.part[1], c.part[2], c.part[3], c.strides, (int)PS, sl, n_slots, gkp, gvp,
+                          KVH, D, search, signs, k8, &r, st);
+    Py_END_ALLOW_THREADS
+    if (rc == HKV_ERR_RANGE) Py_RETURN_NONE;          // (the Python path says which rows overlap)
+    return PyLong_FromLong(rc);
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// write_b8(key, value, flat, strides, PS, slot_mapping, gk, gv, fmt)
+// write_rotary_b8(query, key, value, flat, strides, PS, slot_mapping, positions, cos_sin, gk, gv, query_out, interleaved, fmt)
+template <bool ROT>
+PyObject* write_b8_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  try {
+    if (n != (ROT ? 14 : 9) || !abi.write_b8) Py_RETURN_NONE;
+    PyObject* const* b = a + (ROT ? 1 : 0);            // key, value, flat, strides, PS, slot_mapping
+    PyObject* const* s = ROT ? a + 9 : a + 6;          // gk, gv
+    const at::Tensor *k = tensor(b[0]), *v = tensor(b[1]), *slots = tensor(b[5]), *gk = tensor(s[0]), *gv = tensor(s[1]);
+    if (!k || !k->is_cuda()) Py_RETURN_NONE;
+    const int dev = k->device().index();
+    long long PS;
+    int fmt;
+    Tiles c;
+    hkv_rotary r;
+    if (dev != c10::cuda::current_device() || !new_rows(k, v, slots, dev) || !integer(b[4], &PS) || PS != (int)PS ||
+        !format_of(a[n - 1], &fmt) || !scales(gk, gv, k->size(1), dev) || !tiles_of(b[2], b[3], dev, &c) ||
+        (ROT && !rotary_of(tensor(a[0]), k, slots, a[7], a[8], a[11], a[12], dev, &r)))
+      Py_RETURN_NONE;
+    const void *kp = k->data_ptr(), *vp = v->data_ptr();
+    const int64_t k0 = k->stride(0), k1 = k->stride(1), v0 = v->stride(0), v1 = v->stride(1), n_slots = slots->size(0);
+    const int64_t* sl = static_cast<const int64_t*>(slots->data_ptr());
+    const float *gkp = static_cast<const float*>(gk->data_ptr()), *gvp = static_cast<const float*>(gv->data_ptr());
+    const int KVH = (int)k->size(1), D = (int)k->size(2);
+    void* st = c10::cuda::getCurrentCUDAStream(dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = abi.write_b8(kp, vp, k0, k1, v0, v1, c.k, c.v, c.strides, (int)PS, sl, n_slots, gkp, gvp, KVH, D, fmt, ROT ? &r : nullptr, st);
+    Py_END_ALLOW_THREADS
+    if (ROT && rc == HKV_ERR_RANGE) Py_RETURN_NONE;    // (as above)
+    return PyLong_FromLong(rc);
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
+// decode_b8(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, bmm2_scale, gk, gv, qlmax, out, workspace, fmt,
+//           window, sinks, splits, lse)
+PyObject* decode_b8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  try {
+    if (n != 19 || !abi.decode_b8) Py_RETURN_NONE;
+    const at::Tensor *q = tensor(a[0]), *bt = tensor(a[4]), *lens = tensor(a[5]), *qsl = tensor(a[6]), *gk = tensor(a[9]),
+                     *gv = tensor(a[10]), *out = tensor(a[12]), *ws = tensor(a[13]);
+    if (!q || !bt || !lens || !qsl || !gk || !out || !ws || !q->is_cuda() || gk->dim() != 1) Py_RETURN_NONE;
+    const int dev = q->device().index();
+    long long PS, qlmax, splits = 0;
+    double s1, s2;
+    int fmt;
+    Tiles c;
+    Window w;
+    if (dev != c10::cuda::current_device() || !integer(a[3], &PS) || PS != (int)PS || !number(a[7], &s1) || !number(a[8], &s2) ||
+        !integer(a[11], &qlmax) || qlmax != (int)qlmax || !format_of(a[14], &fmt) ||
+        (a[17] != Py_None && (!integer(a[17], &splits) || splits != (int)splits)))
+      Py_RETURN_NONE;
+    if (q->scalar_type() != at::kBFloat16 || out->scalar_type() != at::kBFloat16 || q->dim() != 3 || out->dim() != 3 ||
+        out->size(1) != q->size(1) || out->size(2) != q->size(2) || out->size(0) < q->size(0) || !q->is_contiguous() ||
+        !out->is_contiguous() || bt->dim() != 2 || lens->dim() != 1 || qsl->dim() != 1 || lens->size(0) != bt->size(0) ||
+        qsl->size(0) != bt->size(0) + 1 || !on(*out, dev) || !on(*ws, dev))
+      Py_RETURN_NONE;
+    for (const at::Tensor* t : {bt, lens, qsl})
+      if (!on(*t, dev) || t->scalar_type() != at::kInt || !t->is_contiguous()) Py_RETURN_NONE;
+    const int64_t B = bt->size(0), MP = bt->size(1), KVH = gk->size(0), HQ = q->size(1), D = q->size(2);
+    if (KVH < 1 || HQ % KVH || B > INT32_MAX || MP > INT32_MAX || HQ > INT32_MAX || D > INT32_MAX || !scales(gk, gv, KVH, dev) ||
+        !tiles_of(a[1], a[2], dev, &c) || !window_of(a[15], a[16], a[18], q->size(0), HQ, dev, &w))
+      Py_RETURN_NONE;
+    const void* qp = q->data_ptr();
+    const int32_t *btp = static_cast<const int32_t*>(bt->data_ptr()), *lp = static_cast<const int32_t*>(lens->data_ptr()),
+                  *sp = static_cast<const int32_t*>(qsl->data_ptr());
+    const float *gkp = static_cast<const float*>(gk->data_ptr()), *gvp = static_cast<const float*>(gv->data_ptr());
+    void *op = out->data_ptr(), *wp = ws->data_ptr(), *st = c10::cuda::getCurrentCUDAStream(dev).stream();
+    const size_t wsb = ws->nbytes();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = abi.decode_b8(qp, c.k, c.v, c.strides, (int)PS, btp, (int)MP, lp, sp, (int)B, (int)KVH, (int)(HQ / KVH), (int)D, (int)qlmax,
+                       (float)s1, (float)s2, gkp, gvp, wp, wsb, (int)splits, fmt, w.window, w.sinks, w.lse, op, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
   } catch (...) {
     Py_RETURN_NONE;
   }
@@ -430,6 +598,23 @@ PyObject* layer_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
+// [(table row, q0, q1, L)] within B requests, NT query tokens and a table's reach
+bool prefill_rows(PyObject* list, int64_t B, int64_t reach, int64_t NT, std::vector<int32_t>* rows) {
+  if (!PyList_CheckExact(list) || PyList_GET_SIZE(list) > INT32_MAX) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(list);
+  rows->resize(4 * n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* t = PyList_GET_ITEM(list, i);
+    long long v[4];
+    if (!PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != 4) return false;
+    for (int k = 0; k < 4; ++k)
+      if (!integer(PyTuple_GET_ITEM(t, k), &v[k])) return false;
+    if (v[3] > reach || v[0] < 0 || v[0] >= B || v[1] < 0 || v[1] >= v[2] || v[2] > NT || v[3] < 1 || v[3] > INT32_MAX) return false;
+    for (int k = 0; k < 4; ++k) (*rows)[4 * i + k] = (int32_t)v[k];
+  }
+  return true;
+}
+
 // prefill(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, chunk, signs, k8, workspace);
 // prefill_window: .., window, sinks, lse
 template <bool WIN>
@@ -458,19 +643,9 @@ PyObject* prefill_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (HQ % KVH || B > INT32_MAX || MP > INT32_MAX || NT > INT32_MAX || HQ > INT32_MAX || D > INT32_MAX ||
         !sign_vector(a[11], D, dev, &signs) || (k8 && signs) || !cache_of(a[1], a[2], dev, &c))
       Py_RETURN_NONE;
-    const Py_ssize_t n_rows = PyList_GET_SIZE(a[5]);
-    if (n_rows > INT32_MAX) Py_RETURN_NONE;
-    std::vector<int32_t> rows(4 * n_rows);
-    for (Py_ssize_t i = 0; i < n_rows; ++i) {
-      PyObject* t = PyList_GET_ITEM(a[5], i);
-      long long v[4];
-      if (!PyTuple_CheckExact(t) || PyTuple_GET_SIZE(t) != 4) Py_RETURN_NONE;
-      for (int k = 0; k < 4; ++k)
-        if (!integer(PyTuple_GET_ITEM(t, k), &v[k])) Py_RETURN_NONE;
-      if (v[3] > MP * PS || v[0] < 0 || v[0] >= B || v[1] < 0 || v[1] >= v[2] || v[2] > NT || v[3] < 1 || v[3] > INT32_MAX)
-        Py_RETURN_NONE;
-      for (int k = 0; k < 4; ++k) rows[4 * i + k] = (int32_t)v[k];
-    }
+    std::vector<int32_t> rows;
+    if (!prefill_rows(a[5], B, MP * PS, NT, &rows)) Py_RETURN_NONE;
+    const Py_ssize_t n_rows = (Py_ssize_t)(rows.size() / 4);
     const int G = (int)(HQ / KVH);
     Window w;
     if (WIN && !window_of(a[14], a[15], a[16], NT, HQ, dev, &w)) Py_RETURN_NONE;
@@ -500,10 +675,55 @@ PyObject* prefill_any(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
 }
 
+// prefill_b8(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, fmt, window, sinks, chunk, workspace, lse)
+PyObject* prefill_b8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  try {
+    if (n != 16 || !abi.prefill_b8) Py_RETURN_NONE;
+    const at::Tensor *q = tensor(a[0]), *bt = tensor(a[4]), *out = tensor(a[9]), *ws = a[14] == Py_None ? nullptr : tensor(a[14]);
+    if (!q || !bt || !out || (!ws && a[14] != Py_None) || !q->is_cuda()) Py_RETURN_NONE;
+    const int dev = q->device().index();
+    long long PS, KVH, chunk;
+    double s1, s2;
+    int fmt;
+    Tiles c;
+    Window w;
+    if (dev != c10::cuda::current_device() || !integer(a[3], &PS) || PS < 1 || PS != (int)PS || !number(a[6], &s1) || !number(a[7], &s2) ||
+        !integer(a[8], &KVH) || KVH < 1 || KVH != (int)KVH || !format_of(a[10], &fmt) || !integer(a[13], &chunk))
+      Py_RETURN_NONE;
+    const bool out_f32 = out->scalar_type() == at::kFloat;
+    if (q->scalar_type() != at::kBFloat16 || (out->scalar_type() != at::kBFloat16 && !out_f32) || q->dim() != 3 || out->dim() != 3 ||
+        out->size(1) != q->size(1) || out->size(2) != q->size(2) || out->size(0) < q->size(0) || !q->is_contiguous() ||
+        !out->is_contiguous() || !on(*out, dev) || !on(*bt, dev) || bt->scalar_type() != at::kInt || bt->dim() != 2 ||
+        !bt->is_contiguous() || (ws && (!on(*ws, dev) || ws->nbytes() < 64)))
+      Py_RETURN_NONE;
+    const int64_t B = bt->size(0), MP = bt->size(1), NT = q->size(0), HQ = q->size(1), D = q->size(2);
+    std::vector<int32_t> rows;
+    if (HQ % KVH || B > INT32_MAX || MP > INT32_MAX || NT > INT32_MAX || HQ > INT32_MAX || D > INT32_MAX || !tiles_of(a[1], a[2], dev, &c) ||
+        !prefill_rows(a[5], B, MP * PS, NT, &rows) || !window_of(a[11], a[12], a[15], NT, HQ, dev, &w))
+      Py_RETURN_NONE;
+    const int G = (int)(HQ / KVH), n_rows = (int)(rows.size() / 4);
+    const size_t nb = abi.prefill_window_scratch_bytes(rows.data(), n_rows, (int)NT, (int)KVH, G, (int)D, chunk, 0, w.window, w.sinks);
+    const void* qp = q->data_ptr();
+    const int32_t* btp = static_cast<const int32_t*>(bt->data_ptr());
+    void *op = out->data_ptr(), *wp = ws ? ws->data_ptr() : nullptr;
+    const at::Tensor scratch = at::empty({(int64_t)(nb ? nb : 1)}, q->options().dtype(at::kByte));
+    void *sp = scratch.data_ptr(), *st = c10::cuda::getCurrentCUDAStream(dev).stream();
+    int rc;
+    Py_BEGIN_ALLOW_THREADS
+    rc = abi.prefill_b8(qp, 0, c.k, c.v, c.strides, (int)PS, btp, (int)B, (int)MP, rows.data(), n_rows, (int)NT, (int)KVH, G, (int)D,
+                        (float)s1, (float)s2, chunk, fmt, w.window, w.sinks, w.lse, sp, nb, op, out_f32, wp, st);
+    Py_END_ALLOW_THREADS
+    return PyLong_FromLong(rc);
+  } catch (...) {
+    Py_RETURN_NONE;
+  }
+}
+
 // bind(addresses of the entry points in the order of Abi)
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long p[13];
-  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8], &p[9], &p[10], &p[11], &p[12]))
+  unsigned long long p[17];
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKKKKKKKKK", &p[0], &p[1], &p[2], &p[3], &p[4], &p[5], &p[6], &p[7], &p[8], &p[9], &p[10], &p[11],
+                        &p[12], &p[13], &p[14], &p[15], &p[16]))
     return nullptr;
   int i = 0;
   auto take = [&](auto& f) { f = reinterpret_cast<std::remove_reference_t<decltype(f)>>(p[i++]); };
@@ -520,6 +740,10 @@ PyObject* bind(PyObject*, PyObject* args) {
   take(abi.prefill_window);
   take(abi.accumulate_weights);
   take(abi.evict);
+  take(abi.write_rotary);
+  take(abi.write_b8);
+  take(abi.decode_b8);
+  take(abi.prefill_b8);
   Py_RETURN_NONE;
 }
 
@@ -534,6 +758,11 @@ PyMethodDef methods[] = {
     {"prefill_window", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill_any<true>)), METH_FASTCALL, "status, or None: not the plain form"},
     {"accumulate_weights", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(accumulate_weights)), METH_FASTCALL, "status, or None: not the plain form"},
     {"evict", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(evict)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"write_rotary", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(write_rotary)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"write_b8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(write_b8_any<false>)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"write_rotary_b8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(write_b8_any<true>)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"decode_b8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(decode_b8)), METH_FASTCALL, "status, or None: not the plain form"},
+    {"prefill_b8", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(prefill_b8)), METH_FASTCALL, "status, or None: not the plain form"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "hkv_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

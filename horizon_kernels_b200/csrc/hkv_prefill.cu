@@ -206,6 +206,22 @@ __device__ __forceinline__ uint32_t operand_pair(uint32_t h2) {       // f16x2 -
   return *reinterpret_cast<const uint32_t*>(&b);
 }
 
+// values of 16 bytes of the 8-bit cache (K8 = 2: E4M3, 3: int8) times their tile's scale, a power of two. The product is exact in
+// f16 for the exponents that the cache's writer uses, and in bf16.
+template <int K8>
+__device__ __forceinline__ void b8_values(const uint8_t* tile, int D, int row, int blk, uint32_t (&o)[8]) {
+  const uint4 w = *reinterpret_cast<const uint4*>(tile + row * D + ((blk ^ (row & 7)) << 4));
+  const __half2 s2 = __float2half2_rn(*reinterpret_cast<const float*>(tile + 16 * D));
+  const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t lo, hi;
+    b8_to_f16x2<K8 == 3>(ws[i], lo, hi);
+    o[2 * i] = hmul2h(lo, s2);
+    o[2 * i + 1] = hmul2h(hi, s2);
+  }
+}
+
 // One CTA = one key tile of one kv head and side: 128 x D values of 4 (K8: 8) bits in, 16 bits out. Keys: D / 64 images
 // of 128 rows (keys) x 128 bytes; values: 2 images of D rows (channels) x 128 bytes (64 keys). Byte b of row r lies at
 // r * 128 + (b ^ ((r & 7) << 4)): the 128-byte swizzle. HBM-bound on its output; every value is converted once per
@@ -235,7 +251,11 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
       for (int i = 0; i < 8; ++i) o[i] = 0;
       if (there(pos)) {
         const long long page = __ldg(bt + pos / p.PS), off = pos % p.PS;
-        if (K8) {
+        if (K8 >= 2) {
+          b8_values<K8>(p.kd + page * p.dsp + h * p.dsh + (off >> 4) * (16 * D + 16), D, (int)off & 15, blk, o);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) o[i] = operand_pair<BF16>(o[i]);
+        } else if (K8) {
           const uint4 w8 = *reinterpret_cast<const uint4*>(p.kd + page * p.dsp + off * p.dst + h * p.dsh + blk * 16);
           const uint32_t ws[4] = {w8.x, w8.y, w8.z, w8.w};
 #pragma unroll
@@ -272,6 +292,15 @@ __global__ void __launch_bounds__(128) tile_kernel(const __grid_constant__ TileP
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const int pos = pos0 + kb * 64 + c * 8 + k;
+        if (K8 >= 2) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) e[k][i] = 0;
+          if (there(pos)) {
+            const long long page = __ldg(bt + pos / p.PS), off = pos % p.PS;
+            b8_values<K8>(p.vd + page * p.dsp + h * p.dsh + (off >> 4) * (16 * D + 16), D, (int)off & 15, blk, e[k]);
+          }
+          continue;
+        }
         uint2 w = make_uint2(0, 0);
         uint32_t sb = 0;
         if (there(pos)) {
@@ -1353,7 +1382,7 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
   if (n_rows < 0) return HKV_ERR_RANGE;
   int rc = check_rows(rows, n_rows, n_tokens, KVH, G, D);
   if (rc != HKV_OK) return rc;
-  if (k8 && D != 256) return HKV_ERR_UNSUPPORTED;
+  if (k8 == 1 && D != 256) return HKV_ERR_UNSUPPORTED;
   if (!q || !kd || !ksf || !vd || !vsf || !strides || !block_tables || !scratch || !out) return HKV_ERR_NULL;
   if (signs && (k8 || q_f16)) return HKV_ERR_UNSUPPORTED;
   if (PS < 1) return HKV_ERR_UNSUPPORTED;
@@ -1410,7 +1439,11 @@ static int prefill_impl(const void* q, int q_f16, const void* kd, const void* ks
   t.sinks = win.sinks;
   t.k_flip = c < 0.0f ? 0x80008000u : 0u;
   void (*tk)(const TileParams);
-  if (k8) tk = q_f16 ? tile_kernel<256, 0, 1, WIN> : tile_kernel<256, 1, 1, WIN>;
+  if (k8 == 3) tk = D == 128 ? (q_f16 ? tile_kernel<128, 0, 3, WIN> : tile_kernel<128, 1, 3, WIN>)
+                             : q_f16 ? tile_kernel<256, 0, 3, WIN> : tile_kernel<256, 1, 3, WIN>;
+  else if (k8 == 2) tk = D == 128 ? (q_f16 ? tile_kernel<128, 0, 2, WIN> : tile_kernel<128, 1, 2, WIN>)
+                                  : q_f16 ? tile_kernel<256, 0, 2, WIN> : tile_kernel<256, 1, 2, WIN>;
+  else if (k8) tk = q_f16 ? tile_kernel<256, 0, 1, WIN> : tile_kernel<256, 1, 1, WIN>;
   else if (D == 128) tk = q_f16 ? tile_kernel<128, 0, 0, WIN> : tile_kernel<128, 1, 0, WIN>;
   else tk = q_f16 ? tile_kernel<256, 0, 0, WIN> : tile_kernel<256, 1, 0, WIN>;
   void (*ak)(const PrefillParams);
@@ -1492,4 +1525,26 @@ extern "C" int hkv_prefill_window(const void* q, int q_f16, const void* kd, cons
   w.lse = lse;
   return prefill_impl<true>(q, q_f16, kd, ksf, vd, vsf, strides, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D,
                             qk_scale, out_scale, signs, k8, chunk, scratch, scratch_bytes, out, out_f32, workspace, stream, false, w);
+}
+
+extern "C" int hkv_prefill_b8(const void* q, int q_f16, const void* kt, const void* vt, const int64_t strides[2], int PS,
+                              const int32_t* block_tables, int n_tables, int MP, const int32_t* rows, int n_rows, int n_tokens,
+                              int KVH, int G, int D, float qk_scale, float out_scale, int64_t chunk, int fmt, int window, int sinks,
+                              float* lse, void* scratch, size_t scratch_bytes, void* out, int out_f32, void* workspace, void* stream) {
+  if (window < 0 || sinks < 0) return HKV_ERR_RANGE;
+  if (fmt != HKV_B8_E4M3 && fmt != HKV_B8_INT8) return HKV_ERR_UNSUPPORTED;
+  if (PS < 16 || (PS & (PS - 1)) != 0) return HKV_ERR_UNSUPPORTED;
+  if (!strides) return n_rows == 0 ? HKV_OK : HKV_ERR_NULL;
+  if (((uintptr_t)kt | (uintptr_t)vt | (uintptr_t)strides[0] | (uintptr_t)strides[1]) & 15 || (uintptr_t)lse & 3) return HKV_ERR_ALIGN;
+  const int64_t st[6] = {strides[0], 0, strides[1], strides[0], 0, strides[1]};
+  const int k8 = fmt == HKV_B8_INT8 ? 3 : 2;
+  hkv::PfWindow w;
+  w.window = hkv::window_of(rows, n_rows, window);
+  w.sinks = sinks;
+  w.lse = lse;
+  if (w.window == 0 && !lse)
+    return prefill_impl<false>(q, q_f16, kt, kt, vt, vt, st, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D, qk_scale,
+                               out_scale, nullptr, k8, chunk, scratch, scratch_bytes, out, out_f32, workspace, stream, false);
+  return prefill_impl<true>(q, q_f16, kt, kt, vt, vt, st, PS, block_tables, n_tables, MP, rows, n_rows, n_tokens, KVH, G, D, qk_scale,
+                            out_scale, nullptr, k8, chunk, scratch, scratch_bytes, out, out_f32, workspace, stream, false, w);
 }

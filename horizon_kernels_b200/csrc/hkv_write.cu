@@ -21,6 +21,7 @@
 #include <cuda_fp8.h>
 
 #include "hkv_common.cuh"
+#include "hkv_rotary.cuh"
 
 namespace hkv {
 
@@ -237,11 +238,19 @@ __device__ __forceinline__ void score(const f32x2 (&AX)[8], float amax, float sc
 // K8 = 1 (with LPB = 1): the K8V4 slot of the reference (kv_fp4_ref.py:283-311): keys are stored as D signed E4M3
 // bytes, e4m3(k / gk) with an IEEE division, round to nearest even, saturating at +-448 (what vLLM's fp8 cache
 // holds); values keep the FP4 format. A key lane stores 16 bytes instead of 8 code bytes + a scale byte.
-template <int D, int SEARCH, int LPB, int HAD, int K8 = 0>
-__global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
+//
+// ROT = 1: the keys are turned by their positions first (hkv_rotary.cuh) and rounded to bf16, as a launch before this one would
+// have left them; everything above then sees the turned keys. A lane reads its own 16 channels, the 16 they are paired with and
+// their angles; the rows of query heads are turned by further CTAs of the launch.
+template <int D, int SEARCH, int LPB, int HAD, int K8, int ROT>
+__device__ __forceinline__ void write_body(const WriteParams& p, const RotaryParams* r) {
   constexpr int NB = D / 16;                      // blocks per row
   pdl_wait();                                     // inputs and the cache may come from the preceding launch
   pdl_launch_dependents();
+  if (ROT && blockIdx.x >= r->first_block) {
+    rotate_queries<D>(*r, (long long)(blockIdx.x - r->first_block) * blockDim.x + threadIdx.x);
+    return;
+  }
   const int n_blocks = 2 * p.KVH * NB;            // per token (a multiple of 16)
   const long long gid = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / LPB;
   const int cand = LPB == 4 ? (threadIdx.x & 3) : 0;
@@ -282,7 +291,12 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
   const __nv_bfloat16* src = side ? p.val + t * p.vs0 + h * p.vs1 : p.key + t * p.ks0 + h * p.ks1;
   const uint4 w0 = *reinterpret_cast<const uint4*>(src + blk * 16);
   const uint4 w1 = *reinterpret_cast<const uint4*>(src + blk * 16 + 8);
-  const uint32_t ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+  uint32_t ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+  if (ROT && side == 0) {
+    const uint8_t* angles = table_row(*r, t);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) turn_own_group(*r, angles, src, 2 * blk + g, ws + 4 * g);
+  }
   float x[16];
   float amax = 0.0f;
 #pragma unroll
@@ -453,6 +467,15 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
   if (cand == 0) (side ? p.vsf : p.ksf)[page * p.ssp + pos * p.sst + h * p.ssh + blk] = (uint8_t)cb;
 }
 
+template <int D, int SEARCH, int LPB, int HAD, int K8 = 0>
+__global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
+  write_body<D, SEARCH, LPB, HAD, K8, 0>(p, nullptr);
+}
+template <int D, int SEARCH, int LPB, int HAD, int K8 = 0>
+__global__ void __launch_bounds__(256) rotary_write_kernel(const WriteParams p, const RotaryParams r) {
+  write_body<D, SEARCH, LPB, HAD, K8, 1>(p, &r);
+}
+
 // ---- self-test of the conversions the write and decode kernels rely on (see hkv_selftest_codec in include/hkv.h)
 // counts[0]: non-negative non-NaN fp32 bit patterns (0 .. +inf) whose hardware E2M1 code differs from the threshold
 // chain e2m1_mag; counts[1]: the same among the NaN patterns above +inf.
@@ -614,13 +637,14 @@ int record_cuda(cudaError_t e) {
 static int write_impl(const void* key, const void* val, int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, void* kd,
                       void* ksf, void* vd, void* vsf, const int64_t strides[6], int PS, const int64_t* slots,
                       int64_t n_slots, const float* gk, const float* gv, int KVH, int D, int search,
-                      const float* signs, int k8, void* stream) {
+                      const float* signs, int k8, const hkv_rotary* rotary, void* stream) {
   using namespace hkv;
   if (k8 && D != 256) return HKV_ERR_UNSUPPORTED;      // the K8V4 slot exists at head_dim 256 only, like the reference's
   if (k8 && strides && (((uintptr_t)kd | (uintptr_t)strides[0] | (uintptr_t)strides[1] | (uintptr_t)strides[2]) & 15))
     return HKV_ERR_ALIGN;                              // 16-byte key stores
   if (n_slots < 0) return HKV_ERR_RANGE;
-  if (n_slots == 0) return HKV_OK;
+  if (rotary && rotary->n_tokens == 0 && n_slots == 0) return HKV_OK;
+  if (n_slots == 0 && !rotary) return HKV_OK;
   if (!key || !val || !kd || !ksf || !vd || !vsf || !strides || !slots || !gk || !gv) return HKV_ERR_NULL;
   if (D != 128 && D != 256) return HKV_ERR_UNSUPPORTED;
   if (KVH < 1 || KVH > 1024 || PS < 1) return HKV_ERR_UNSUPPORTED;
@@ -662,6 +686,28 @@ static int write_impl(const void* key, const void* val, int64_t ks0, int64_t ks1
   const long long blocks = (lanes + threads - 1) / threads;
   if (blocks > 0x7fffffffll) return HKV_ERR_RANGE;
   cudaStream_t st = (cudaStream_t)stream;
+  if (rotary) {
+    RotaryParams r = {};
+    const int rc = rotary_params(rotary, D, n_slots, key, ks0, ks1, val, vs0, vs1, KVH, &r);
+    if (rc != HKV_OK) return rc;
+    r.first_block = (unsigned)blocks;
+    const long long all = blocks + (query_threads(r, D) + threads - 1) / threads;
+    if (all > 0x7fffffffll) return HKV_ERR_RANGE;
+    void (*rk)(const WriteParams, const RotaryParams);
+    if (k8) {
+      rk = search ? rotary_write_kernel<256, 1, 1, 0, 1> : rotary_write_kernel<256, 0, 1, 0, 1>;
+    } else if (signs) {
+      rk = D == 128 ? (search ? rotary_write_kernel<128, 1, 1, 1> : rotary_write_kernel<128, 0, 1, 1>)
+                    : (search ? rotary_write_kernel<256, 1, 1, 1> : rotary_write_kernel<256, 0, 1, 1>);
+    } else if (D == 128) {
+      rk = lpb == 1 ? (search ? rotary_write_kernel<128, 1, 1, 0> : rotary_write_kernel<128, 0, 1, 0>)
+                    : (search ? rotary_write_kernel<128, 1, 4, 0> : rotary_write_kernel<128, 0, 4, 0>);
+    } else {
+      rk = lpb == 1 ? (search ? rotary_write_kernel<256, 1, 1, 0> : rotary_write_kernel<256, 0, 1, 0>)
+                    : (search ? rotary_write_kernel<256, 1, 4, 0> : rotary_write_kernel<256, 0, 4, 0>);
+    }
+    return record_cuda(launch_pdl(rk, dim3((unsigned)all), dim3(threads), 0, st, p, r));
+  }
   void (*k)(const WriteParams);
   if (k8) {
     k = search ? write_kernel<256, 1, 1, 0, 1> : write_kernel<256, 0, 1, 0, 1>;
@@ -683,7 +729,7 @@ extern "C" int hkv_write(const void* key, const void* val, int64_t ks0, int64_t 
                          const int64_t* slots, int64_t n_slots, const float* gk, const float* gv, int KVH, int D,
                          int search, void* stream) {
   return write_impl(key, val, ks0, ks1, vs0, vs1, kd, ksf, vd, vsf, strides, PS, slots, n_slots, gk, gv, KVH, D,
-                    search, nullptr, 0, stream);
+                    search, nullptr, 0, nullptr, stream);
 }
 
 extern "C" int hkv_write_rot(const void* key, const void* val, int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1,
@@ -692,7 +738,7 @@ extern "C" int hkv_write_rot(const void* key, const void* val, int64_t ks0, int6
                              int search, const float* signs, void* stream) {
   if (!signs) return HKV_ERR_NULL;
   return write_impl(key, val, ks0, ks1, vs0, vs1, kd, ksf, vd, vsf, strides, PS, slots, n_slots, gk, gv, KVH, D,
-                    search, signs, 0, stream);
+                    search, signs, 0, nullptr, stream);
 }
 
 extern "C" int hkv_write_k8(const void* key, const void* val, int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1,
@@ -700,5 +746,15 @@ extern "C" int hkv_write_k8(const void* key, const void* val, int64_t ks0, int64
                             int64_t n_slots, const float* gk, const float* gv, int KVH, int D, int search,
                             void* stream) {
   return write_impl(key, val, ks0, ks1, vs0, vs1, kd, kd, vd, vsf, strides, PS, slots, n_slots, gk, gv, KVH, D, search,
-                    nullptr, 1, stream);
+                    nullptr, 1, nullptr, stream);
+}
+
+extern "C" int hkv_write_rotary(const void* key, const void* val, int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, void* kd,
+                                void* ksf, void* vd, void* vsf, const int64_t strides[6], int PS, const int64_t* slots,
+                                int64_t n_slots, const float* gk, const float* gv, int KVH, int D, int search, const float* signs,
+                                int k8, const hkv_rotary* rotary, void* stream) {
+  if (!rotary) return HKV_ERR_NULL;
+  if (signs && k8) return HKV_ERR_UNSUPPORTED;
+  return write_impl(key, val, ks0, ks1, vs0, vs1, kd, ksf, vd, vsf, strides, PS, slots, n_slots, gk, gv, KVH, D, search, signs, k8 != 0,
+                    rotary, stream);
 }

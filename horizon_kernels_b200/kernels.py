@@ -10,7 +10,7 @@ import ctypes as C
 import torch
 
 from . import _lib
-from .layout import flat_views  # noqa: F401  (re-exported: part of the reference's API)
+from .layout import B8_FORMATS, b8_views, flat_views  # noqa: F401  (re-exported: part of the reference's API)
 
 LOG2E = 1.4426950408889634
 WORKSPACE_HEADER_BYTES = 64        # the status word and its padding, at the start of every workspace
@@ -103,20 +103,8 @@ def _check_signs(signs, D):
         raise TypeError("signs must be a contiguous fp32 tensor of head_dim entries")
 
 
-def write(key, value, flat, strides, PS, slot_mapping, gk, gv, search=True, signs=None, k8=False):
-    """key / value (NT, KVH, D) bf16 views (any token / head strides, last dim contiguous); slot_mapping (NSL,) int64,
-    slot < 0 skipped, tokens beyond NSL untouched; flat / strides from flat_views; gk / gv (KVH,) fp32.
-    signs (D,) fp32 of +-1 on the device: the keys are rotated (FWHT(k * signs) * D^-0.5 in fp32) before they are
-    quantised. Bit-exact to the reference's write_reference (kv_fp4_ref.py:233-245). Signature of
-    kv_fp4_serving.py:994."""
-    rc = (_lib._host or _lib.host()).write(key, value, flat, strides, PS, slot_mapping, gk, gv, search, signs, k8)
-    if rc is not None:
-        if rc:
-            _lib.check(rc, "hkv_write")
-        return
-    # not the plain form that the native side takes: check, raise or serve it here
-    if k8 and signs is not None:
-        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+def _check_write(key, value, flat, slot_mapping, gk, gv, signs=None):
+    """the arguments that the writes share"""
     if key.dtype != torch.bfloat16 or value.dtype != torch.bfloat16:
         raise TypeError("key / value must be bf16")
     if key.dim() != 3 or value.shape != key.shape:
@@ -131,6 +119,23 @@ def write(key, value, flat, strides, PS, slot_mapping, gk, gv, search=True, sign
     _need_cuda(key, value, slot_mapping, gk, gv, *flat)
     _check_signs(signs, key.shape[2])
     _one_device(key, value, slot_mapping, gk, gv, signs, *flat)
+
+
+def write(key, value, flat, strides, PS, slot_mapping, gk, gv, search=True, signs=None, k8=False):
+    """key / value (NT, KVH, D) bf16 views (any token / head strides, last dim contiguous); slot_mapping (NSL,) int64,
+    slot < 0 skipped, tokens beyond NSL untouched; flat / strides from flat_views; gk / gv (KVH,) fp32.
+    signs (D,) fp32 of +-1 on the device: the keys are rotated (FWHT(k * signs) * D^-0.5 in fp32) before they are
+    quantised. Bit-exact to the reference's write_reference (kv_fp4_ref.py:233-245). Signature of
+    kv_fp4_serving.py:994."""
+    rc = (_lib._host or _lib.host()).write(key, value, flat, strides, PS, slot_mapping, gk, gv, search, signs, k8)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_write")
+        return
+    # not the plain form that the native side takes: check, raise or serve it here
+    if k8 and signs is not None:
+        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+    _check_write(key, value, flat, slot_mapping, gk, gv, signs)
     KVH, D = key.shape[1], key.shape[2]
     kd, ksf, vd, vsf = flat
     st = (C.c_int64 * 6)(*strides)
@@ -145,6 +150,125 @@ def write(key, value, flat, strides, PS, slot_mapping, gk, gv, search=True, sign
         else:
             rc = _lib.load().hkv_write_rot(*args, _ptr(signs), _stream())
     _lib.check(rc, "hkv_write")
+
+
+def _rotary(query, key, value, slot_mapping, positions, cos_sin, query_out, interleaved):
+    """the hkv_rotary of a call, its arguments checked"""
+    NT = query.shape[0]
+    if query.dtype != torch.bfloat16 or query_out.dtype != torch.bfloat16:
+        raise TypeError("query / query_out must be bf16")
+    if query.dim() != 3 or query_out.shape != query.shape or query.shape[2] != key.shape[2]:
+        raise ValueError("query / query_out must be (tokens, heads, head_dim) tensors of one shape")
+    if query.stride(-1) != 1 or query_out.stride(-1) != 1:
+        raise ValueError("query / query_out need a contiguous last dimension")
+    if positions.dtype != torch.int64 or not positions.is_contiguous():
+        raise TypeError("positions must be contiguous int64")
+    if positions.shape != (NT,) or slot_mapping.shape[0] > NT:
+        raise ValueError("one position per query token, at most as many slots")
+    if cos_sin.dtype not in (torch.float32, torch.bfloat16) or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+        raise TypeError("cos_sin must be a contiguous fp32 or bf16 tensor (positions, rotated channels)")
+    if cos_sin.shape[1] % 16 or not 16 <= cos_sin.shape[1] <= key.shape[2]:
+        raise ValueError("the rotated channels are a multiple of 16, up to head_dim")
+    _need_cuda(query, positions, cos_sin, query_out)
+    _one_device(key, query, positions, cos_sin, query_out)
+    for a in (query, key, value) if NT else ():
+        same = a is query and a.data_ptr() == query_out.data_ptr() and a.stride() == query_out.stride()
+        if not same and not _rows_apart(a, query_out):
+            raise ValueError("query_out is neither the query itself nor apart from query, key and value")
+    return _lib.Rotary(query.data_ptr(), query.stride(0), query.stride(1), query_out.data_ptr(), query_out.stride(0),
+                       query_out.stride(1), NT, positions.data_ptr(), cos_sin.data_ptr(), cos_sin.shape[0], query.shape[1],
+                       cos_sin.shape[1], int(cos_sin.dtype == torch.bfloat16), int(bool(interleaved)))
+
+
+def _rows_apart(a, b):
+    """whether two (tokens, heads, head_dim) tensors have no element in common: apart as a whole, or columns of the same rows"""
+    span = [(t.shape[1] - 1) * t.stride(1) + t.shape[2] for t in (a, b)]
+    end = [t.data_ptr() + 2 * ((t.shape[0] - 1) * t.stride(0) + s) for t, s in zip((a, b), span)]
+    if end[0] <= b.data_ptr() or end[1] <= a.data_ptr():
+        return True
+    if a.stride(0) != b.stride(0) or a.stride(0) < 1:
+        return False
+    first = a.data_ptr() <= b.data_ptr()
+    off = abs(b.data_ptr() - a.data_ptr()) % (2 * a.stride(0))
+    lo, hi = span if first else span[::-1]
+    return off >= 2 * lo and off + 2 * hi <= 2 * a.stride(0)
+
+
+def write_rotary(query, key, value, flat, strides, PS, slot_mapping, positions, cos_sin, gk, gv, query_out, interleaved=False,
+                 search=True, signs=None, k8=False):
+    """write of keys that are turned by their positions on the way, with the queries, in one launch. query (NT, HQ, D) bf16, any token
+    and head strides; positions (NT,) int64; cos_sin (rows, rot) fp32 or bf16, a row the rot / 2 cosines of a position, then its sines
+    (a position outside takes the nearest row). Channel pairs (x1, x2), i and i + rot / 2 or (interleaved) 2 i and 2 i + 1, become
+    (x1 c - x2 s, x2 c + x1 s) in fp32, rounded once to bf16; channels from rot on stay. query_out, like query, takes the turned
+    queries: the query itself or a tensor apart. Tokens without a slot, or with a negative one, have their queries turned only. The
+    cache's bytes are those of write over the turned keys; the other arguments are as in write."""
+    rc = (_lib._host or _lib.host()).write_rotary(query, key, value, flat, strides, PS, slot_mapping, positions, cos_sin, gk, gv,
+                                                  query_out, interleaved, search, signs, k8)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_write_rotary")
+        return query_out
+    if k8 and signs is not None:
+        raise ValueError("the K8V4 slot keeps FP8 keys: no rotation")
+    _check_write(key, value, flat, slot_mapping, gk, gv, signs)
+    rotary = _rotary(query, key, value, slot_mapping, positions, cos_sin, query_out, interleaved)
+    kd, ksf, vd, vsf = flat
+    with torch.cuda.device(key.device):
+        rc = _lib.load().hkv_write_rotary(
+            _ptr(key), _ptr(value), key.stride(0), key.stride(1), value.stride(0), value.stride(1), _ptr(kd), _ptr(ksf), _ptr(vd),
+            _ptr(vsf), (C.c_int64 * 6)(*strides), int(PS), _ptr(slot_mapping), slot_mapping.shape[0], _ptr(gk), _ptr(gv), key.shape[1],
+            key.shape[2], int(bool(search)), None if signs is None else _ptr(signs), int(bool(k8)), C.byref(rotary), _stream())
+    _lib.check(rc, "hkv_write_rotary")
+    return query_out
+
+
+def _b8_format(fmt):
+    if fmt not in B8_FORMATS:
+        raise ValueError(f"codes of the 8-bit cache are one of {tuple(B8_FORMATS)}, not {fmt!r}")
+    return B8_FORMATS[fmt]
+
+
+def write_b8(key, value, flat, strides, PS, slot_mapping, gk, gv, fmt="e4m3"):
+    """appends to the 8-bit cache: flat / strides from layout.b8_views, fmt "e4m3" or "int8", the other arguments as in write. The
+    tokens of one tile of 16 slots have to be neighbours in slot_mapping (of a slot that is named twice the last token stays). A call
+    that names a tile's first slot begins the tile anew; any other keeps its rows, under a scale that may grow: a power of two, the
+    smallest with codes of at most 448 (int8: 127) for what the call adds, or the tile's own. Rows that the call does not name are
+    rounded to a scale that grows. e4m3 keeps a NaN, int8 turns it into 0."""
+    rc = (_lib._host or _lib.host()).write_b8(key, value, flat, strides, PS, slot_mapping, gk, gv, fmt)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_write_b8")
+        return
+    _write_b8(key, value, flat, strides, PS, slot_mapping, gk, gv, fmt, None)
+
+
+def write_rotary_b8(query, key, value, flat, strides, PS, slot_mapping, positions, cos_sin, gk, gv, query_out, interleaved=False,
+                    fmt="e4m3"):
+    """write_b8 of keys that are turned by their positions on the way, with the queries, as in write_rotary"""
+    rc = (_lib._host or _lib.host()).write_rotary_b8(query, key, value, flat, strides, PS, slot_mapping, positions, cos_sin, gk, gv,
+                                                     query_out, interleaved, fmt)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_write_b8")
+        return query_out
+    _write_b8(key, value, flat, strides, PS, slot_mapping, gk, gv, fmt, (query, positions, cos_sin, query_out, interleaved))
+    return query_out
+
+
+def _write_b8(key, value, flat, strides, PS, slot_mapping, gk, gv, fmt, turn):
+    code = _b8_format(fmt)
+    kt, vt = flat
+    _check_write(key, value, flat, slot_mapping, gk, gv)
+    rotary = None
+    if turn is not None:
+        query, positions, cos_sin, query_out, interleaved = turn
+        rotary = _rotary(query, key, value, slot_mapping, positions, cos_sin, query_out, interleaved)
+    with torch.cuda.device(key.device):
+        rc = _lib.load().hkv_write_b8(
+            _ptr(key), _ptr(value), key.stride(0), key.stride(1), value.stride(0), value.stride(1), _ptr(kt), _ptr(vt),
+            (C.c_int64 * 2)(*strides), int(PS), _ptr(slot_mapping), slot_mapping.shape[0], _ptr(gk), _ptr(gv), key.shape[1],
+            key.shape[2], code, None if rotary is None else C.byref(rotary), _stream())
+    _lib.check(rc, "hkv_write_b8")
 
 
 def _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, signs):
@@ -407,6 +531,65 @@ def prefill_window(query, flat, strides, PS, block_tables, rows, qk_scale, out_s
             None if signs is None else _ptr(signs), int(bool(k8)), int(chunk), window, sinks, None if lse is None else _ptr(lse),
             _ptr(scratch), nb, _ptr(out), int(out.dtype == torch.float32), None if workspace is None else _ptr(workspace), _stream())
     _lib.check(rc, "hkv_prefill_window")
+    return out
+
+
+def decode_b8(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale, bmm2_scale, gk, gv, qlmax, out, workspace,
+              fmt="e4m3", window=0, sinks=0, splits=None, lse=None):
+    """decode_window over the 8-bit cache (flat / strides from layout.b8_views, fmt as in write_b8); window 0: every key up to the row's
+    own. The workspace is alloc_workspace's, and one may serve both caches."""
+    rc = (_lib._host or _lib.host()).decode_b8(query, flat, strides, PS, block_tables, seq_lens, query_start_loc, bmm1_scale,
+                                               bmm2_scale, gk, gv, qlmax, out, workspace, fmt, window, sinks, splits, lse)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_decode_b8")
+        return out
+    code, window, sinks = _b8_format(fmt), int(window), int(sinks)
+    _check_window(window, sinks)
+    kt, vt = flat
+    KVH, G = _check_decode(query, flat, block_tables, seq_lens, query_start_loc, gk, gv, out, workspace, None)
+    _check_lse(lse, query.shape[0], query.shape[1])
+    _one_device(query, lse)
+    (B, MP), D = block_tables.shape, query.shape[2]
+    with torch.cuda.device(query.device):
+        rc = _lib.load().hkv_decode_b8(
+            _ptr(query), _ptr(kt), _ptr(vt), (C.c_int64 * 2)(*strides), int(PS), _ptr(block_tables), MP, _ptr(seq_lens),
+            _ptr(query_start_loc), B, KVH, G, D, int(qlmax), float(bmm1_scale), float(bmm2_scale), _ptr(gk), _ptr(gv), _ptr(workspace),
+            workspace.numel() * workspace.element_size(), 0 if splits is None else int(splits), code, window, sinks,
+            None if lse is None else _ptr(lse), _ptr(out), _stream())
+    _lib.check(rc, "hkv_decode_b8")
+    return out
+
+
+def prefill_b8(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, fmt="e4m3", window=0, sinks=0, chunk=65536,
+               workspace=None, lse=None):
+    """prefill_window over the 8-bit cache (flat / strides from layout.b8_views, fmt as in write_b8); window 0: every key up to the
+    row's own. As in prefill the cached values are taken without their global scales."""
+    rc = (_lib._host or _lib.host()).prefill_b8(query, flat, strides, PS, block_tables, rows, qk_scale, out_scale, KVH, out, fmt, window,
+                                                sinks, chunk, workspace, lse)
+    if rc is not None:
+        if rc:
+            _lib.check(rc, "hkv_prefill_b8")
+        return out
+    code, window, sinks = _b8_format(fmt), int(window), int(sinks)
+    _check_window(window, sinks)
+    kt, vt = flat
+    _check_prefill(query, flat, PS, block_tables, rows, KVH, out, None, workspace)
+    (B, MP), (NT, HQ, D) = block_tables.shape, query.shape
+    _check_lse(lse, NT, HQ)
+    _one_device(query, lse)
+    n = len(rows)
+    host_rows = (C.c_int32 * (4 * n))(*[int(x) for r in rows for x in r])
+    lib = _lib.load()
+    with torch.cuda.device(query.device):
+        nb = int(lib.hkv_prefill_window_scratch_bytes(host_rows, n, NT, KVH, HQ // KVH, D, int(chunk), 0, window, sinks))
+        scratch = torch.empty(max(nb, 1), dtype=torch.uint8, device=query.device)
+        rc = lib.hkv_prefill_b8(
+            _ptr(query), int(query.dtype == torch.float16), _ptr(kt), _ptr(vt), (C.c_int64 * 2)(*strides), int(PS), _ptr(block_tables), B,
+            MP, host_rows, n, NT, KVH, HQ // KVH, D, float(qk_scale), float(out_scale), int(chunk), code, window, sinks,
+            None if lse is None else _ptr(lse), _ptr(scratch), nb, _ptr(out), int(out.dtype == torch.float32),
+            None if workspace is None else _ptr(workspace), _stream())
+    _lib.check(rc, "hkv_prefill_b8")
     return out
 
 

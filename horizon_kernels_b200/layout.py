@@ -93,3 +93,25 @@ def k8_flat_views(kd, vd, vsf):
     is a placeholder (the value scales again), as in the reference's backend (backend.py:287-291)"""
     (fk, fs, fv, fvs), st = flat_views(kd, vsf, vd, vsf)
     return (fk, fvs, fv, fvs), st
+
+
+B8_FORMATS = {"e4m3": 0, "int8": 1}          # codes of the 8-bit cache
+
+
+def b8_slot_bytes(D: int) -> int:
+    """a token's share of the 8-bit cache per kv head and side: D codes and a sixteenth of its tile's 16 scale bytes"""
+    return D + 1
+
+
+def b8_views(kv_cache: torch.Tensor, KVH: int, D: int):
+    """8-bit cache, logical (pages, 2 * KVH, PS, D + 1) uint8, heads [0, KVH) = K and [KVH, 2 * KVH) = V -> ((key tiles, value
+    tiles) flat from their first byte on, byte strides (page, head)). A head's PS / 16 tiles of a page, 16 * D codes and 16 scale
+    bytes each, have to be back to back: the last two dimensions say how many bytes there are, not where a token lies."""
+    if kv_cache.dtype != torch.uint8 or kv_cache.dim() != 4 or kv_cache.shape[1] != 2 * KVH or kv_cache.shape[3] != b8_slot_bytes(D):
+        raise ValueError(f"expected uint8 (pages, {2 * KVH}, PS, {b8_slot_bytes(D)}), got {tuple(kv_cache.shape)}")
+    if kv_cache.stride(3) != 1 or kv_cache.stride(2) != b8_slot_bytes(D):
+        raise ValueError("the tiles of a page and head must be back to back (heads outermost inside a page)")
+    u, o = kv_cache, kv_cache.storage_offset()
+    n = u.untyped_storage().nbytes()
+    v = o + KVH * u.stride(1)
+    return (torch.as_strided(u, (n - o,), (1,), o), torch.as_strided(u, (max(0, n - v),), (1,), v)), (int(u.stride(0)), int(u.stride(1)))

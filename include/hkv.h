@@ -328,6 +328,75 @@ int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t strides[6]
               float* out_weights, int64_t ow_b, int64_t ow_h, int OW, void* stream);
 
 /*
+ * Position rotation on the way into a cache. Pairs of channels (x1, x2) of query and key rows become (x1 c - x2 s, x2 c + x1 s),
+ * products and sums rounded singly in fp32, the result once to bf16; keys are quantised from that, values are not turned. No
+ * counterpart in the reference, whose model rotates in a launch before its write.
+ *   query       bf16 (n_tokens, HQ, D), element strides qs0 (token) and qs1 (head), rows of D contiguous and 16-byte aligned
+ *   query_out   the turned rows, strides os0, os1: the query itself (the same address and strides), or rows that lie apart from the
+ *               query's, the keys' and the values' (columns of the same rows are apart)
+ *   positions   int64[n_tokens], n_tokens >= n_slots: token i's slot is slots[i]; tokens from n_slots on, or with a negative slot,
+ *               have their queries turned and nothing else. A position outside the table takes the nearest row
+ *   table       (rows, rot) contiguous, 16-byte aligned, fp32 or (table_bf16) bf16: rot / 2 cosines, then as many sines
+ *   rot         channels turned, a multiple of 16 up to D; the others stay. Pairs are i and i + rot / 2, or (interleaved) 2 i and 2 i + 1
+ */
+typedef struct hkv_rotary {
+  const void* query;
+  int64_t qs0, qs1;
+  void* query_out;
+  int64_t os0, os1;
+  int64_t n_tokens;
+  const int64_t* positions;
+  const void* table;
+  int64_t rows;
+  int HQ, rot, table_bf16, interleaved;
+} hkv_rotary;
+/* hkv_write (signs: hkv_write_rot, k8: hkv_write_k8 with ksf unused but not NULL; not both) of turned keys, and the turned queries,
+ * in one launch */
+int hkv_write_rotary(const void* key, const void* val, int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, void* kd, void* ksf,
+                     void* vd, void* vsf, const int64_t strides[6], int PS, const int64_t* slots, int64_t n_slots, const float* gk,
+                     const float* gv, int KVH, int D, int search, const float* signs, int k8, const hkv_rotary* rotary, void* stream);
+
+/*
+ * The 8-bit cache: for models that do not bear four bits. No counterpart in the reference.
+ *   tile    16 tokens of one kv head and side, 16 * D + 16 bytes: token t's D codes at t * D, their 16-byte chunk j at chunk
+ *           j ^ (t % 8) (so that the attention kernels read a tile from shared memory without bank conflicts); then the tile's scale, a
+ *           power of two in fp32, and 12 bytes that nothing reads
+ *   value   code * scale * g, the code E4M3 (HKV_B8_E4M3) or int8 (HKV_B8_INT8), g the global scale of the kv head (gk, gv)
+ *   cache   kt, vt: the first tile of page 0 and head 0, keys and values, 16-byte aligned; strides = {page, head} in bytes, multiples of
+ *           16; a head's PS / 16 tiles of a page follow one another. PS a power of two >= 16
+ *
+ * hkv_write_b8   appends: token i goes to slot slots[i] = page * PS + position, a negative slot skips it. key, val, strides as
+ *                hkv_write. The tokens of one tile have to be neighbours in `slots`, as a batch has them; a slot that is named twice
+ *                among them takes the last of its tokens. A call that names a tile's first token begins the tile anew: its other rows
+ *                are whatever they are until they are written. Any other call keeps the tile's rows: the scale is the larger
+ *                one of its own and the smallest 2^e with |x / g| <= 2^e * 448 (int8: 127), HKV_B8_*_MIN <= e <= HKV_B8_*_MAX, and where it grows, the
+ *                rows that the call does not name are rounded to it. Codes are rounded to nearest even; what is beyond
+ *                the largest one takes that, a NaN stays one (int8: 0) and does not count for the scale.
+ *                rotary: turns keys and queries first, or NULL
+ * hkv_decode_b8  hkv_decode_window over this cache (window 0 and lse NULL: hkv_decode); the workspace is hkv_decode's, and the same one
+ *                may serve both caches
+ * hkv_prefill_b8 hkv_prefill_window over it (window 0: every key up to the row's own; scratch: hkv_prefill_window_scratch_bytes with
+ *                rotated 0). Values beyond f16's range (65504) saturate there before they reach the cache: see HKV_B8_*_MAX
+ */
+#define HKV_B8_E4M3 0
+#define HKV_B8_INT8 1
+#define HKV_B8_E4M3_MIN (-15)
+#define HKV_B8_E4M3_MAX 7
+#define HKV_B8_INT8_MIN (-24)
+#define HKV_B8_INT8_MAX 9
+int hkv_write_b8(const void* key, const void* val, int64_t ks0, int64_t ks1, int64_t vs0, int64_t vs1, void* kt, void* vt,
+                 const int64_t strides[2], int PS, const int64_t* slots, int64_t n_slots, const float* gk, const float* gv, int KVH,
+                 int D, int fmt, const hkv_rotary* rotary, void* stream);
+int hkv_decode_b8(const void* q, const void* kt, const void* vt, const int64_t strides[2], int PS, const int32_t* block_tables,
+                  int MP, const int32_t* seq_lens, const int32_t* query_start_loc, int B, int KVH, int G, int D, int qlmax,
+                  float sm_scale, float v_scale, const float* gk, const float* gv, void* workspace, size_t workspace_bytes, int splits,
+                  int fmt, int window, int sinks, float* lse, void* out, void* stream);
+int hkv_prefill_b8(const void* q, int q_f16, const void* kt, const void* vt, const int64_t strides[2], int PS,
+                   const int32_t* block_tables, int n_tables, int MP, const int32_t* rows, int n_rows, int n_tokens, int KVH, int G,
+                   int D, float qk_scale, float out_scale, int64_t chunk, int fmt, int window, int sinks, float* lse, void* scratch,
+                   size_t scratch_bytes, void* out, int out_f32, void* workspace, void* stream);
+
+/*
  * Self-test of the narrow-float conversions the kernels stand on, no counterpart in the reference (whose CPU tests
  * pin the equivalent bit formulas exhaustively: scripts/kernels/kvfp4/test_kvfp4_cpu.py:54-99, :390-434,
  * test_kvfp4_serving_cpu.py:47-110). Writes to `out` (device memory, 8-byte aligned, HKV_SELFTEST_CODEC_BYTES):
