@@ -6,6 +6,7 @@
 #include <cuda_bf16.h>
 
 #include "hkv_common.cuh"
+#include "hkv_f32x2.cuh"
 
 namespace hkv {
 
@@ -18,14 +19,32 @@ struct RotaryParams {
   long long rows;                                    // of the table
   long long n_tokens;
   int HQ, rot, bf16, neighbours;
-  unsigned first_block;                              // CTAs from this one on rotate queries
+  unsigned others;                                   // CTAs that do not rotate queries
+  unsigned long long share;                          // of those that do, times 2^32, rounded up
 };
 
+// True for a CTA that rotates queries; `index` counts the CTAs of its kind. Queries are a matter of memory bandwidth. ALTERNATE: their CTAs
+// lie between those that write the cache, so that an SM has both at a time, which pays where these are bound by their instructions
+// (NVFP4, 16384 tokens, 32 + 2 x 8 heads x 128: 93 us, 102 with the queries last, 106 with them first); else they come last, and
+// fill the SMs that the others leave (the 8-bit cache, 2048 tokens: 12.9 us against 14.8).
+template <bool ALTERNATE>
+__device__ __forceinline__ bool query_block(const RotaryParams& r, unsigned& index) {
+  if (!ALTERNATE) {
+    index = blockIdx.x < r.others ? blockIdx.x : blockIdx.x - r.others;
+    return blockIdx.x >= r.others;
+  }
+  const unsigned before = (unsigned)(blockIdx.x * r.share >> 32), with = (unsigned)((blockIdx.x + 1ull) * r.share >> 32);
+  index = with > before ? before : blockIdx.x - before;
+  return with > before;
+}
+
 // (a position outside the table takes the nearest row)
-__device__ __forceinline__ const uint8_t* table_row(const RotaryParams& r, long long token) {
-  long long pos = __ldg(r.positions + token);
-  pos = pos < 0 ? 0 : pos >= r.rows ? r.rows - 1 : pos;
-  return r.table + pos * r.rot * (r.bf16 ? 2 : 4);
+__device__ __forceinline__ int table_index(const RotaryParams& r, long long token) {
+  const long long pos = __ldg(r.positions + token);
+  return (int)(pos < 0 ? 0 : pos >= r.rows ? r.rows - 1 : pos);
+}
+__device__ __forceinline__ const uint8_t* table_row(const RotaryParams& r, int index) {
+  return r.table + (long long)index * r.rot * (r.bf16 ? 2 : 4);
 }
 __device__ __forceinline__ void bf16x2_floats(uint32_t w, float& lo, float& hi) {
   lo = __uint_as_float(w << 16);
@@ -35,16 +54,21 @@ __device__ __forceinline__ uint32_t floats_bf16x2(float lo, float hi) {
   const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&b);
 }
+template <bool SHARED, typename T>
+__device__ __forceinline__ T table_load(const T* p) {                // SHARED: the row may be a copy in shared memory
+  if (SHARED) return *p;
+  else return __ldg(p);
+}
 // N (4 or 8) neighbouring numbers of a table row, from number `at` (a multiple of N) on
-template <int N>
+template <int N, bool SHARED = false>
 __device__ __forceinline__ void table_numbers(const RotaryParams& r, const uint8_t* row, int at, float (&x)[N]) {
   if (r.bf16) {
     uint32_t w[N / 2];
     if (N == 8) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row + 2 * at));
+      const uint4 v = table_load<SHARED>(reinterpret_cast<const uint4*>(row + 2 * at));
       w[0] = v.x; w[1] = v.y; w[N / 2 - 2] = v.z; w[N / 2 - 1] = v.w;
     } else {
-      const uint2 v = __ldg(reinterpret_cast<const uint2*>(row + 2 * at));
+      const uint2 v = table_load<SHARED>(reinterpret_cast<const uint2*>(row + 2 * at));
       w[0] = v.x; w[1] = v.y;
     }
 #pragma unroll
@@ -52,15 +76,24 @@ __device__ __forceinline__ void table_numbers(const RotaryParams& r, const uint8
   } else {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      const float4 v = __ldg(reinterpret_cast<const float4*>(row + 4 * at) + i);
+      const float4 v = table_load<SHARED>(reinterpret_cast<const float4*>(row + 4 * at) + i);
       x[4 * i] = v.x; x[4 * i + 1] = v.y; x[4 * i + 2] = v.z; x[4 * i + 3] = v.w;
     }
   }
 }
-__device__ __forceinline__ void turn(float& a, float& b, float c, float s) {
-  const float x = __fsub_rn(__fmul_rn(a, c), __fmul_rn(b, s));
-  b = __fadd_rn(__fmul_rn(b, c), __fmul_rn(a, s));
-  a = x;
+// x c - y s, pairwise, each product and the difference rounded: an fma by -1, which cannot absorb the packed product that feeds its
+// first operand, and single products for its addend. (With packed products for both, ptxas 12.9 rounded once where this has to round
+// twice: a bit of one turned value in a few thousand.)
+__device__ __forceinline__ f32x2 turn2(f32x2 x, f32x2 y, f32x2 c, f32x2 s) {
+  return fma2(mul2(y, s), 0xbf800000bf800000ull, pk(__fmul_rn(lo(x), lo(c)), __fmul_rn(hi(x), hi(c))));
+}
+constexpr f32x2 kSigns = 0x8000000080000000ull;
+__device__ __forceinline__ f32x2 bf16x2_pair(uint32_t w) { return (f32x2)(w & 0xffff0000u) << 32 | (w << 16); }
+__device__ __forceinline__ uint32_t pair_bf16x2(f32x2 v) { return floats_bf16x2(lo(v), hi(v)); }
+// two neighbouring values, turned as one of the "neighbours" pairs
+__device__ __forceinline__ uint32_t turn_neighbours(uint32_t w, float c, float s) {
+  const f32x2 v = bf16x2_pair(w);
+  return pair_bf16x2(turn2(v, pk(hi(v), lo(v)), pk(c, c), pk(s, -s)));
 }
 
 // Cosines and sines of a lane's two groups of eight channels. A row is spread over D / 16 lanes; lane j has two groups such that
@@ -90,18 +123,19 @@ __device__ __forceinline__ LaneTurn lane_turn(int j, int rot, int neighbours) {
 struct Angles {
   float c[8], s[8];                                  // halves: of the eight pairs; neighbours: four of group a, four of group b
 };
+template <bool SHARED = false>
 __device__ __forceinline__ void load_angles(const RotaryParams& r, const uint8_t* row, const LaneTurn& t, Angles& a) {
   const int half = r.rot / 2;
   if (t.kind == 1) {
-    table_numbers<8>(r, row, 8 * t.ga, a.c);
-    table_numbers<8>(r, row, half + 8 * t.ga, a.s);
+    table_numbers<8, SHARED>(r, row, 8 * t.ga, a.c);
+    table_numbers<8, SHARED>(r, row, half + 8 * t.ga, a.s);
   } else if (t.kind == 2) {
     float c[4], s[4];
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
       if (g ? t.tb : t.ta) {
-        table_numbers<4>(r, row, 4 * (g ? t.gb : t.ga), c);
-        table_numbers<4>(r, row, half + 4 * (g ? t.gb : t.ga), s);
+        table_numbers<4, SHARED>(r, row, 4 * (g ? t.gb : t.ga), c);
+        table_numbers<4, SHARED>(r, row, half + 4 * (g ? t.gb : t.ga), s);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           a.c[4 * g + i] = c[i];
@@ -117,28 +151,15 @@ __device__ __forceinline__ void turn_groups(uint4& a, uint4& b, const LaneTurn& 
   if (t.kind == 1) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float a0, a1, b0, b1;
-      bf16x2_floats(wa[i], a0, a1);
-      bf16x2_floats(wb[i], b0, b1);
-      turn(a0, b0, an.c[2 * i], an.s[2 * i]);
-      turn(a1, b1, an.c[2 * i + 1], an.s[2 * i + 1]);
-      wa[i] = floats_bf16x2(a0, a1);
-      wb[i] = floats_bf16x2(b0, b1);
+      const f32x2 x = bf16x2_pair(wa[i]), y = bf16x2_pair(wb[i]), c = pk(an.c[2 * i], an.c[2 * i + 1]), s = pk(an.s[2 * i], an.s[2 * i + 1]);
+      wa[i] = pair_bf16x2(turn2(x, y, c, s));
+      wb[i] = pair_bf16x2(turn2(y, x, c, s ^ kSigns));
     }
   } else if (t.kind == 2) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float x, y;
-      if (t.ta) {
-        bf16x2_floats(wa[i], x, y);
-        turn(x, y, an.c[i], an.s[i]);
-        wa[i] = floats_bf16x2(x, y);
-      }
-      if (t.tb) {
-        bf16x2_floats(wb[i], x, y);
-        turn(x, y, an.c[4 + i], an.s[4 + i]);
-        wb[i] = floats_bf16x2(x, y);
-      }
+      if (t.ta) wa[i] = turn_neighbours(wa[i], an.c[i], an.s[i]);
+      if (t.tb) wb[i] = turn_neighbours(wb[i], an.c[4 + i], an.s[4 + i]);
     }
   }
   a = make_uint4(wa[0], wa[1], wa[2], wa[3]);
@@ -154,12 +175,7 @@ __device__ __forceinline__ void turn_own_group(const RotaryParams& r, const uint
     table_numbers<4>(r, angles, 4 * g, c);
     table_numbers<4>(r, angles, half + 4 * g, s);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float x, y;
-      bf16x2_floats(w[i], x, y);
-      turn(x, y, c[i], s[i]);
-      w[i] = floats_bf16x2(x, y);
-    }
+    for (int i = 0; i < 4; ++i) w[i] = turn_neighbours(w[i], c[i], s[i]);
   } else {
     const bool second = 8 * g >= half;
     const int at = second ? 8 * g - half : 8 * g;     // first of the group's pairs
@@ -168,16 +184,10 @@ __device__ __forceinline__ void turn_own_group(const RotaryParams& r, const uint
     float c[8], s[8];
     table_numbers<8>(r, angles, at, c);
     table_numbers<8>(r, angles, half + at, s);
+    const f32x2 sign = second ? kSigns : 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = second ? -s[i] : s[i];         // x2 c + x1 s = x2 c - x1 (-s), bit for bit
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float x0, x1, y0, y1;
-      bf16x2_floats(w[i], x0, x1);
-      bf16x2_floats(wo[i], y0, y1);
-      w[i] = floats_bf16x2(__fsub_rn(__fmul_rn(x0, c[2 * i]), __fmul_rn(y0, s[2 * i])),
-                           __fsub_rn(__fmul_rn(x1, c[2 * i + 1]), __fmul_rn(y1, s[2 * i + 1])));
-    }
+    for (int i = 0; i < 4; ++i)
+      w[i] = pair_bf16x2(turn2(bf16x2_pair(w[i]), bf16x2_pair(wo[i]), pk(c[2 * i], c[2 * i + 1]), pk(s[2 * i], s[2 * i + 1]) ^ sign));
   }
 }
 
@@ -202,7 +212,7 @@ __device__ __forceinline__ void rotate_queries(const RotaryParams& r, long long 
     b[i] = *reinterpret_cast<const uint4*>(src + i * r.qs1 + 8 * t.gb);
   }
   Angles an;
-  load_angles(r, table_row(r, token), t, an);
+  load_angles(r, table_row(r, table_index(r, token)), t, an);
 #pragma unroll
   for (int i = 0; i < kHeadsAtOnce; ++i) {
     if (h0 + i >= r.HQ) break;
@@ -211,8 +221,12 @@ __device__ __forceinline__ void rotate_queries(const RotaryParams& r, long long 
     *reinterpret_cast<uint4*>(dst + i * r.os1 + 8 * t.gb) = b[i];
   }
 }
-inline long long query_threads(const RotaryParams& r, int D) {
-  return r.n_tokens * ((r.HQ + kHeadsAtOnce - 1) / kHeadsAtOnce) * (D / 16);
+// CTAs of the launch, of which `blocks` do something else than rotate queries
+inline long long with_queries(RotaryParams& r, int D, long long blocks, int threads) {
+  const long long n = r.n_tokens * ((r.HQ + kHeadsAtOnce - 1) / kHeadsAtOnce) * (D / 16), q = (n + threads - 1) / threads, all = blocks + q;
+  r.others = (unsigned)blocks;
+  r.share = all > 0 && all < (1ll << 31) ? (((unsigned long long)q << 32) + all - 1) / all : 0;
+  return all;
 }
 
 // ----------------------------------------------------------------------------------------------------- host side
@@ -232,7 +246,7 @@ inline bool rows_disjoint(const void* a, int64_t a0, int64_t a_span, int64_t na,
 inline int rotary_params(const hkv_rotary* u, int D, int64_t n_slots, const void* key, int64_t ks0, int64_t ks1, const void* val,
                          int64_t vs0, int64_t vs1, int KVH, RotaryParams* r) {
   if (!u->query || !u->query_out || !u->positions || !u->table) return HKV_ERR_NULL;
-  if (u->n_tokens < n_slots || u->n_tokens >= (1ll << 31) || u->rows < 1 || u->rows > (1ll << 40)) return HKV_ERR_RANGE;
+  if (u->n_tokens < n_slots || u->n_tokens >= (1ll << 31) || u->rows < 1 || u->rows >= (1ll << 31)) return HKV_ERR_RANGE;
   if (u->HQ < 1 || u->HQ > 65536 || u->rot < 16 || u->rot > D || u->rot % 16) return HKV_ERR_UNSUPPORTED;
   if (u->qs0 < 0 || u->qs1 < 0 || u->os0 < 0 || u->os1 < 0) return HKV_ERR_RANGE;
   if (((uintptr_t)u->query | (uintptr_t)u->query_out | (uintptr_t)u->table) & 15) return HKV_ERR_ALIGN;

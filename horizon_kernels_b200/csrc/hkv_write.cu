@@ -21,6 +21,7 @@
 #include <cuda_fp8.h>
 
 #include "hkv_common.cuh"
+#include "hkv_f32x2.cuh"
 #include "hkv_rotary.cuh"
 
 namespace hkv {
@@ -69,24 +70,6 @@ __device__ __forceinline__ unsigned mag_of(float ax, float s) { return s > 0.0f 
 // sm_100 has fp32 instructions on register pairs (mul / fma .f32x2): each half is an ordinary IEEE operation with
 // round to nearest even, so two of the reference's operations cost one issue slot. Two neighbouring channels of a block
 // travel as one pair.
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pk(float lo, float hi) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float lo(f32x2 v) { return __uint_as_float((uint32_t)v); }
-__device__ __forceinline__ float hi(f32x2 v) { return __uint_as_float((uint32_t)(v >> 32)); }
-__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
 // RN(a - p) for a product p = mul2(..): written as fma(p, -1, a), one rounding of the exact difference like a
 // subtraction. A sub.rn.f32x2 (or add) fed by a mul.rn.f32x2 is contracted by ptxas 12.9 into ONE fused multiply-add,
 // rounding once where the reference rounds twice (seen as a different winner of the scale search in about one block in
@@ -247,12 +230,13 @@ __device__ __forceinline__ void write_body(const WriteParams& p, const RotaryPar
   constexpr int NB = D / 16;                      // blocks per row
   pdl_wait();                                     // inputs and the cache may come from the preceding launch
   pdl_launch_dependents();
-  if (ROT && blockIdx.x >= r->first_block) {
-    rotate_queries<D>(*r, (long long)(blockIdx.x - r->first_block) * blockDim.x + threadIdx.x);
+  unsigned block = blockIdx.x;
+  if (ROT && query_block<true>(*r, block)) {
+    rotate_queries<D>(*r, (long long)block * blockDim.x + threadIdx.x);
     return;
   }
   const int n_blocks = 2 * p.KVH * NB;            // per token (a multiple of 16)
-  const long long gid = ((long long)blockIdx.x * blockDim.x + threadIdx.x) / LPB;
+  const long long gid = ((long long)block * blockDim.x + threadIdx.x) / LPB;
   const int cand = LPB == 4 ? (threadIdx.x & 3) : 0;
   long long t;
   if (p.div_shift >= 0) {
@@ -293,7 +277,7 @@ __device__ __forceinline__ void write_body(const WriteParams& p, const RotaryPar
   const uint4 w1 = *reinterpret_cast<const uint4*>(src + blk * 16 + 8);
   uint32_t ws[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
   if (ROT && side == 0) {
-    const uint8_t* angles = table_row(*r, t);
+    const uint8_t* angles = table_row(*r, table_index(*r, t));
 #pragma unroll
     for (int g = 0; g < 2; ++g) turn_own_group(*r, angles, src, 2 * blk + g, ws + 4 * g);
   }
@@ -472,7 +456,7 @@ __global__ void __launch_bounds__(256) write_kernel(const WriteParams p) {
   write_body<D, SEARCH, LPB, HAD, K8, 0>(p, nullptr);
 }
 template <int D, int SEARCH, int LPB, int HAD, int K8 = 0>
-__global__ void __launch_bounds__(256) rotary_write_kernel(const WriteParams p, const RotaryParams r) {
+__global__ void __launch_bounds__(256, 4) rotary_write_kernel(const WriteParams p, const RotaryParams r) {
   write_body<D, SEARCH, LPB, HAD, K8, 1>(p, &r);
 }
 
@@ -645,7 +629,8 @@ static int write_impl(const void* key, const void* val, int64_t ks0, int64_t ks1
   if (n_slots < 0) return HKV_ERR_RANGE;
   if (rotary && rotary->n_tokens == 0 && n_slots == 0) return HKV_OK;
   if (n_slots == 0 && !rotary) return HKV_OK;
-  if (!key || !val || !kd || !ksf || !vd || !vsf || !strides || !slots || !gk || !gv) return HKV_ERR_NULL;
+  if (n_slots > 0 && (!key || !val || !slots)) return HKV_ERR_NULL;
+  if (!kd || !ksf || !vd || !vsf || !strides || !gk || !gv) return HKV_ERR_NULL;
   if (D != 128 && D != 256) return HKV_ERR_UNSUPPORTED;
   if (KVH < 1 || KVH > 1024 || PS < 1) return HKV_ERR_UNSUPPORTED;
   // 16-byte row loads of bf16 and 8-byte code stores
@@ -690,8 +675,7 @@ static int write_impl(const void* key, const void* val, int64_t ks0, int64_t ks1
     RotaryParams r = {};
     const int rc = rotary_params(rotary, D, n_slots, key, ks0, ks1, val, vs0, vs1, KVH, &r);
     if (rc != HKV_OK) return rc;
-    r.first_block = (unsigned)blocks;
-    const long long all = blocks + (query_threads(r, D) + threads - 1) / threads;
+    const long long all = with_queries(r, D, blocks, threads);
     if (all > 0x7fffffffll) return HKV_ERR_RANGE;
     void (*rk)(const WriteParams, const RotaryParams);
     if (k8) {
