@@ -62,13 +62,18 @@ constexpr int RPAD = 8;          // query rows per (request, kv head) of one pas
 //   LAYOUT 4  the 8-bit cache, E4M3 codes: tiles of 16 token rows of D bytes and the tile's scale (include/hkv.h); keys and
 //             values of 16 tokens are a bulk copy of 16 * D + 16 bytes each
 //   LAYOUT 5  the same with int8 codes
+//   LAYOUT 6, 7   4 and 5 in units of 32 tokens
 template <int D, int LAYOUT>
 struct Geo {
-  static constexpr bool B8 = LAYOUT >= 4;
+  static constexpr bool B8 = LAYOUT >= 4, INT8 = LAYOUT == 5 || LAYOUT == 7;
   static constexpr int SD = D / 2, SS = D / 16, SLOT = B8 ? D + 1 : SD + SS;
-  static constexpr int UB = B8 ? 1 : (D == 128 || LAYOUT != 2) ? 2 : 1;   // 16-token blocks per unit (1 for the K8V4 slot and the 8-bit cache)
+  static constexpr int UB = B8 ? (LAYOUT >= 6 ? 2 : 1) : (D == 128 || LAYOUT != 2) ? 2 : 1;   // 16-token blocks per unit (1 for the K8V4 slot)
   static constexpr int UT = 16 * UB, LOG_UT = UB == 2 ? 5 : 4;
-  static constexpr int NS = D == 128 ? 3 : LAYOUT == 2 ? 3 : 2;   // stages per warp
+  // stages per warp. 8-bit cache at head_dim 128, 16-token units, three CTAs an SM, 2 / 3 stages: 8 requests of 65536 tokens, group 8, 173 /
+  // 185 us, 64 of 1024 to 32768 197 / 208; 32-token units, two stages, two / three CTAs 180 / 185 and 196 / 206. What is on its way beyond
+  // what the memory's latency asks for (100 KB an SM) only delays the first and the last units. At 256, 2 / 3 stages: 96 requests of
+  // 500 to 16384 tokens 85 / 93
+  static constexpr int NS = B8 ? 2 : D == 128 ? 3 : LAYOUT == 2 ? 3 : 2;
   static constexpr int MINB = D == 128 ? 3 : 2;        // CTAs per SM the register budget is sized for
   static constexpr bool K8 = LAYOUT == 2;
   static constexpr int SLOT8 = D + SD + SS;            // K8V4 slot: 400 bytes at head_dim 256
@@ -647,8 +652,8 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
 #pragma unroll
               for (int v = 0; v < 4; ++v) {           // k-step v of the chunk: channels 4v .. 4v+3 of rows r0, r1
                 uint32_t A[4];
-                b8_to_f16x2<LAYOUT == 5>(wa[v], A[0], A[2]);
-                b8_to_f16x2<LAYOUT == 5>(wb[v], A[1], A[3]);
+                b8_to_f16x2<Gm::INT8>(wa[v], A[0], A[2]);
+                b8_to_f16x2<Gm::INT8>(wb[v], A[1], A[3]);
 #pragma unroll
                 for (int q = 0; q < QT; ++q) score_mma(sa[q][v & (Gm::NCH - 1)], A, q, 4 * u + v);
               }
@@ -748,7 +753,8 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
 #pragma unroll
           for (int bi = 0; bi < BB; ++bi) {
             const uint32_t ta = st + (bb + bi) * 16 * Gm::SLOT + 16 * D;
-            const uint32_t ks = lds32(ta) & 0x7f800000u, vs = lds32(ta + Gm::V_BASE) & 0x7f800000u;
+            // (a block that is not there has any scale: its weights are zero, and their factor must be a number)
+            const uint32_t ks = lds32(ta) & 0x7f800000u, vs = min(lds32(ta + Gm::V_BASE) & 0x7f800000u, 0x7e800000u);
             const float f = sc_abs * __uint_as_float(ks), ev = (float)((int)(vs >> 23) - 127);
             lw[bi] = __uint_as_float(0x7f000000u - vs);
 #pragma unroll
@@ -762,7 +768,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
           // rows past the context hold arbitrary bytes: their scores become -inf below, and their value scales are
           // set to zero here, in shared memory, so that the value product needs no masking code
           // (B8: the value codes themselves, since an E4M3 code may be a NaN; any int8 code times a weight of zero is zero)
-          if (LAYOUT != 5 && bb == 0 && lane < UT && (tbase + lane >= L || (WIN && tbase + lane < window_from(p, L, ql) && tbase + lane >= p.sinks))) {
+          if (!Gm::INT8 && bb == 0 && lane < UT && (tbase + lane >= L || (WIN && tbase + lane < window_from(p, L, ql) && tbase + lane >= p.sinks))) {
             const uint32_t a = st + Gm::V_BASE + (Gm::B8 ? (lane >> 4) * 16 * Gm::SLOT + (lane & 15) * D : Gm::SF_BASE + lane * Gm::SF_ROW);
 #pragma unroll
             for (int i = 0; i < (Gm::B8 ? D : Gm::SS); i += 8) sts64_zero(a + i);
@@ -854,8 +860,8 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
               for (int i = 0; i < 8; ++i) {           // channels 2i, 2i + 1 of the chunk: byte pairs over two tokens
                 const uint32_t sel = i & 1 ? 0x7362 : 0x5140;
                 uint32_t A[4];
-                b8_to_f16x2<LAYOUT == 5>(__byte_perm(wa[i >> 1], wb[i >> 1], sel), A[0], A[1]);
-                b8_to_f16x2<LAYOUT == 5>(__byte_perm(wc[i >> 1], wd[i >> 1], sel), A[2], A[3]);
+                b8_to_f16x2<Gm::INT8>(__byte_perm(wa[i >> 1], wb[i >> 1], sel), A[0], A[1]);
+                b8_to_f16x2<Gm::INT8>(__byte_perm(wc[i >> 1], wd[i >> 1], sel), A[2], A[3]);
 #pragma unroll
                 for (int q = 0; q < QT; ++q) mma_f16(o[q][8 * hf + i], A[0], A[1], A[2], A[3], pb[q][bi][0], pb[q][bi][1]);
               }

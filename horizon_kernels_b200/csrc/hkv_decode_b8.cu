@@ -30,14 +30,16 @@ template <int D, int LAYOUT, int QT, bool WIN>
 static B8Variant variant() {
   return {b8_kernel<D, LAYOUT, QT, WIN>, Smem<D, LAYOUT, QT>::TOTAL, QT == 2 ? 2 : Geo<D, LAYOUT>::MINB};
 }
-template <int D, int LAYOUT>
+// (sixteen rows at head_dim 128 in units of 32 tokens: 64 requests of 500 to 8000 tokens, group 8 x 2 query tokens, 79 us, 85 in units of 16)
+template <int D, int FMT>
 static B8Variant variant_of(bool two, bool win) {
-  return two ? (win ? variant<D, LAYOUT, 2, true>() : variant<D, LAYOUT, 2, false>())
-             : win ? variant<D, LAYOUT, 1, true>() : variant<D, LAYOUT, 1, false>();
+  constexpr int L1 = 4 + FMT, L2 = (D == 128 ? 6 : 4) + FMT;
+  return two ? (win ? variant<D, L2, 2, true>() : variant<D, L2, 2, false>())
+             : win ? variant<D, L1, 1, true>() : variant<D, L1, 1, false>();
 }
 static B8Variant variant_of(int D, int fmt, bool two, bool win) {
-  return D == 128 ? (fmt ? variant_of<128, 5>(two, win) : variant_of<128, 4>(two, win))
-                  : fmt ? variant_of<256, 5>(two, win) : variant_of<256, 4>(two, win);
+  return D == 128 ? (fmt ? variant_of<128, 1>(two, win) : variant_of<128, 0>(two, win))
+                  : fmt ? variant_of<256, 1>(two, win) : variant_of<256, 0>(two, win);
 }
 
 struct B8Device {
