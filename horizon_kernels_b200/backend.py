@@ -23,7 +23,7 @@ import torch
 
 from . import _lib
 from . import kernels as K
-from .layout import flat_views, k8_flat_views, k8_slot_bytes, k8_views, slot_bytes, slot_views
+from .layout import B8_FORMATS, b8_slot_bytes, b8_views, flat_views, k8_flat_views, k8_slot_bytes, k8_views, slot_bytes, slot_views
 
 HEAD_SIZES = (128, 256)
 PAGE_SIZES = (16, 32, 64)
@@ -33,6 +33,18 @@ _STATE = {}                       # per device: decode workspace
 
 def _env(name, default):
     return os.environ.get(name, default)
+
+
+def _b8():
+    """HORIZON_KVFP4_B8 = e4m3 or int8: the 8-bit cache with a scale per 16 tokens and kv head, for models that do not bear four bits"""
+    fmt = _env("HORIZON_KVFP4_B8", "0")
+    if fmt in ("0", ""):
+        return None
+    if fmt not in B8_FORMATS:
+        raise ValueError(f"HORIZON_KVFP4_B8 is one of {tuple(B8_FORMATS)}, not {fmt!r}")
+    if _env("HORIZON_KVFP4_K8", "0") == "1" or _env("HORIZON_KVFP4_HAD", "0") == "1":
+        raise ValueError("HORIZON_KVFP4_B8 goes with neither HORIZON_KVFP4_K8 nor HORIZON_KVFP4_HAD")
+    return fmt
 
 
 def _vllm_bases():
@@ -91,6 +103,8 @@ def _build_classes():
                 return spec
             if spec.head_size not in HEAD_SIZES or spec.head_size_v != spec.head_size:
                 raise ValueError(f"horizon_kvfp4 needs head_dim in {HEAD_SIZES}, got {spec.head_size}")
+            if _b8():                                         # 8-bit codes, a tile's scale on average a byte per token
+                return replace(spec, num_head_slots=2 * spec.num_kv_heads, state_content_bytes=b8_slot_bytes(spec.head_size))
             if _env("HORIZON_KVFP4_K8", "0") == "1":          # FP8 keys + FP4 values: one 400-byte slot per kv head
                 if spec.head_size != 256:
                     raise ValueError("the K8V4 slot (HORIZON_KVFP4_K8) exists at head_dim 256 only")
@@ -109,8 +123,8 @@ def _build_classes():
         def supported_kv_cache_layouts(cls):
             """both page orders of the reference (backend.py:107-110): head-major pages (a head's 16-token tile is one
             contiguous run, fetched with one bulk copy: the fast path) first, positions-outermost pages second (fetched
-            row by row). The K8V4 slot is served head-major only."""
-            both = _env("HORIZON_KVFP4_K8", "0") != "1"
+            row by row). The K8V4 slot and the 8-bit cache are served head-major only."""
+            both = _env("HORIZON_KVFP4_K8", "0") != "1" and not _b8()
             try:
                 if _vllm_bases() is None:
                     raise RuntimeError("not inside vLLM")
@@ -219,6 +233,7 @@ def _build_classes():
             self.k8 = _env("HORIZON_KVFP4_K8", "0") == "1"
             if self.k8 and (head_size != 256 or _env("HORIZON_KVFP4_HAD", "0") == "1"):
                 raise ValueError("HORIZON_KVFP4_K8 needs head_dim 256 and keeps FP8 keys: the rotation must be off")
+            self.b8 = _b8()
             # HORIZON_KVFP4_HAD=1: keys are written rotated (Hadamard) and queries rotated inside the decode kernel
             # (reference backend.py:214-222, kv_fp4_ref.py:31-35)
             self.had = _env("HORIZON_KVFP4_HAD", "0") == "1"
@@ -274,7 +289,9 @@ def _build_classes():
             v = self._views
             if v is not None and v[0] == kv_cache.data_ptr() and v[1] == tuple(kv_cache.stride()):
                 return v[2]
-            if self.k8:                                           # (blocks, KVH, PS, 400)
+            if self.b8:                                           # (blocks, 2*KVH, PS, D + 1)
+                flat, strides = b8_views(kv_cache, self.num_kv_heads, self.head_size)
+            elif self.k8:                                         # (blocks, KVH, PS, 400)
                 if kv_cache.shape[1] != self.num_kv_heads:
                     raise ValueError(f"K8V4 cache must have one slot per kv head, got shape {tuple(kv_cache.shape)}")
                 flat, strides = k8_flat_views(*k8_views(kv_cache, self.head_size))
@@ -318,6 +335,11 @@ def _build_classes():
             gk, gv = (self._gk, self._gv) if self._gk is not None else self._scales(layer, key.device)
             D = self.head_size
             self._keep_to(kv_cache)
+            if self.b8:
+                v = self._cache_views(kv_cache)
+                K.write_b8(key.view(key.shape[0], self.num_kv_heads, D), value.view(value.shape[0], self.num_kv_heads, D), v["flat"],
+                           v["strides"], v["PS"], slot_mapping, gk, gv, fmt=self.b8)
+                return
             # the usual arguments are taken as they are; through the views below the call takes half as long again
             rc = (_lib._host or _lib.host()).layer_write(key, value, kv_cache, slot_mapping, gk, gv, D, self.search,
                                                          self._rot(key.device) if self.had else None, self.k8)
@@ -330,6 +352,25 @@ def _build_classes():
             v3 = value.view(value.shape[0], self.num_kv_heads, D) if value.dim() == 2 else value
             K.write(k3, v3, v["flat"], v["strides"], v["PS"], slot_mapping, gk, gv, self.search,
                     signs=self._rot(key.device), k8=self.k8)
+
+        def rotary_kv_cache_update(self, layer, query, key, value, kv_cache, slot_mapping, positions, cos_sin, interleaved=False,
+                                   query_out=None):
+            """do_kv_cache_update of keys that the model has not rotated yet, and the query's rotation, in one launch: query and key are
+            turned by their positions (cos_sin: a row of cosines, then sines, per position; interleaved: pairs of neighbouring channels
+            instead of halves) on the way. Returns the turned query: query_out, or query itself."""
+            gk, gv = (self._gk, self._gv) if self._gk is not None else self._scales(layer, key.device)
+            D, H = self.head_size, self.num_kv_heads
+            self._keep_to(kv_cache)
+            v = self._cache_views(kv_cache)
+            out = query if query_out is None else query_out
+            q3, o3 = (t.view(t.shape[0], self.num_heads, D) if t.dim() == 2 else t for t in (query, out))
+            k3, v3 = (t.view(t.shape[0], H, D) if t.dim() == 2 else t for t in (key, value))
+            args = q3, k3, v3, v["flat"], v["strides"], v["PS"], slot_mapping, positions, cos_sin, gk, gv, o3
+            if self.b8:
+                K.write_rotary_b8(*args, interleaved=interleaved, fmt=self.b8)
+            else:
+                K.write_rotary(*args, interleaved=interleaved, search=self.search, signs=self._rot(key.device), k8=self.k8)
+            return out
 
         # -------------------------------------------------------------------------------------------- forward
         def forward(self, layer, query, key, value, kv_cache, attn_metadata, output, output_scale=None,
@@ -345,7 +386,7 @@ def _build_classes():
             gk, gv = (self._gk, self._gv) if self._gk is not None else self._scales(layer, query.device)
             decode = m.has_decode and m.num_reqs > 0
             self._keep_to(kv_cache)
-            if decode and not self.window:            # as in do_kv_cache_update: the usual arguments as they are
+            if decode and not self.window and not self.b8:   # as in do_kv_cache_update: the usual arguments as they are
                 rc = (_lib._host or _lib.host()).layer_decode(
                     query, kv_cache, m.block_table, m.seq_lens, m.query_start_loc, T, self.scale, float(layer._v_scale_float),
                     gk, gv, m.qlmax, output, st["ws"], self.cps, self.num_heads, self.head_size,
@@ -363,7 +404,11 @@ def _build_classes():
             if not q.is_contiguous():
                 q = q.contiguous()
             out = output.view(output.shape[0], self.num_heads, self.head_size) if output.dim() == 2 else output
-            if decode and self.window:
+            if decode and self.b8:
+                # (the cache's values carry the V scale, once)
+                K.decode_b8(q, v["flat"], v["strides"], v["PS"], m.block_table, m.seq_lens, m.query_start_loc, self.scale, 1.0, gk, gv,
+                            m.qlmax, out, st["ws"], fmt=self.b8, window=self.window, sinks=self.sinks, splits=self.cps or None)
+            elif decode and self.window:
                 K.decode_window(q, v["flat"], v["strides"], v["PS"], m.block_table, m.seq_lens, m.query_start_loc,
                                 self.scale, float(layer._v_scale_float), gk, gv, m.qlmax, out, st["ws"], self.window, self.sinks,
                                 splits=self.cps or None, signs=self._rot(q.device), k8=self.k8)
@@ -400,11 +445,13 @@ def _build_classes():
             bt = m.block_table if m.block_table.is_contiguous() else m.block_table.contiguous()
             args = (q, v["flat"], v["strides"], v["PS"], bt, rows, self.scale * float(layer._k_scale_float),
                     float(layer._v_scale_float), self.num_kv_heads, o)
-            more = dict(chunk=self.prefill_chunk, signs=signs, k8=self.k8, workspace=self._state(q.device)["ws"])
-            if self.window:
-                K.prefill_window(*args, self.window, self.sinks, **more)
+            more = dict(chunk=self.prefill_chunk, workspace=self._state(q.device)["ws"])
+            if self.b8:
+                K.prefill_b8(*args, fmt=self.b8, window=self.window, sinks=self.sinks, **more)
+            elif self.window:
+                K.prefill_window(*args, self.window, self.sinks, signs=signs, k8=self.k8, **more)
             else:
-                K.prefill(*args, **more)
+                K.prefill(*args, signs=signs, k8=self.k8, **more)
             if not direct:
                 for _, q0, q1, _ in rows:
                     out[q0:q1].copy_(o[q0:q1])

@@ -4,11 +4,12 @@ dimension 256, the FP8-key slot, rotated keys). `bench.py` at the repository roo
 module is what the ncu summaries of the other kernels and variants are captured from.
 
     python -m horizon_kernels_b200.microbench write   [--tokens 32768] [--kvh 8] [--d 128] [--iters 10] [--had] [--k8]
+                                                      [--rotary --g 4] [--b8 e4m3|int8 [--run 16]]
     python -m horizon_kernels_b200.microbench dequant [--tokens 262144] [--kvh 8] [--d 128] [--iters 10] [--f16]
     python -m horizon_kernels_b200.microbench pipes
     python -m horizon_kernels_b200.microbench decode  [--batch 192] [--kvh 2] [--g 8] [--d 256] [--min-len 128]
                                                       [--max-len 32768] [--iters 10] [--had] [--k8] [--nhd] [--ql 1]
-                                                      [--window 0] [--sinks 4]
+                                                      [--window 0] [--sinks 4] [--b8 e4m3|int8]
     python -m horizon_kernels_b200.microbench weights (the arguments of decode)
     python -m horizon_kernels_b200.microbench evict   (the arguments of decode) [--keep 2048] [--recent 256]
 """
@@ -56,6 +57,14 @@ def _token_bytes(D, k8):
     return Lt.K8_SLOT if k8 else 2 * Lt.slot_bytes(D)
 
 
+def _turn(a, NT):
+    """queries, positions and a table for a write that rotates"""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    q = torch.randn(NT, a.kvh * a.g, a.d, generator=g, device="cuda").to(torch.bfloat16)
+    return dict(q=q, out=torch.empty_like(q), pos=torch.arange(NT, device="cuda"), table=torch.rand(NT, a.d, generator=g, device="cuda"),
+                bytes=NT * (4 * a.kvh * a.g * a.d + 8 + 4 * a.d))
+
+
 def write(a):
     NT, KVH, D, PS = a.tokens, a.kvh, a.d, 16
     g = torch.Generator(device="cuda").manual_seed(1)
@@ -64,6 +73,23 @@ def write(a):
     k = k.to(torch.bfloat16)
     v = torch.randn(NT, KVH, D, generator=g, device="cuda").to(torch.bfloat16)
     NP = NT // PS + 8
+    if a.b8:
+        # runs of `--run` tokens, each from the start of a tile or (shorter ones) from its second token on
+        n = (NT + a.run - 1) // a.run
+        per = (a.run + 15) // 16
+        flat, st = Lt.b8_views(torch.zeros((n * per, 2 * KVH, PS, D + 1), dtype=torch.uint8, device="cuda"), KVH, D)
+        slots = (torch.randperm(n, generator=g, device="cuda")[:, None] * 16 * per + (a.run < 16) + torch.arange(a.run, device="cuda")).view(-1)[:NT]
+        one = torch.ones(KVH, device="cuda")
+        byts = NT * KVH * D * 6 + 8 * NT
+        call = lambda: K.write_b8(k, v, flat, st, PS, slots, one, one, fmt=a.b8)  # noqa: E731
+        if a.rotary:
+            turn = _turn(a, NT)
+            byts += turn["bytes"]
+            call = lambda: K.write_rotary_b8(turn["q"], k, v, flat, st, PS, slots, turn["pos"], turn["table"], one, one, turn["out"], fmt=a.b8)  # noqa: E731
+        ms = _time(call, a.iters)
+        print(json.dumps({"kernel": "write", "b8": a.b8, "tokens": NT, "run": a.run, "kv_heads": KVH, "head_dim": D, "rotary": a.rotary,
+                          "us": ms * 1e3, "algorithmic_gbs": byts / ms / 1e6}))
+        return
     flat, st, _ = _pool(NP, KVH, D, PS, a.k8)
     signs = K.hadamard_signs(D, device="cuda") if a.had else None
     slots = torch.randperm(NP * PS, generator=g, device="cuda")[:NT]
@@ -71,11 +97,16 @@ def write(a):
     # boundary of the 4-bit grid
     gk = torch.full((KVH,), float(k.float().abs().max()) / (6 * 448), device="cuda")
     gv = torch.full((KVH,), float(v.float().abs().max()) / (6 * 448), device="cuda")
-    byts = NT * KVH * (D * 4 + _token_bytes(D, a.k8)) + 8 * NT
+    byts = NT * KVH * (D * 4 + _token_bytes(D, a.k8)) + 8 * NT + (NT * (4 * KVH * a.g * D + 8 + 4 * D) if a.rotary else 0)
+    turn = _turn(a, NT) if a.rotary else None
     for search in (True, False):
-        ms = _time(lambda: K.write(k, v, flat, st, PS, slots, gk, gv, search, signs=signs, k8=a.k8), a.iters)
+        if turn:
+            ms = _time(lambda: K.write_rotary(turn["q"], k, v, flat, st, PS, slots, turn["pos"], turn["table"], gk, gv, turn["out"],
+                                              search=search, signs=signs, k8=a.k8), a.iters)
+        else:
+            ms = _time(lambda: K.write(k, v, flat, st, PS, slots, gk, gv, search, signs=signs, k8=a.k8), a.iters)
         print(json.dumps({"kernel": "write", "tokens": NT, "kv_heads": KVH, "head_dim": D, "search": search,
-                          "rotated": a.had, "k8": a.k8, "us": ms * 1e3, "algorithmic_gbs": byts / ms / 1e6}))
+                          "rotated": a.had, "k8": a.k8, "rotary": a.rotary, "us": ms * 1e3, "algorithmic_gbs": byts / ms / 1e6}))
 
 
 def dequant(a):
@@ -106,7 +137,10 @@ def decode(a):
     tot, MP = sum(pages), max(pages)
     OMP = (a.keep + PS - 1) // PS if a.kernel == "evict" else 0
     NP = tot + tot // 4 + 8 + B * OMP
-    flat, st, pool = _pool(NP, KVH, D, PS, a.k8, a.nhd)
+    if a.b8:
+        flat, st = Lt.b8_views(torch.zeros((NP, 2 * KVH, PS, D + 1), dtype=torch.uint8, device="cuda"), KVH, D)
+    else:
+        flat, st, pool = _pool(NP, KVH, D, PS, a.k8, a.nhd)
     signs = K.hadamard_signs(D, device="cuda") if a.had else None
     perm = torch.randperm(NP - 1, generator=g, device="cuda") + 1
     fresh, perm = perm[tot:tot + B * OMP].to(torch.int32).view(B, OMP), perm[:tot]
@@ -117,6 +151,8 @@ def decode(a):
         o += n
     gk = torch.full((KVH,), (1.0 if a.k8 else 1 / 6) * 100.0 / 448, device="cuda")
     gv = torch.full((KVH,), 5.0 / (6 * 448), device="cuda")
+    if a.b8:
+        gk = gv = torch.ones(KVH, device="cuda")
     CH = 8192                                      # pages filled per write launch
     for i in range(0, tot, CH):
         pg = perm[i:i + CH]
@@ -125,7 +161,10 @@ def decode(a):
         k[:, :, [3, D // 4 + 3, D // 2 + 3, 3 * D // 4 + 3]] *= 20
         v = torch.randn(n, KVH, D, generator=g, device="cuda")
         sl = (pg[:, None] * PS + torch.arange(PS, device="cuda")[None, :]).reshape(-1)
-        K.write(k.to(torch.bfloat16), v.to(torch.bfloat16), flat, st, PS, sl, gk, gv, False, signs=signs, k8=a.k8)
+        if a.b8:
+            K.write_b8(k.to(torch.bfloat16), v.to(torch.bfloat16), flat, st, PS, sl, gk, gv, fmt=a.b8)
+        else:
+            K.write(k.to(torch.bfloat16), v.to(torch.bfloat16), flat, st, PS, sl, gk, gv, False, signs=signs, k8=a.k8)
     ql = a.ql                                      # query tokens per request (1 + draft tokens), causal among themselves
     q = torch.randn(B * ql, KVH * G, D, generator=g, device="cuda").to(torch.bfloat16)
     sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
@@ -133,7 +172,10 @@ def decode(a):
     out = torch.empty_like(q)
     ws = K.alloc_workspace(B, KVH, G, D, ql, "cuda")
     more = {}
-    if a.kernel == "decode" and not a.window:
+    if a.b8:
+        def call():
+            K.decode_b8(q, flat, st, PS, bt, sl, qsl, D ** -0.5, 1.0, gk, gv, ql, out, ws, fmt=a.b8, window=a.window, sinks=a.sinks)
+    elif a.kernel == "decode" and not a.window:
         def call():
             K.decode_ragged(q, flat, st, PS, bt, sl, qsl, D ** -0.5, 1.0, gk, gv, ql, out, ws, signs=signs, k8=a.k8)
     else:
@@ -142,7 +184,7 @@ def decode(a):
         def call():
             K.decode_window(q, flat, st, PS, bt, sl, qsl, D ** -0.5, 1.0, gk, gv, ql, out, ws, a.window, a.sinks, signs=signs, k8=a.k8, lse=lse)
     seen = [n if not a.window else min(n, a.window + ql - 1) + min(max(0, n - a.window - ql + 1), a.sinks) for n in lens]
-    byts = sum(seen) * KVH * _token_bytes(D, a.k8)
+    byts = sum(seen) * KVH * (2 * D if a.b8 else _token_bytes(D, a.k8))
     if a.kernel != "decode":
         call()
         w = torch.zeros((B, KVH, max(lens)), device="cuda")
@@ -163,7 +205,7 @@ def decode(a):
     if K.workspace_status(ws) != 0 or K.workspace_status(None) != 0 or not bool(torch.isfinite(out.float()).all()):
         raise RuntimeError("decode reported a wait that ran out, or a non-finite output")
     print(json.dumps({"kernel": a.kernel, "batch": B, "kv_heads": KVH, "group": G, "head_dim": D,
-                      "rotated": a.had, "k8": a.k8, "positions_outermost_pages": a.nhd, "query_tokens": ql,
+                      "rotated": a.had, "k8": a.k8, "b8": a.b8, "positions_outermost_pages": a.nhd, "query_tokens": ql,
                       "query_rows_per_kv_head": G * ql, "cached_tokens": sum(lens), "cache_mb": byts / 1e6,
                       "us": ms * 1e3, "algorithmic_gbs": byts / ms / 1e6,
                       **({"window": a.window, "sinks": a.sinks} if a.window else {}), **more}))
@@ -204,6 +246,9 @@ def main():
     ap.add_argument("--max-len", type=int, default=32768)
     ap.add_argument("--had", action="store_true", help="rotated keys (sign flips + Hadamard transform)")
     ap.add_argument("--k8", action="store_true", help="the FP8-key slot (head_dim 256)")
+    ap.add_argument("--b8", choices=list(Lt.B8_FORMATS), default=None, help="write, decode: the 8-bit cache with a scale per 16 tokens")
+    ap.add_argument("--rotary", action="store_true", help="write: keys and queries turned by their positions on the way")
+    ap.add_argument("--run", type=int, default=16, help="write --b8: tokens of a request")
     ap.add_argument("--ql", type=int, default=1, help="decode: query tokens per request (group x ql rows per kv head)")
     ap.add_argument("--nhd", action="store_true", help="decode: pages with positions outermost (row-copy path)")
     ap.add_argument("--window", type=int, default=0, help="decode, weights: a query token sees its last WINDOW tokens and the first SINKS")
@@ -213,6 +258,8 @@ def main():
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--f16", action="store_true")
     a = ap.parse_args()
+    if a.b8 and (a.kernel not in ("write", "decode") or a.had or a.k8 or a.nhd):
+        ap.error("--b8 goes with write and decode, without --had, --k8 and --nhd")
     if a.tokens is None:
         a.tokens = 32768 if a.kernel == "write" else 262144
     if a.kvh is None:
