@@ -5,9 +5,15 @@
 // S^T = K Q^T and O^T += V^T P^T with mma.m16n8k16, merge inside the launch) over this layout. What differs:
 //   * a code is converted to f16 and used as it is. The key scale of a block multiplies its scores; the value scale enters the
 //     exponent of the weights, p = 2^(s + e_v - max), and the sum of the weights takes it out again, so that neither costs an
-//     instruction per element. Both are exact.
+//     instruction per element. Both are exact; a weight, f16, keeps its 11 bits down to 2^-14 of the largest product of a weight and
+//     a value scale, and is off by at most 2^-25 of that product below.
 //   * the chunks of a tile are permuted in the cache, so that a bulk copy brings rows of 128 or 256 bytes whose 16-byte loads touch every
 //     bank once, both along the channels (keys) and along the tokens (values).
+//
+// B200, back to back: 8 requests of 65536 tokens, 8 kv heads x 128, group 8, 174 us (6.2 TB/s, 0.95 of a copy), 64 of 1024 to 32768 197
+// (0.93); 96 of 500 to 16384, 2 x 256, group 8, 85 (0.81), with two query tokens 95 (int8: 97). The memory bounds the long ones; the
+// others lose 10 to 15 us to the start and the end of the launch, sixteen rows at head_dim 256 also to dependency latency at 255 registers
+// and eight warps an SM.
 #include <algorithm>
 #include <atomic>
 #include <mutex>

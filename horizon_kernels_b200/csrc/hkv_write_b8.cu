@@ -5,6 +5,11 @@
 // codes. Rows of a tile that the call does not name keep their codes unless the scale grows; then the same warp rounds them to
 // the new one. A scale is a power of two, so that codes times scales are exact in 16 bits (prefill operands), and growing costs an
 // E4M3 code nothing but its last subnormal bits.
+//
+// What bounds it: the chain of latencies of a tile (slots, rows, the largest of them, stores) over the warps that an SM holds, and the
+// instructions of the rotation. B200, 8 kv heads x 128, back to back: 17108 tokens of twelve prompts 25 us (4.2 TB/s), with the
+// rotation of the keys and 32 query heads 69 us (5.7 TB/s; the queries alone take 44); four single tokens 1.9 and 2.4 us. With the rows
+// in registers instead of shared memory a key warp took 128 of them: 97 us for the prompts; angles from global memory for every head: the same.
 #include <cuda_fp8.h>
 
 #include "hkv_common.cuh"

@@ -230,7 +230,8 @@ def _b8_format(fmt):
 
 def write_b8(key, value, flat, strides, PS, slot_mapping, gk, gv, fmt="e4m3"):
     """appends to the 8-bit cache: flat / strides from layout.b8_views, fmt "e4m3" or "int8", the other arguments as in write. The
-    tokens of one tile of 16 slots have to be neighbours in slot_mapping (of a slot that is named twice the last token stays). A call
+    tokens of one tile of 16 slots have to follow one another in slot_mapping, with no other entry (nor a skipped one) between them;
+    of a slot that is named twice the last token stays. A call
     that names a tile's first slot begins the tile anew; any other keeps its rows, under a scale that may grow: a power of two, the
     smallest with codes of at most 448 (int8: 127) for what the call adds, or the tile's own. Rows that the call does not name are
     rounded to a scale that grows. e4m3 keeps a NaN, int8 turns it into 0."""

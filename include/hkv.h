@@ -204,7 +204,7 @@ int hkv_dequant_k8(const void* kd, const void* vd, const void* vsf, const int64_
 /*
  * Process-wide options. No counterpart in the reference.
  *   HKV_OPT_EARLY_METADATA (0 = off, the default; 1 = on): the caller states that `seq_lens` and `query_start_loc` of
- *     every later hkv_decode / hkv_decode_window / hkv_decode_noalloc call are complete before the kernel that PRECEDES the call on its
+ *     every later hkv_decode / hkv_decode_window / hkv_decode_b8 / hkv_decode_noalloc call are complete before the kernel that PRECEDES the call on its
  *     stream starts (an inference engine writes them once per step, long before the attention layers run; hkv_write never
  *     writes them). hkv_decode then reads these two arrays while the preceding kernel is still running and waits for
  *     it only afterwards, before it touches the block tables, the cache, the queries or the workspace. With the option
@@ -366,17 +366,18 @@ int hkv_write_rotary(const void* key, const void* val, int64_t ks0, int64_t ks1,
  *           16; a head's PS / 16 tiles of a page follow one another. PS a power of two >= 16
  *
  * hkv_write_b8   appends: token i goes to slot slots[i] = page * PS + position, a negative slot skips it. key, val, strides as
- *                hkv_write. The tokens of one tile have to be neighbours in `slots`, as a batch has them; a slot that is named twice
- *                among them takes the last of its tokens. A call that names a tile's first token begins the tile anew: its other rows
- *                are whatever they are until they are written. Any other call keeps the tile's rows: the scale is the larger
- *                one of its own and the smallest 2^e with |x / g| <= 2^e * 448 (int8: 127), HKV_B8_*_MIN <= e <= HKV_B8_*_MAX, and where it grows, the
- *                rows that the call does not name are rounded to it. Codes are rounded to nearest even; what is beyond
- *                the largest one takes that, a NaN stays one (int8: 0) and does not count for the scale.
- *                rotary: turns keys and queries first, or NULL
+ *                hkv_write. The tokens of one tile have to follow one another in `slots`, as a batch has them, in any order, with no
+ *                other entry between them (one without a slot neither): separate runs of one tile would be written at the same time.
+ *                A slot that is named twice in a run takes the last of its tokens. A call that names a tile's first token begins the
+ *                tile anew: its other rows are whatever they are until they are written. Any other call keeps the tile's rows:
+ *                the scale is the larger one of its own and the smallest 2^e with |x / g| <= 2^e * 448 (int8: 127),
+ *                HKV_B8_*_MIN <= e <= HKV_B8_*_MAX, and where it grows, the rows that the call does not name are rounded to it. Codes
+ *                are rounded to nearest even; what is beyond the largest one takes that, a NaN stays one (int8: 0) and does not
+ *                count for the scale. rotary: turns keys and queries first, or NULL
  * hkv_decode_b8  hkv_decode_window over this cache (window 0 and lse NULL: hkv_decode); the workspace is hkv_decode's, and the same one
  *                may serve both caches
  * hkv_prefill_b8 hkv_prefill_window over it (window 0: every key up to the row's own; scratch: hkv_prefill_window_scratch_bytes with
- *                rotated 0). Values beyond f16's range (65504) saturate there before they reach the cache: see HKV_B8_*_MAX
+ *                rotated 0). Code times scale is exact in f16 and bf16 for the exponents above, so that its operands are the values
  */
 #define HKV_B8_E4M3 0
 #define HKV_B8_INT8 1
