@@ -391,13 +391,9 @@ __global__ void __launch_bounds__(256, FEW || D == 256 ? 3 : 4) b8_write_kernel(
       for (int c = 16 * lane; c < bytes; c += 512) cp_async<16>(smem_u32(angles) + i * (4 * D) + c, row + c);
     }
   }
-  if (hs >= sides) {                                 // (no head for this warp)
-    if (copies && leaders) {
-      cp_async_wait();
-      __syncthreads();
-    }
-    return;
-  }
+  // No head for this warp. Only a set's last CTA of eight warps has such, where 2 * KVH is no multiple of eight: it begins at side
+  // 8 * floor(2 * KVH / 8) >= KVH (KVH >= 5), so that it copies no angles and no barrier waits for this warp.
+  if (hs >= sides) return;
   if (FEW && (__ballot_sync(0xffffffffu, tile >= 0 && tile == before) & leaders << 1) == 0) {      // no tile has a second token
     write_singles<D, INT8, ROT>(p, s, r, ROT && !side, leaders, slot, angle, t0);
     return;

@@ -90,12 +90,12 @@ def runs(kind, PS, P, seed):
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
-@pytest.mark.parametrize("D,KVH,PS", [(128, 2, 16), (256, 1, 32), (128, 3, 64)])
+@pytest.mark.parametrize("D,KVH,PS", [(128, 2, 16), (256, 1, 32), (128, 3, 64), (128, 5, 16), (256, 9, 16)])
 @pytest.mark.parametrize("kind", ["prompt", "tokens", "skips", "twice"])
 def test_append(fmt, D, KVH, PS, kind):
     P = 9
     cache = fresh(P, KVH, PS, D, fmt, 11 * D + PS)
-    gk, gv = torch.tensor([1.0, 0.37, 2.0 ** -20])[:KVH], torch.tensor([0.011, 1.0, 3.0])[:KVH]
+    gk, gv = torch.tensor([1.0, 0.37, 2.0 ** -20] * 3)[:KVH], torch.tensor([0.011, 1.0, 3.0] * 3)[:KVH]
     for step in range(3):
         slots = runs(kind, PS, P, step)
         k, v = rows(len(slots) + 2, KVH, D, 100 * step + D, wild=step == 1)
@@ -125,7 +125,8 @@ def test_append_many_tokens(fmt, D, KVH, n):
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("D,KVH,HQ,rot,interleaved,dtype,n", [(128, 8, 32, 128, False, torch.float32, 40), (256, 2, 6, 64, True, torch.bfloat16, 23),
-                                                            (128, 1, 3, 48, False, torch.bfloat16, 7), (256, 4, 24, 256, False, torch.float32, 1100)])
+                                                            (128, 1, 3, 48, False, torch.bfloat16, 7), (256, 4, 24, 256, False, torch.float32, 1100),
+                                                            (128, 5, 10, 128, False, torch.float32, 2100), (256, 9, 9, 192, True, torch.bfloat16, 9000)])
 def test_append_turned(fmt, D, KVH, HQ, rot, interleaved, dtype, n):
     PS, NT = 32, n + 5
     x = qkv(NT, HQ, KVH, D, n)
