@@ -140,6 +140,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
   constexpr int RP = Sm::RP;
   constexpr int NS = Gm::NS, UB = Gm::UB, UT = Gm::UT, LOG_UT = Gm::LOG_UT;
   constexpr int BB = Sm::QSM ? 1 : UB;             // 16-token blocks of a unit worked on at a time (registers)
+  constexpr bool KEEP = WIN || Gm::B8;             // a piece whose sum is a NaN counts in the merge of its sequence
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* ring = smem;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sm::RING);
@@ -984,7 +985,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
             if (WIN && p.lse && tid == rl * tpr) p.lse[(long long)(q0 + t) * (KVH * G) + h * G + gq] = row_lse(mx, den);
           } else {
             dst_p = opart_ws + ((size_t)slot_id * RP + row) * D;
-            if (tid == rl * tpr) lse_ws[slot_id * RP + row] = (WIN ? den != 0.0f : den > 0.0f) ? log2f(den) + mx : -__int_as_float(0x7f800000);
+            if (tid == rl * tpr) lse_ws[slot_id * RP + row] = (KEEP ? den != 0.0f : den > 0.0f) ? log2f(den) + mx : -__int_as_float(0x7f800000);
           }
           for (int ch = (tid - rl * tpr) * 2; ch < D; ch += 2 * tpr) {
             float n0 = 0.0f, n1 = 0.0f;
@@ -1041,7 +1042,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
         og.row0 = nullptr;
         og.part = opart_ws + (size_t)slot0 * RP * D;
         og.lse = lse_ws + slot0 * RP;
-        merge_pieces<D, RP, NTHREADS, WIN>(Pieces{lse_ws, opart_ws, slot0, gr.first, 1, gr.last - gr.first + 1}, sq.R, og, obuf,
+        merge_pieces<D, RP, NTHREADS, KEEP>(Pieces{lse_ws, opart_ws, slot0, gr.first, 1, gr.last - gr.first + 1}, sq.R, og, obuf,
                                       Sm::MERGE / 4 - RP);
         __threadfence();
         __syncthreads();
@@ -1052,7 +1053,7 @@ __device__ __forceinline__ void decode_body(const DecodeParams& p) {
         pc.step = kGroup;
         pc.n = (last - first) / kGroup + 1;
       }
-      merge_pieces<D, RP, NTHREADS, WIN>(pc, sq.R, o, obuf, Sm::MERGE / 4 - RP);
+      merge_pieces<D, RP, NTHREADS, KEEP>(pc, sq.R, o, obuf, Sm::MERGE / 4 - RP);
     }
   }
 

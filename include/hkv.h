@@ -378,6 +378,9 @@ int hkv_write_rotary(const void* key, const void* val, int64_t ks0, int64_t ks1,
  *                may serve both caches
  * hkv_prefill_b8 hkv_prefill_window over it (window 0: every key up to the row's own; scratch: hkv_prefill_window_scratch_bytes with
  *                rotated 0). Code times scale is exact in f16 and bf16 for the exponents above, so that its operands are the values
+ * What no row of a request may see (behind its context, outside every row's window) may hold anything. A NaN key that some rows see
+ * makes these rows NaN in its kv head; a NaN value (E4M3 only) makes its channel of that head NaN in them, and may do so in the request's
+ * rows of the same call that do not see it yet or any more, as zero times NaN. It reaches no other channel, head or request.
  */
 #define HKV_B8_E4M3 0
 #define HKV_B8_INT8 1

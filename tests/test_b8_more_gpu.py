@@ -165,3 +165,35 @@ def test_single_tokens_and_drafts_of_a_large_batch(fmt, D, KVH, n):
 def test_put_keeps_what_lies_between_pages():
     view, big = put(fresh(2, 1, 16, 128, "int8", 1))
     assert bool((big[:, :, -32:] == 0xc3).all()) and view.shape == (2, 2, 16, 129)
+
+
+@pytest.mark.parametrize("side", ["key", "value"])
+@pytest.mark.parametrize("D,G,kind", [(128, 4, "draft"), (256, 8, "draft"), (128, 4, "window"), (128, 4, "prompt"), (256, 8, "prompt")])
+def test_nan_of_the_last_token(D, G, kind, side):
+    """a NaN that only the last of a request's rows sees: a key's makes that row NaN in its kv head, a value's its channel there. Other
+    channels, heads and requests are as without it, and so are the earlier rows, but for the channel of a value"""
+    KVH, PS, lens, ql = 2, 16, [100, 230, 61], 3 if kind != "prompt" else 40
+    cache, bt = paged(lens, KVH, PS, D, "e4m3", 17 + D)
+    bad, at, head = cache.clone(), lens[1] - 1, 1
+    t = bad.view(len(bad), 2 * KVH, PS // 16, 16 * D + 16)[int(bt[1, at // PS]), head + (KVH if side == "value" else 0), at % PS // 16]
+    t[at % 16 * D + ((2 ^ (at % 8)) << 4) + 5] = 0x7f                       # channel 16 * 2 + 5
+    q = torch.randn(3 * ql, KVH * G, D, generator=gen(D)).to(torch.bfloat16).cuda()
+    ws, one = K.alloc_workspace(3, KVH, G, D, ql if kind != "prompt" else 1), torch.ones(KVH, device="cuda")
+    bt_d, lens_d = bt.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    qsl = (torch.arange(4) * ql).to(torch.int32).cuda()
+    got = []
+    for c in (cache, bad):
+        flat, st = Lt.b8_views(c.cuda(), KVH, D)
+        out = torch.zeros_like(q)
+        if kind == "prompt":
+            K.prefill_b8(q, flat, st, PS, bt_d, [(b, b * ql, b * ql + ql, n) for b, n in enumerate(lens)], D ** -0.5, 1.0, KVH, out, workspace=ws)
+        else:
+            K.decode_b8(q, flat, st, PS, bt_d, lens_d, qsl, D ** -0.5, 1.0, one, one, ql, out, ws, window=50 if kind == "window" else 0)
+        got.append(out.view(3, ql, KVH, G, D).cpu())
+    assert K.workspace_status(ws) == 0 and bool(got[0].isfinite().all())
+    touched = torch.zeros(got[0].shape, dtype=torch.bool)
+    touched[1, -1, head, :, slice(None) if side == "key" else 37] = True
+    assert bool(got[1][touched].isnan().all())
+    if side == "value":
+        touched[1, :, head, :, 37] = True
+    assert torch.equal(got[0][~touched].view(torch.int16), got[1][~touched].view(torch.int16))
