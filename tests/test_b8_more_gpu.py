@@ -197,3 +197,34 @@ def test_nan_of_the_last_token(D, G, kind, side):
     if side == "value":
         touched[1, :, head, :, 37] = True
     assert torch.equal(got[0][~touched].view(torch.int16), got[1][~touched].view(torch.int16))
+
+
+@pytest.mark.parametrize("D,G", [(128, 4), (256, 8)])
+@pytest.mark.parametrize("prompt", [False, True])
+def test_nan_outside_the_windows(D, G, prompt):
+    """NaN keys and values of tokens that no row sees, in tiles whose other tokens rows do see: behind the sinks, before the first row's
+    window, behind the context"""
+    KVH, PS, lens, ql, window, sinks = 2, 32, [100, 230, 61, 700], 35 if prompt else 2, 50, 5
+    cache, bt = paged(lens, KVH, PS, D, "e4m3", 71 + D)
+    bad = cache.clone()
+    for b, L in enumerate(lens):
+        seen = torch.stack([R.sees(L - ql + t, L, window, sinks) for t in range(ql)]).any(0)
+        for j in torch.nonzero(~seen).flatten().tolist():
+            t = bad.view(len(bad), 2 * KVH, PS // 16, 16 * D + 16)[int(bt[b, j // PS]), :, j % PS // 16]
+            t[:, j % 16 * D:(j % 16 + 1) * D] = 0xff
+    q = torch.randn(4 * ql, KVH * G, D, generator=gen(D + ql)).to(torch.bfloat16).cuda()
+    ws, one = K.alloc_workspace(4, KVH, G, D, 1 if prompt else ql), torch.ones(KVH, device="cuda")
+    bt_d, lens_d = bt.cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    qsl = (torch.arange(5) * ql).to(torch.int32).cuda()
+    got = []
+    for c in (cache, bad):
+        flat, st = Lt.b8_views(c.cuda(), KVH, D)
+        out, lse = torch.full_like(q, float("nan")), torch.zeros(4 * ql, KVH * G, device="cuda")
+        if prompt:
+            K.prefill_b8(q, flat, st, PS, bt_d, [(b, b * ql, b * ql + ql, n) for b, n in enumerate(lens)], D ** -0.5, 1.0, KVH, out,
+                         window=window, sinks=sinks, workspace=ws, lse=lse)
+        else:
+            K.decode_b8(q, flat, st, PS, bt_d, lens_d, qsl, D ** -0.5, 1.0, one, one, ql, out, ws, window=window, sinks=sinks, lse=lse)
+        got.append((out, lse))
+    assert K.workspace_status(ws) == 0 and bool(got[0][0].isfinite().all() & got[0][1].isfinite().all())
+    assert torch.equal(got[0][0].view(torch.int16), got[1][0].view(torch.int16)) and torch.equal(got[0][1], got[1][1])
