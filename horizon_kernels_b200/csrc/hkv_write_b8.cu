@@ -415,16 +415,14 @@ __global__ void __launch_bounds__(256, FEW || D == 256 ? 3 : 4) b8_write_kernel(
       if (plain) {
         if (lane >= first && lane < first + len) tok = (int)(t0 - 1) + j0 + lane - first;
         ang = (j0 + lane - first) & 31;
-        if (ROT && FEW) ang = ~__shfl_sync(0xffffffffu, angle, ang);
       } else {
-        for (int i = j0; i < j0 + len; ++i) {
+        for (int i = j0; i < j0 + len; ++i)
           if (lane == ((int)__shfl_sync(0xffffffffu, slot, i) & 15)) {
             tok = (int)(t0 - 1) + i;
             ang = i;
           }
-        if (ROT && FEW) ang = ~__shfl_sync(0xffffffffu, angle, ang);
-        }
       }
+      if (ROT && FEW) ang = ~__shfl_sync(0xffffffffu, angle, ang);
       // runs past the lanes' tokens: only those that lie well inside a set, or name a row twice
       for (long long t = t0 + 31; j0 + len == 32 && t < p.n; t += 32) {
         const long long more = slot_of(t + lane);
