@@ -129,7 +129,9 @@ __device__ __forceinline__ uint2 codes8(const uint4& v, const ToCode& t) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float q = __fmul_rn(y[i], t.r);
-      y[i] = __fmul_rn(__fmaf_rn(__fmaf_rn(-t.m, q, y[i]), t.r, q), t.f);
+      float x = __fmaf_rn(__fmaf_rn(-t.m, q, y[i]), t.r, q);
+      if (!INT8) x = copysignf(x, q);                // (a zero's own sign: its remainder is +0, and so is the sum with q = -0)
+      y[i] = __fmul_rn(x, t.f);
       if (INT8) y[i] = y[i] == y[i] ? fminf(fmaxf(y[i], -127.0f), 127.0f) : 0.0f;
     }
   }
