@@ -161,16 +161,19 @@ struct B8Side {
   int rr;                                            // this lane's row of those that are worked on at a time
 };
 
-// A tile's exponent from the largest magnitude among the call's rows, and whether there is an infinity among them
+// A tile's exponent from the largest magnitude among the call's rows, and whether there is an infinity among them. `was`: the tile's
+// scale word. One that this writer has left is a power of two; a tile whose first slot nobody has written may hold any word, of which the
+// exponent counts, and which is replaced as a whole: the word is compared, not its exponent.
 struct TileScale {
   int e, old;
   bool inf;
+  __device__ __forceinline__ uint32_t word() const { return (uint32_t)(e + 127) << 23; }
 };
 template <bool INT8>
-__device__ __forceinline__ TileScale tile_scale(float g, float amax, bool fresh, int was) {
+__device__ __forceinline__ TileScale tile_scale(float g, float amax, bool fresh, uint32_t was) {
   const int need = tile_exponent<INT8>(__fdiv_rn(amax, g));
   TileScale t;
-  t.old = min(max(was, INT8 ? HKV_B8_INT8_MIN : HKV_B8_E4M3_MIN), INT8 ? HKV_B8_INT8_MAX : HKV_B8_E4M3_MAX);
+  t.old = min(max((int)(was >> 23 & 255u) - 127, INT8 ? HKV_B8_INT8_MIN : HKV_B8_E4M3_MIN), INT8 ? HKV_B8_INT8_MAX : HKV_B8_E4M3_MAX);
   t.e = fresh ? need : max(need, t.old);
   t.inf = amax > 3.38953139e38f;
   return t;
@@ -234,12 +237,12 @@ __device__ __forceinline__ void write_singles(const B8WriteParams& p, const B8Si
     const int row = (int)sl & 15;
     uint8_t* const tile = s.base + tile_offset<D>(p, sl >> 4);
     uint4 a = make_uint4(0, 0, 0, 0), b = a;
-    int was = -127;
+    uint32_t was = 0;
     if (mine) {
       const __nv_bfloat16* src = s.src + (t0 - 1 + j) * s.s0;
       a = *reinterpret_cast<const uint4*>(src + 8 * s.lt.ga);
       b = *reinterpret_cast<const uint4*>(src + 8 * s.lt.gb);
-      if (row) was = (int)(*reinterpret_cast<const uint32_t*>(tile + 16 * D) >> 23 & 255u) - 127;
+      if (row) was = *reinterpret_cast<const uint32_t*>(tile + 16 * D);
     }
     if (ROT && turned && mine && s.lt.kind) {
       Angles an;
@@ -253,7 +256,7 @@ __device__ __forceinline__ void write_singles(const B8WriteParams& p, const B8Si
       const TileScale sc = tile_scale<INT8>(s.g, amax, row == 0, was);
       if (row && sc.e > sc.old) recode_rows<D, INT8>(s, tile, 1u << row, sc.e - sc.old, 0, 1);
       store_row<D, INT8>(s, tile, row, a, b, to_code(s.g, sc.e), sc.inf);
-      if ((threadIdx.x & (LPR - 1)) == 0 && sc.e != was) *reinterpret_cast<uint32_t*>(tile + 16 * D) = (uint32_t)(sc.e + 127) << 23;
+      if ((threadIdx.x & (LPR - 1)) == 0 && sc.word() != was) *reinterpret_cast<uint32_t*>(tile + 16 * D) = sc.word();
     }
     __syncwarp();
 #pragma unroll
@@ -267,7 +270,7 @@ __device__ __forceinline__ void write_singles(const B8WriteParams& p, const B8Si
 // A few rows (RPP: as many as the warp's lanes have at a time), of drafts and prompts' ends: in registers.
 template <int D, bool INT8, bool ROT>
 __device__ __forceinline__ void write_few(const B8Side<D>& s, const RotaryParams& r, bool turned, int tok, int angle, unsigned named,
-                                          uint8_t* tile, int was) {
+                                          uint8_t* tile, uint32_t was) {
   constexpr int RPP = 512 / D;
   unsigned m = named;
 #pragma unroll
@@ -289,7 +292,7 @@ __device__ __forceinline__ void write_few(const B8Side<D>& s, const RotaryParams
   const TileScale sc = tile_scale<INT8>(s.g, warp_largest(largest(largest(__floats2bfloat162_rn(0.0f, 0.0f), a), b)), named & 1u, was);
   if (!(named & 1u) && sc.e > sc.old) recode_rows<D, INT8>(s, tile, named, sc.e - sc.old, s.rr, RPP);
   if (mine) store_row<D, INT8>(s, tile, row, a, b, to_code(s.g, sc.e), sc.inf);
-  if ((threadIdx.x & 31) == 0 && sc.e != was) *reinterpret_cast<uint32_t*>(tile + 16 * D) = (uint32_t)(sc.e + 127) << 23;
+  if ((threadIdx.x & 31) == 0 && sc.word() != was) *reinterpret_cast<uint32_t*>(tile + 16 * D) = sc.word();
 }
 
 // More rows go through the warp's 16 rows of shared memory: a lane copies what it alone works on, all rows at once, so that a warp has 4
@@ -297,7 +300,7 @@ __device__ __forceinline__ void write_few(const B8Side<D>& s, const RotaryParams
 // known, the codes. `copies`: the angles are still being copied (every warp of the CTA comes by here then).
 template <int D, bool INT8, bool ROT>
 __device__ __forceinline__ void write_tile(const B8Side<D>& s, const RotaryParams& r, bool turned, const uint8_t* angles, bool& copies,
-                                           uint8_t* rows, int tok, int angle, unsigned named, uint8_t* tile, int was) {
+                                           uint8_t* rows, int tok, int angle, unsigned named, uint8_t* tile, uint32_t was) {
   constexpr int RPP = 512 / D;
   uint8_t* const my = rows + s.rr * (2 * D);         // this lane's row of the first ones; its groups lie at 16 * ga and 16 * gb
   auto any = [&](int i) { return (named >> i & ((1u << RPP) - 1)) != 0; };    // (i: first row of a pass)
@@ -343,7 +346,7 @@ __device__ __forceinline__ void write_tile(const B8Side<D>& s, const RotaryParam
     if (named >> (i + s.rr) & 1u)
       store_row<D, INT8>(s, tile, i + s.rr, *reinterpret_cast<const uint4*>(my + i * (2 * D) + 16 * s.lt.ga),
                          *reinterpret_cast<const uint4*>(my + i * (2 * D) + 16 * s.lt.gb), tc, sc.inf);
-  if ((threadIdx.x & 31) == 0 && sc.e != was) *reinterpret_cast<uint32_t*>(tile + 16 * D) = (uint32_t)(sc.e + 127) << 23;
+  if ((threadIdx.x & 31) == 0 && sc.word() != was) *reinterpret_cast<uint32_t*>(tile + 16 * D) = sc.word();
 }
 template <int D>
 constexpr int b8_write_smem(bool rot, int warps) { return (rot ? 32 * 4 * D : 0) + warps * 32 * D; }
@@ -438,7 +441,7 @@ __global__ void __launch_bounds__(256, FEW || D == 256 ? 3 : 4) b8_write_kernel(
       if (lane >= 16) tok = -1;
     }
     const unsigned named = __ballot_sync(0xffffffffu, tok >= 0);
-    const int was = named & 1u ? -127 : (int)(was_bits >> 23 & 255u) - 127;
+    const uint32_t was = named & 1u ? 0 : was_bits;
     if (FEW && __popc(named) <= 512 / D) write_few<D, INT8, ROT>(s, r, ROT && !side, tok, ang, named, t_, was);
     else write_tile<D, INT8, ROT>(s, r, ROT && !side, angles, copies, rows, tok, ang, named, t_, was);
     __syncwarp();

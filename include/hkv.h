@@ -371,7 +371,8 @@ int hkv_write_rotary(const void* key, const void* val, int64_t ks0, int64_t ks1,
  *                A slot that is named twice in a run takes the last of its tokens. A call that names a tile's first token begins the
  *                tile anew: its other rows are whatever they are until they are written. Any other call keeps the tile's rows:
  *                the scale is the larger one of its own and the smallest 2^e with |x / g| <= 2^e * 448 (int8: 127),
- *                HKV_B8_*_MIN <= e <= HKV_B8_*_MAX, and where it grows, the rows that the call does not name are rounded to it. Codes
+ *                HKV_B8_*_MIN <= e <= HKV_B8_*_MAX, and where it grows, the rows that the call does not name are rounded to it (of a
+ *                word that no call has left there, the exponent counts, within these bounds, and a power of two takes its place). Codes
  *                are rounded to nearest even; what is beyond the largest one takes that, a NaN stays one (int8: 0) and does not
  *                count for the scale. rotary: turns keys and queries first, or NULL
  * hkv_decode_b8  hkv_decode_window over this cache (window 0 and lse NULL: hkv_decode); the workspace is hkv_decode's, and the same one
