@@ -73,3 +73,39 @@ def test_order_of_a_tile_s_tokens(fmt, D, KVH, HQ, rot, interleaved, dtype, kind
         check_queries(out, q.cpu(), pos, t, interleaved)
         cache = R.append(cache, R.turn(k.cpu(), pos, t, interleaved), v.cpu(), slots.tolist(), one, one, fmt)
         same(view.cpu(), cache, fmt)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("turned", [False, True])
+@pytest.mark.parametrize("D,KVH", [(128, 1), (128, 4), (128, 5), (256, 2), (256, 7)])
+@pytest.mark.parametrize("n", [700, 2100, 8200])
+def test_large_batches_of_every_kind(fmt, turned, D, KVH, n):
+    """prompts from and to the middle of a tile, drafts, single tokens, repeated and shuffled rows and skipped tokens in one call, for heads of
+    one CTA and of several; the second call grows the scales of the first one's tiles. What is without a slot at the end stays unread"""
+    PS, HQ = 64, KVH
+    cache = fresh(n // 6 + 20, KVH, PS, D, fmt, n + D)
+    one = torch.tensor([1.0, 0.5, 2.0, 0.37, 4.0, 1.0, 1.0])[:KVH]
+    view, _ = put(cache)
+    flat, st = Lt.b8_views(view, KVH, D)
+    t = table(300, D, torch.float32)
+    for step in range(2):
+        slots, tiles = slots_of("mixed", n // 2, n // 2, n + step), torch.arange(n // 2, n) * 16
+        prompts, at = [], 0                                             # of 17 to 400 tokens, each in tiles of its own
+        while sum(map(len, prompts)) < n - n // 2:
+            m, first = int(torch.randint(17, 400, (1,), generator=gen(n + at))), int(torch.randint(0, 16, (1,), generator=gen(n + at + 1)))
+            prompts.append(int(tiles[at]) + first + torch.arange(m))
+            at += (first + m + 15) // 16
+        slots = torch.cat((slots, *prompts))[:n]
+        assert int(slots.max()) < len(cache) * PS
+        pos = torch.randint(0, 300, (n + 3,), generator=gen(n + step))
+        x = qkv(n + 3, HQ, KVH, D, n + 3 * step)
+        x *= 2.0 ** (torch.randint(-3, 4, (n + 3, 1), generator=gen(n + 5 * step)) + step).to(torch.bfloat16)
+        q, k, v = parts(x.cuda(), HQ, KVH, D)
+        if turned:
+            out = torch.zeros(n + 3, HQ, D, dtype=torch.bfloat16, device="cuda")
+            K.write_rotary_b8(q, k, v, flat, st, PS, slots.cuda(), pos.cuda(), t.cuda(), one.cuda(), one.cuda(), out, fmt=fmt)
+            check_queries(out, q.cpu(), pos, t, False)
+        else:
+            K.write_b8(k, v, flat, st, PS, slots.cuda(), one.cuda(), one.cuda(), fmt=fmt)
+        cache = R.append(cache, R.turn(k.cpu(), pos, t, False) if turned else k.cpu(), v.cpu(), slots.tolist(), one, one, fmt)
+        same(view.cpu(), cache, fmt)
