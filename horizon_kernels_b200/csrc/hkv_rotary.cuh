@@ -254,7 +254,8 @@ inline int rotary_params(const hkv_rotary* u, int D, int64_t n_slots, const void
   const int64_t n = u->n_tokens, q_span = (u->HQ - 1) * u->qs1 + D, o_span = (u->HQ - 1) * u->os1 + D;
   // rows that are written must not overlap one another, nor what else is read
   if (!rows_apart((int)n, u->HQ, D, u->os0, u->os1)) return HKV_ERR_RANGE;
-  const bool same = u->query == u->query_out && u->qs0 == u->os0 && u->qs1 == u->os1;
+  // (a stride between one row and no other says nothing)
+  const bool same = u->query == u->query_out && (n < 2 || u->qs0 == u->os0) && (u->HQ < 2 || u->qs1 == u->os1);
   if (!same && !rows_disjoint(u->query, u->qs0, q_span, n, u->query_out, u->os0, o_span, n)) return HKV_ERR_RANGE;
   if (ks0 >= 0 && ks1 >= 0 && !rows_disjoint(key, ks0, (KVH - 1) * ks1 + D, n_slots, u->query_out, u->os0, o_span, n)) return HKV_ERR_RANGE;
   if (vs0 >= 0 && vs1 >= 0 && !rows_disjoint(val, vs0, (KVH - 1) * vs1 + D, n_slots, u->query_out, u->os0, o_span, n)) return HKV_ERR_RANGE;

@@ -172,7 +172,8 @@ def _rotary(query, key, value, slot_mapping, positions, cos_sin, query_out, inte
     _need_cuda(query, positions, cos_sin, query_out)
     _one_device(key, query, positions, cos_sin, query_out)
     for a in (query, key, value) if NT else ():
-        same = a is query and a.data_ptr() == query_out.data_ptr() and a.stride() == query_out.stride()
+        same = a is query and a.data_ptr() == query_out.data_ptr() and all(
+            n < 2 or s == o for n, s, o in zip(a.shape, a.stride(), query_out.stride()))
         if not same and not _rows_apart(a, query_out):
             raise ValueError("query_out is neither the query itself nor apart from query, key and value")
     return _lib.Rotary(query.data_ptr(), query.stride(0), query.stride(1), query_out.data_ptr(), query_out.stride(0),

@@ -1,0 +1,57 @@
+"""Queries turned where they lie: under other views of the same rows. Every entry point, natively and through ctypes."""
+import pytest
+import torch
+
+import b8_ref as R
+from horizon_kernels_b200 import _lib
+from horizon_kernels_b200 import kernels as K
+from horizon_kernels_b200 import layout as Lt
+from test_b8_gpu import fresh, same
+from test_rotary_gpu import cache_of, check_queries, gen, table
+
+pytestmark = pytest.mark.gpu
+
+
+def in_place(x, query, key, value, out, b8, interleaved=False):
+    """one call whose query_out lies on the query; `x` holds all three. Queries, cache and the rest of x as the definition says"""
+    (NT, HQ, D), KVH, PS = query.shape, key.shape[1], 16
+    t, pos, slots = table(400, D, torch.float32), torch.arange(NT) * 3 + 1, torch.arange(NT) + 5
+    g = torch.full((KVH,), 0.01)
+    before, q0, k0, v0 = x.cpu(), query.cpu(), key.cpu(), value.cpu()
+    for host in (None, _lib._NoHost()):
+        x.copy_(before)
+        args = slots.cuda(), pos.cuda(), t.cuda(), g.cuda(), g.cuda(), out
+        was, _lib._host = _lib._host, host or _lib._host
+        try:
+            if b8:
+                start = fresh(NT // PS + 2, KVH, PS, D, b8, 4)
+                cache = start.cuda()
+                flat, st = Lt.b8_views(cache, KVH, D)
+                K.write_rotary_b8(query, key, value, flat, st, PS, *args, interleaved=interleaved, fmt=b8)
+                same(cache, R.append(start, R.turn(k0, pos, t, interleaved), v0, slots.tolist(), g, g, b8), b8)
+            else:
+                phys, flat, st = cache_of("slot", NT // PS + 2, PS, KVH, D, False)
+                ref, flat_r, _ = cache_of("slot", NT // PS + 2, PS, KVH, D, False)
+                K.write_rotary(query, key, value, flat, st, PS, *args, interleaved=interleaved)
+                K.write(R.turn(k0, pos, t, interleaved).cuda(), v0.cuda(), flat_r, st, PS, args[0], args[3], args[4])
+                assert torch.equal(phys, ref)
+        finally:
+            _lib._host = was
+        check_queries(query, q0, pos, t, interleaved)
+        assert torch.equal(key.cpu(), k0) and torch.equal(value.cpu(), v0)
+        query.copy_(q0)
+        assert torch.equal(x.cpu(), before)                             # nothing beside the queries was written
+
+
+@pytest.mark.parametrize("b8", [None, "e4m3", "int8"])
+@pytest.mark.parametrize("NT,HQ", [(1, 8), (1, 1), (9, 1)])
+def test_strides_of_single_rows(b8, NT, HQ):
+    """one token, or one head: strides that differ where there is nothing to stride over"""
+    D, KVH = 128, 1
+    W = (HQ + 2 * KVH) * D
+    x = torch.randn(NT, W, generator=gen(HQ)).to(torch.bfloat16).cuda()
+    q = x.as_strided((NT, HQ, D), (W, D, 1))
+    out = x.as_strided((NT, HQ, D), (W if NT > 1 else HQ * D, D if HQ > 1 else 5 * D, 1))
+    assert q.stride() != out.stride()
+    k, v = (x[:, (HQ + i) * D:(HQ + i + 1) * D].view(NT, 1, D) for i in range(2))
+    in_place(x, q, k, v, out, b8)
