@@ -5,6 +5,9 @@
 
 #include <cuda_bf16.h>
 
+#include <initializer_list>
+#include <numeric>
+
 #include "hkv_common.cuh"
 #include "hkv_f32x2.cuh"
 
@@ -230,17 +233,32 @@ inline long long with_queries(RotaryParams& r, int D, long long blocks, int thre
 }
 
 // ----------------------------------------------------------------------------------------------------- host side
-// whether two sets of rows (row i < n at base + i * s0, `span` elements from there on) have no byte in common: apart as a whole, or
-// columns of the same rows
-inline bool rows_disjoint(const void* a, int64_t a0, int64_t a_span, int64_t na, const void* b, int64_t b0, int64_t b_span, int64_t nb) {
-  const uintptr_t pa = (uintptr_t)a, pb = (uintptr_t)b;
-  if (na < 1 || nb < 1) return true;
-  if (pa + 2 * (uint64_t)((na - 1) * a0 + a_span) <= pb || pb + 2 * (uint64_t)((nb - 1) * b0 + b_span) <= pa) return true;
-  if (a0 != b0 || a0 < 1) return false;
+// rows of D 16-bit numbers: row (i, h), i < n, h < heads, at p + 2 * (i * s0 + h * s1) bytes
+struct RowSet {
+  const void* p;
+  int64_t s0, s1, n, heads;
+};
+// Whether two sets of rows have no byte in common, by one of three rules: they lie apart as a whole; they are columns of the same long rows
+// (queries and keys of a fused product); or they are columns of something smaller (heads of queries, keys and values in turn): every
+// stride is a multiple of g, and modulo g a row of one set lies beside a row of the other.
+inline bool rows_disjoint(const RowSet& a, const RowSet& b, int64_t D) {
+  if (a.n < 1 || b.n < 1) return true;
+  const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+  const int64_t a_span = (a.heads - 1) * a.s1 + D, b_span = (b.heads - 1) * b.s1 + D;
+  if (pa + 2 * (uint64_t)((a.n - 1) * a.s0 + a_span) <= pb || pb + 2 * (uint64_t)((b.n - 1) * b.s0 + b_span) <= pa) return true;
   const bool first = pa <= pb;
-  const uint64_t off = (first ? pb - pa : pa - pb) % (2 * (uint64_t)a0);
-  const int64_t lo_span = first ? a_span : b_span, hi_span = first ? b_span : a_span;
-  return off >= 2 * (uint64_t)lo_span && off + 2 * (uint64_t)hi_span <= 2 * (uint64_t)a0;
+  const uint64_t apart = first ? pb - pa : pa - pb;
+  auto beside = [apart](int64_t m, int64_t lo_span, int64_t hi_span) {
+    const uint64_t off = apart % (2 * (uint64_t)m);
+    return off >= 2 * (uint64_t)lo_span && off + 2 * (uint64_t)hi_span <= 2 * (uint64_t)m;
+  };
+  if (a.s0 == b.s0 && a.s0 > 0 && beside(a.s0, first ? a_span : b_span, first ? b_span : a_span)) return true;
+  int64_t g = 0;
+  for (const RowSet* r : {&a, &b}) {
+    if (r->n > 1) g = std::gcd(g, r->s0);
+    if (r->heads > 1) g = std::gcd(g, r->s1);
+  }
+  return g > 0 && beside(g, D, D);
 }
 // checks a caller's hkv_rotary; keys and values (n tokens of KVH heads) must not be where the queries go
 inline int rotary_params(const hkv_rotary* u, int D, int64_t n_slots, const void* key, int64_t ks0, int64_t ks1, const void* val,
@@ -251,14 +269,15 @@ inline int rotary_params(const hkv_rotary* u, int D, int64_t n_slots, const void
   if (u->qs0 < 0 || u->qs1 < 0 || u->os0 < 0 || u->os1 < 0) return HKV_ERR_RANGE;
   if (((uintptr_t)u->query | (uintptr_t)u->query_out | (uintptr_t)u->table) & 15) return HKV_ERR_ALIGN;
   if (((uintptr_t)u->positions & 7) || ((u->qs0 | u->qs1 | u->os0 | u->os1) & 7)) return HKV_ERR_ALIGN;
-  const int64_t n = u->n_tokens, q_span = (u->HQ - 1) * u->qs1 + D, o_span = (u->HQ - 1) * u->os1 + D;
+  const int64_t n = u->n_tokens;
+  const RowSet out{u->query_out, u->os0, u->os1, n, u->HQ};
   // rows that are written must not overlap one another, nor what else is read
   if (!rows_apart((int)n, u->HQ, D, u->os0, u->os1)) return HKV_ERR_RANGE;
   // (a stride between one row and no other says nothing)
   const bool same = u->query == u->query_out && (n < 2 || u->qs0 == u->os0) && (u->HQ < 2 || u->qs1 == u->os1);
-  if (!same && !rows_disjoint(u->query, u->qs0, q_span, n, u->query_out, u->os0, o_span, n)) return HKV_ERR_RANGE;
-  if (ks0 >= 0 && ks1 >= 0 && !rows_disjoint(key, ks0, (KVH - 1) * ks1 + D, n_slots, u->query_out, u->os0, o_span, n)) return HKV_ERR_RANGE;
-  if (vs0 >= 0 && vs1 >= 0 && !rows_disjoint(val, vs0, (KVH - 1) * vs1 + D, n_slots, u->query_out, u->os0, o_span, n)) return HKV_ERR_RANGE;
+  if (!same && !rows_disjoint({u->query, u->qs0, u->qs1, n, u->HQ}, out, D)) return HKV_ERR_RANGE;
+  if (ks0 >= 0 && ks1 >= 0 && !rows_disjoint({key, ks0, ks1, n_slots, KVH}, out, D)) return HKV_ERR_RANGE;
+  if (vs0 >= 0 && vs1 >= 0 && !rows_disjoint({val, vs0, vs1, n_slots, KVH}, out, D)) return HKV_ERR_RANGE;
   r->q = (const __nv_bfloat16*)u->query;
   r->out = (__nv_bfloat16*)u->query_out;
   r->qs0 = u->qs0; r->qs1 = u->qs1; r->os0 = u->os0; r->os1 = u->os1;

@@ -6,6 +6,7 @@ The wrappers only marshal pointers, sizes and the current CUDA stream into the C
 They never synchronise and allocate nothing (prefill: its scratch, from torch's allocator), so calls can be captured in
 a CUDA graph. There is no CPU or PyTorch fallback."""
 import ctypes as C
+import math
 
 import torch
 
@@ -182,17 +183,22 @@ def _rotary(query, key, value, slot_mapping, positions, cos_sin, query_out, inte
 
 
 def _rows_apart(a, b):
-    """whether two (tokens, heads, head_dim) tensors have no element in common: apart as a whole, or columns of the same rows"""
-    span = [(t.shape[1] - 1) * t.stride(1) + t.shape[2] for t in (a, b)]
-    end = [t.data_ptr() + 2 * ((t.shape[0] - 1) * t.stride(0) + s) for t, s in zip((a, b), span)]
+    """whether two (tokens, heads, head_dim) tensors have no element in common: apart as a whole, columns of the same rows, or heads beside
+    one another (every stride a multiple of one length, within which a head of one lies beside a head of the other)"""
+    D, size = a.shape[2], a.element_size()
+    span = [(t.shape[1] - 1) * t.stride(1) + D for t in (a, b)]
+    end = [t.data_ptr() + size * ((t.shape[0] - 1) * t.stride(0) + s) for t, s in zip((a, b), span)]
     if end[0] <= b.data_ptr() or end[1] <= a.data_ptr():
         return True
-    if a.stride(0) != b.stride(0) or a.stride(0) < 1:
-        return False
-    first = a.data_ptr() <= b.data_ptr()
-    off = abs(b.data_ptr() - a.data_ptr()) % (2 * a.stride(0))
-    lo, hi = span if first else span[::-1]
-    return off >= 2 * lo and off + 2 * hi <= 2 * a.stride(0)
+    first, apart = a.data_ptr() <= b.data_ptr(), abs(b.data_ptr() - a.data_ptr())
+
+    def beside(m, lo, hi):
+        off = apart % (size * m)
+        return off >= size * lo and off + size * hi <= size * m
+    if a.stride(0) == b.stride(0) and a.stride(0) > 0 and beside(a.stride(0), *(span if first else span[::-1])):
+        return True
+    g = math.gcd(*[t.stride(i) for t in (a, b) for i in (0, 1) if t.shape[i] > 1])
+    return g > 0 and beside(g, D, D)
 
 
 def write_rotary(query, key, value, flat, strides, PS, slot_mapping, positions, cos_sin, gk, gv, query_out, interleaved=False,

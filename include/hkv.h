@@ -333,7 +333,7 @@ int hkv_evict(void* kd, void* ksf, void* vd, void* vsf, const int64_t strides[6]
  * counterpart in the reference, whose model rotates in a launch before its write.
  *   query       bf16 (n_tokens, HQ, D), element strides qs0 (token) and qs1 (head), rows of D contiguous and 16-byte aligned
  *   query_out   the turned rows, strides os0, os1: the query itself (the same address and strides), or rows that lie apart from the
- *               query's, the keys' and the values' (columns of the same rows are apart)
+ *               query's, the keys' and the values' (columns of the same rows are apart, heads in turn too)
  *   positions   int64[n_tokens], n_tokens >= n_slots: token i's slot is slots[i]; tokens from n_slots on, or with a negative slot,
  *               have their queries turned and nothing else. A position outside the table takes the nearest row
  *   table       (rows, rot) contiguous, 16-byte aligned, fp32 or (table_bf16) bf16: rot / 2 cosines, then as many sines

@@ -55,3 +55,12 @@ def test_strides_of_single_rows(b8, NT, HQ):
     assert q.stride() != out.stride()
     k, v = (x[:, (HQ + i) * D:(HQ + i + 1) * D].view(NT, 1, D) for i in range(2))
     in_place(x, q, k, v, out, b8)
+
+
+@pytest.mark.parametrize("b8", [None, "e4m3", "int8"])
+@pytest.mark.parametrize("NT,H,interleaved", [(1, 2, False), (21, 4, False), (40, 3, True)])
+def test_heads_of_queries_keys_and_values_in_turn(b8, NT, H, interleaved):
+    """(tokens, heads, 3, head_dim), as a fused product may leave them"""
+    D = 128
+    x = torch.randn(NT, H, 3, D, generator=gen(H)).to(torch.bfloat16).cuda()
+    in_place(x, x[:, :, 0], x[:, :, 1], x[:, :, 2], x[:, :, 0], b8, interleaved)
