@@ -2,6 +2,9 @@
 bounded cache: `decode_window`, `prefill_window`, `accumulate_weights`, `evict`, the write that rotates (`write_rotary`) and those of the
 8-bit cache: `write_b8`, `write_rotary_b8`, `decode_b8`, `prefill_b8`.
 
+`write_rotary` and `write_rotary_b8` take the query as their query_out too, as torch's own ops take an input as out=: their schemas
+name query_out as what is written. A front end that gives mutated arguments as copies turns the copy, from the query as it was.
+
 The ops are thin: they pass the tensors' device pointers, the strides and the current CUDA stream to `libhkv.so`
 (include/hkv.h) and mutate their output arguments in place, like the reference's TileLang-launched kernels mutate the
 cache and the output buffer (kv_fp4_serving.py:994-1005, :894-915 in the reference). Registering them with torch lets

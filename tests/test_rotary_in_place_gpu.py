@@ -1,4 +1,5 @@
-"""Queries turned where they lie: under other views of the same rows. Every entry point, natively and through ctypes."""
+"""Queries turned where they lie: under other views of the same rows, among the heads of keys and values, through the custom
+ops. Every entry point, natively and through ctypes."""
 import pytest
 import torch
 
@@ -6,8 +7,9 @@ import b8_ref as R
 from horizon_kernels_b200 import _lib
 from horizon_kernels_b200 import kernels as K
 from horizon_kernels_b200 import layout as Lt
+from horizon_kernels_b200 import ops
 from test_b8_gpu import fresh, same
-from test_rotary_gpu import cache_of, check_queries, gen, table
+from test_rotary_gpu import cache_of, check_queries, gen, parts, table
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +66,26 @@ def test_heads_of_queries_keys_and_values_in_turn(b8, NT, H, interleaved):
     D = 128
     x = torch.randn(NT, H, 3, D, generator=gen(H)).to(torch.bfloat16).cuda()
     in_place(x, x[:, :, 0], x[:, :, 1], x[:, :, 2], x[:, :, 0], b8, interleaved)
+
+
+@pytest.mark.parametrize("b8", [None, "int8"])
+def test_custom_ops_in_place(b8):
+    """query_out may be the query, as an out= argument may be an input"""
+    hkv = ops.register()
+    D, KVH, HQ, PS, NT = 128, 2, 6, 16, 30
+    x = torch.randn(NT, (HQ + 2 * KVH) * D, generator=gen(1)).to(torch.bfloat16).cuda()
+    q, k, v = parts(x, HQ, KVH, D)
+    t, pos, slots = table(200, D, torch.float32).cuda(), torch.arange(NT).cuda() * 5, torch.arange(NT).cuda()
+    g, q0 = torch.full((KVH,), 0.02, device="cuda"), q.cpu()
+    got = []
+    for out in (torch.zeros(NT, HQ, D, dtype=torch.bfloat16, device="cuda"), q):
+        if b8:
+            cache = torch.zeros((2, 2 * KVH, PS, D + 1), dtype=torch.uint8, device="cuda")
+            flat, st = Lt.b8_views(cache, KVH, D)
+            hkv.write_rotary_b8(q, k, v, *flat, list(st), PS, slots, pos, t, g, g, False, b8, out)
+        else:
+            cache, flat, st = cache_of("slot", 2, PS, KVH, D, False)
+            hkv.write_rotary(q, k, v, *flat, list(st), PS, slots, pos, t, g, g, False, True, None, False, out)
+        check_queries(out, q0, pos.cpu(), t.cpu(), False)
+        got.append(cache)
+    assert torch.equal(*got) and torch.equal(q.cpu(), out.cpu())
