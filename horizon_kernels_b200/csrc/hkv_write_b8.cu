@@ -485,10 +485,17 @@ extern "C" int hkv_write_b8(const void* key, const void* val, int64_t ks0, int64
   p.n = (int)n_slots; p.KVH = KVH;
   p.lps = 0;
   while ((1 << p.lps) < PS) ++p.lps;
-  // tokens of a set: one where a CTA each is done at once, more where most of their CTAs would find nothing to begin (a prompt's) or few
-  // tiles at a time (single tokens). 8 kv heads x 128, 1 / 4 / 8 / 16 tokens a set: 1024 single tokens 6.9 / 3.8 / 3.6 / 9.0 us, a
-  // prompt of 4096 - / 9.4 / 8.0 / 6.7; 512 tokens in pairs, 2 x 256: 2.7 / 4.1 / 6.4 / -
-  p.per = n_slots <= 512 ? 1 : n_slots < 2048 ? 4 : n_slots < 8192 ? 8 : 16;
+  // Tokens of a set. A set of one has a warp for each of its tokens' rows, which is best while the GPU holds these warps at once (148 SMs
+  // with three CTAs of eight); larger sets leave fewer warps without a tile to begin, and take several tiles of single tokens at a time.
+  // us at 1 / 4 / 8 tokens a set, e4m3, caches larger than the L2, rows = 2 * KVH * tokens:
+  //   2 x 256, rotating, 512 tokens (2048 rows) single 6.1 / 5.4 / 7.8, in pairs 6.1 / 6.7 / 10.1
+  //   8 x 128, rotating, 256 tokens (4096) single 6.1 / 3.7 / 4.9, in pairs 5.1 / 6.0 / 9.0; 512 (8192) 9.0 / 4.5 / 5.8, 7.9 / 7.1 / 10.7
+  //   2 x 256, 1024 tokens (4096) in pairs 4.4 / 5.2 / 7.8; 3000 (12000) 8.4 / 5.9 / 8.4; 4096 (16384) 10.4 / 9.3 / 9.0
+  //   8 x 128, 1536 tokens (24576) of a prompt 11.1 / 6.4 / 5.8; 1 x 128, 4096 (8192) in drafts of four 6.3 / 3.7 / 5.2
+  // From 8192 tokens on a call is of prompts: sets of 16, in whose kernel the keys' angles are copied once for all heads. There 8 / 16 tokens a
+  // set take 39 / 34 (a prompt of 8192 tokens, 8 x 128, rotating) and 15.6 / 13.3 (not rotating), but 46 / 103 were they all single.
+  const int64_t rows = n_slots * 2 * KVH, at_once = 148 * 24;
+  p.per = n_slots >= 8192 ? 16 : rows <= at_once ? 1 : rows <= 4 * at_once ? 4 : 8;
   const int warps = 2 * KVH < 8 ? 2 * KVH : 8;
   p.groups = (unsigned)((2 * KVH + warps - 1) / warps);
   const long long blocks = (n_slots + p.per - 1) / p.per * p.groups;
