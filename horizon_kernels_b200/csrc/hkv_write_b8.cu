@@ -7,9 +7,10 @@
 // E4M3 code nothing but its last subnormal bits.
 //
 // What bounds it: the chain of latencies of a tile (slots, rows, the largest of them, stores) over the warps that an SM holds, and the
-// instructions of the rotation. B200, 8 kv heads x 128, back to back: 17108 tokens of twelve prompts 25 us (4.2 TB/s), with the
+// instructions of the rotation. B200, 8 kv heads x 128, back to back: 17108 tokens of twelve prompts 24 us (4.4 TB/s), with the
 // rotation of the keys and 32 query heads 69 us (5.7 TB/s; the queries alone take 44); four single tokens 1.9 and 2.4 us. With the rows
 // in registers instead of shared memory a key warp took 128 of them: 97 us for the prompts; angles from global memory for every head: the same.
+// Without a rotation a prompt's floor is 16 us, and a warp has one tile on its way at a time: rows, the largest magnitude, codes.
 #include <cuda_fp8.h>
 
 #include "hkv_common.cuh"
@@ -348,11 +349,13 @@ __device__ __forceinline__ void write_tile(const B8Side<D>& s, const RotaryParam
                          *reinterpret_cast<const uint4*>(my + i * (2 * D) + 16 * s.lt.gb), tc, sc.inf);
   if ((threadIdx.x & 31) == 0 && sc.word() != was) *reinterpret_cast<uint32_t*>(tile + 16 * D) = sc.word();
 }
+// The first part, 32 rows of angles, is for the kernels of sets of 16 tokens. Those of smaller sets read angles where they need them and leave
+// it unused, which costs them CTAs: at head_dim 256 with eight warps 96 KB allow two an SM where 64 would allow three.
 template <int D>
 constexpr int b8_write_smem(bool rot, int warps) { return (rot ? 32 * 4 * D : 0) + warps * 32 * D; }
 
-// A CTA has the tiles that begin with one of `per` neighbouring tokens, of up to eight kv heads and sides: a warp for each. The keys'
-// angles are copied into shared memory, once for all of its heads, while the rows are on their way.
+// A CTA has the tiles that begin with one of `per` neighbouring tokens, of up to eight kv heads and sides: a warp for each. In sets of 16
+// (FEW false) the keys' angles are copied into shared memory, once for all of its heads, while the rows are on their way.
 template <int D, bool INT8, bool ROT, bool FEW>
 __global__ void __launch_bounds__(256, FEW || D == 256 ? 3 : 4) b8_write_kernel(const B8WriteParams p, const RotaryParams r) {
   constexpr int LPR = D / 16;                        // lanes of a row
